@@ -4,7 +4,8 @@
  *
  * Conventions
  *   - All tensors are fp32 (flags uint8, indices int32/int64), device
- *     pointers, row-major, contiguous.  "B" is the number of domains
+ *     pointers, row-major, contiguous (the last section's entry points take
+ *     bf16 and row strides too).  "B" is the number of domains
  *     (boxes); "R" is the number of backward rows per domain (spec queries
  *     Q, or 2k seeded rows); a backward row m belongs to domain m / R.
  *   - Every call is asynchronous on the given HIP stream (hipStream_t passed
@@ -1115,6 +1116,74 @@ int vc_mlp_bab_round(const int32_t *dims, int n_relu, const float *frag,
                      vc_stream_t aux_stream, int32_t *stop_host,
                      int64_t *pinned, int64_t *counts, int32_t *fail_phase,
                      vc_stream_t stream);
+
+/* ---- The network itself: fc layers, loss, optimiser ------------------ */
+
+/* Types of a call's tensors, activations, reductions.  The tensors of the
+ * entry points below are of one of these types, row-major, rows `ld` values
+ * apart where an ld is given (contiguous where none is), at any alignment of
+ * their type.  Sums are held in fp32, results rounded once.  Workspaces are
+ * the caller's, of the bytes that the _workspace function gives for the same
+ * sizes (-1: refused); their contents need not be kept between calls. */
+#define VC_FP32 0
+#define VC_BF16 1
+#define VC_ACT_NONE 0
+#define VC_ACT_RELU 1
+#define VC_ACT_GELU 2 /* z (1 + erf(z / sqrt 2)) / 2 */
+#define VC_ACT_SILU 3 /* z / (1 + exp(-z)) */
+#define VC_REDUCE_NONE 0
+#define VC_REDUCE_SUM 1
+#define VC_REDUCE_MEAN 2
+
+/* y = act(z) + res, z = x W^T + bias: x (M, K), W (N, K), bias (N) or NULL,
+ * res (M, N) or NULL; y (M, N), and z (M, N) unless NULL.  y and z overlap
+ * nothing else. */
+int64_t vc_linear_workspace(int type, int64_t M, int K, int N);
+int vc_linear(int type, const void *x, int64_t M, int K, int64_t ldx,
+              const void *W, int N, const void *bias, int act,
+              const void *res, int64_t ldr, void *y, void *z, void *work,
+              int64_t work_bytes, vc_stream_t stream);
+
+/* Its gradients: dz = dy act'(z) (z is not read without an activation),
+ * dx = dz W (M, K), dW = dz^T x (N, K), db = column sums of dz (N), each
+ * unless NULL (need: 1 dx, 2 dW, 4 db).  In bf16 dz is rounded before the
+ * products, not before its sums. */
+int64_t vc_linear_backward_workspace(int type, int64_t M, int K, int N,
+                                     int act, int need);
+int vc_linear_backward(int type, const void *dy, int64_t ldy, const void *x,
+                       int64_t ldx, const void *W, const void *z, int64_t ldz,
+                       int act, int64_t M, int K, int N, void *dx, void *dW,
+                       void *db, void *work, int64_t work_bytes,
+                       vc_stream_t stream);
+
+/* Softmax cross-entropy of R rows of V logits with label smoothing e,
+ * loss = lse - (1 - e) z_t - e mean(z): per row (reduction none, loss (R)),
+ * summed, or averaged over the rows whose target is not `ignore` (loss (1);
+ * NaN where there is none).  dlogits, unless NULL, is the gradient of that
+ * loss (of each row's for none), of the logits' type; it may be the logits.
+ * Ignored rows: loss and gradient zero.  A target that is no class: NaN.
+ * A row without a logit above -inf: loss +inf, gradient zero. */
+int64_t vc_cross_entropy_workspace(int64_t R, int reduction);
+int vc_cross_entropy(int type, const void *logits, int64_t R, int64_t V,
+                     int64_t ld, const int64_t *target, int64_t ignore,
+                     float smoothing, int reduction, float *loss,
+                     void *dlogits, int64_t ldd, void *work,
+                     int64_t work_bytes, vc_stream_t stream);
+
+/* One AdamW step over `count` tensors: p, g and copy (or NULL, or NULL
+ * entries) are host arrays of device pointers, n of their sizes; p is of type
+ * ptype, g of gtype, copy receives the new p in bf16.  The state is two
+ * arrays for all tensors, each tensor padded to blocks of 256 values, 16-byte
+ * aligned: m and v in fp32 (bits 32), or m and sqrt(v) as e4m3 bytes with a
+ * scale per block in m_scale and v_scale (bits 8).  step counts from 1.
+ * scale (one device float, or NULL) multiplies the gradients; where it is not
+ * finite nothing is changed.  Same results for the same inputs. */
+int vc_adamw_step(const void *const *p, const void *const *g,
+                  const void *const *copy, const int64_t *n, int count,
+                  int ptype, int gtype, int bits, void *m, void *v,
+                  float *m_scale, float *v_scale, double lr, double b1,
+                  double b2, double eps, double weight_decay, int64_t step,
+                  const float *scale, vc_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,602 @@
+"""The fc layer forward and backward, the loss with its gradient and the AdamW
+step against plain 64-bit computations of the same formulas.
+
+Tolerances.  fp32 products: the parts left out are under 2^-22 of |x| |W|^T, each
+addition of a step's sum (one per 32 products, cut or rounded) under 2^-23 of it.
+bf16: one rounding of the result (2^-8 of it) above the same sums; a gradient that
+passes through a rounded dz, 2^-8 of |dz| |W| more.  Activations and slopes: a few
+units in the last place of fp32, 2^-20 of their argument's size.
+"""
+import math
+
+import pytest
+import torch
+
+from vibecheck_amd import train
+
+pytestmark = pytest.mark.gpu
+F32, F64, BF16 = torch.float32, torch.float64, torch.bfloat16
+
+
+def _randn(gpu, seed):
+    g = torch.Generator(device=gpu).manual_seed(seed)
+
+    def f(*shape, to=F32, std=1.0):
+        return (torch.randn(shape, generator=g, device=gpu) * std).to(to)
+    return f
+
+
+def _act(z, act):
+    return {None: z, 'relu': z.clamp(min=0), 'gelu': z * torch.special.ndtr(z),
+            'silu': z * torch.sigmoid(z)}[act]
+
+
+def _slope(z, act):
+    q = torch.sigmoid(z)
+    return {None: torch.ones_like(z), 'relu': (z > 0).double(),
+            'gelu': torch.special.ndtr(z) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi),
+            'silu': q + z * q * (1 - q)}[act]
+
+
+def _within(got, want, tol, what):
+    d = (got.double() - want).abs()
+    bad = ~(d <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float((d / tol.clamp(min=1e-300)).max()))
+
+
+def _close(got, want):
+    """The same computation by another kernel: sums in another order, one rounding more."""
+    rel = float((got.double() - want.double()).norm() / want.double().norm())
+    assert rel <= (2.0 ** -8 if got.dtype == BF16 else 1e-5), rel
+
+
+def _sum_tol(a, b, K):
+    """The products' own error of a sum over K: a, b are magnitudes (rows, K), (K, columns)."""
+    return (K / 16 + 16) * 2.0 ** -23 * (a @ b)
+
+
+# M, K, N
+SIZES = [(1, 1, 1), (1, 5, 50), (3, 64, 64), (1, 4096, 130), (17, 333, 65), (64, 128, 256),
+         (131, 203, 117), (129, 72, 513), (300, 8, 1000), (257, 1031, 40), (520, 784, 1024),
+         (2050, 512, 1030)]
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('M,K,N', SIZES)
+@pytest.mark.parametrize('act,res', [(None, True), ('relu', False), ('gelu', True), ('silu', False)])
+def test_linear(gpu, to, M, K, N, act, res):
+    f = _randn(gpu, M + 7 * K + 11 * N)
+    x, W, b = f(M, K, to=to), f(N, K, to=to, std=K ** -0.5), f(N, to=to)
+    r = f(M, N, to=to) if res else None
+    y, z = train.linear(x, W, b, act=act, residual=r, save=True)
+    zw = x.double() @ W.double().t() + b.double()
+    yw = _act(zw, act) + (r.double() if res else 0)
+    tol = _sum_tol(x.double().abs(), W.double().abs().t(), K) + 2.0 ** -20 * (zw.abs() + 1e-30)
+    tol = 1.2 * tol + 2.0 ** -20 * yw.abs()
+    half = 2.0 ** -8 if to == BF16 else 0.0
+    _within(y, yw, tol + half * yw.abs(), 'y')
+    if act and not (act == 'relu' and not res):
+        _within(z, zw, tol + half * zw.abs(), 'z')
+    elif act:
+        assert z is y
+    assert torch.equal(y, train.linear(x, W, b, act=act, residual=r))  # and again the same bits
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('M,K,N', SIZES)
+@pytest.mark.parametrize('act', [None, 'relu', 'gelu', 'silu'])
+def test_linear_backward(gpu, to, M, K, N, act):
+    f = _randn(gpu, 3 * M + 5 * K + N)
+    x, W, dy, z = f(M, K, to=to), f(N, K, to=to, std=K ** -0.5), f(M, N, to=to), f(M, N, to=to)
+    dx, dW, db = train.linear_backward(dy, x, W, z=z if act else None, act=act)
+    xd, Wd = x.double(), W.double()
+    dz = dy.double() * _slope(z.double(), act)
+    half = 2.0 ** -8 if to == BF16 else 0.0
+    e = dy.double().abs() * 2.0 ** -20 * (1 + z.double().abs())  # of dz
+    em = e + half * dz.abs()                                     # of dz in the products
+    for got, want, a, b, ea, K_ in (
+            (dx, dz @ Wd, dz.abs(), Wd.abs(), em @ Wd.abs(), N),
+            (dW, dz.t() @ xd, dz.abs().t(), xd.abs(), em.t() @ xd.abs(), M)):
+        _within(got, want, _sum_tol(a, b, K_) + ea + half * want.abs() + 1e-30, 'product')
+    want = dz.sum(0)
+    _within(db, want, M * 2.0 ** -24 * dz.abs().sum(0) + e.sum(0) + half * want.abs() + 1e-30, 'db')
+    again = train.linear_backward(dy, x, W, z=z if act else None, act=act)
+    assert all(torch.equal(p, q) for p, q in zip((dx, dW, db), again))
+    part = train.linear_backward(dy, x, W, z=z if act else None, act=act, need=('W',))
+    assert part[0] is None and part[2] is None and torch.equal(part[1], dW)
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+def test_linear_strides_and_alignment(gpu, to):
+    """Rows apart, bases off a 16-byte boundary, an expanded row, leading axes: the same results
+    as of contiguous copies."""
+    f = _randn(gpu, 5)
+    big, W, b = f(70, 200, to=to), f(96, 128, to=to, std=0.1), f(97, to=to)[1:]
+    wide = f(70, 300, to=to)
+    for off in (0, 1, 8):
+        x, r = big[:, off:off + 128], wide[:, off:off + 96]
+        y = train.linear(x, W, b, act='silu', residual=r)
+        _close(y, train.linear(x.contiguous(), W, b, act='silu', residual=r.contiguous()))
+        dy = wide[:, 100 + off:196 + off]
+        got = train.linear_backward(dy, x, W, z=r, act='gelu')
+        want = train.linear_backward(dy.contiguous(), x.contiguous(), W, z=r.contiguous(), act='gelu')
+        for p, q in zip(got, want):
+            _close(p, q)
+    x = big[:1, :128].expand(33, 128)
+    _close(train.linear(x, W), train.linear(x.contiguous(), W))
+    x = f(5, 7, 2, 128, to=to).transpose(0, 1)
+    y = train.linear(x, W, b)
+    assert y.shape == (7, 5, 2, 96)
+    _close(y.reshape(70, 96), train.linear(x.reshape(70, 128), W, b))
+    _close(train.linear(x[0, 0, 0], W, b), train.linear(x[0, 0, :1], W, b)[0])
+    Wt = f(128, 96, to=to).t()
+    _close(train.linear(big[:, :128], Wt), train.linear(big[:, :128], Wt.contiguous()))
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+def test_linear_empty(gpu, to):
+    f = _randn(gpu, 1)
+    W, b = f(6, 5, to=to), f(6, to=to)
+    assert train.linear(f(0, 5, to=to), W, b, act='relu').shape == (0, 6)
+    assert train.linear(f(3, 5, to=to), W[:0]).shape == (3, 0)
+    y = train.linear(f(3, 0, to=to), W[:, :0], b, act='relu')  # a sum of nothing
+    assert torch.equal(y, b.clamp(min=0).expand(3, 6))
+    dx, dW, db = train.linear_backward(f(0, 6, to=to), f(0, 5, to=to), W)
+    assert dx.shape == (0, 5) and not dW.any() and not db.any()
+    dx, dW, db = train.linear_backward(f(3, 0, to=to), f(3, 5, to=to), W[:0])
+    assert not dx.any() and dW.shape == (0, 5) and db.shape == (0,)
+    dx, dW, db = train.linear_backward(f(3, 6, to=to), f(3, 0, to=to), W[:, :0])
+    assert dx.shape == (3, 0) and dW.shape == (6, 0) and db.shape == (6,)
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('M,K,N', [(3, 40, 40), (200, 136, 130), (70, 2048, 66)])
+def test_linear_infinities_and_nan(gpu, to, M, K, N):
+    """An infinity or NaN reaches the results that the plain product lets it reach, and no others;
+    the largest finite values stay finite where their sums do."""
+    f = _randn(gpu, K)
+    x, W = f(M, K, to=to), f(N, K, to=to)
+    top = torch.finfo(to).max
+    W[:, 3], W[1, 3], W[2, 3] = 1.0, 0.0, -1.0
+    W[:, 4] = 0.0
+    x[0, 3], x[1, 3], x[2, 4] = math.inf, math.nan, top
+    W[0, 4] = 1.0
+    y = train.linear(x, W).double()
+    want = x.double() @ W.double().t()
+    assert torch.equal(y.isnan(), want.isnan())
+    inf = want.isinf()
+    assert torch.equal(y[inf], want[inf]) and bool(y[~inf & ~want.isnan()].isfinite().all())
+    assert abs(float(y[2, 0]) / top - 1) < 2.0 ** -7
+
+
+def test_linear_long_offsets(gpu):
+    """Rows past 2^32 values."""
+    K, M = 4096, (1 << 20) + 64
+    x = torch.zeros(M, K, dtype=BF16, device=gpu)
+    x[-1] = torch.arange(K, device=gpu) % 3 - 1
+    W = torch.ones(8, K, dtype=BF16, device=gpu)
+    W[1:, ::2] = 2
+    y = train.linear(x, W)
+    assert torch.equal(y[-1].double(), (x[-1:].double() @ W.double().t()).to(BF16)[0].double())
+    assert not y[:-1].any()
+    dW = train.linear_backward(y, x, W, need=('W',))[1]
+    want = (y[-1:].double().t() @ x[-1:].double()).to(BF16)
+    assert torch.equal(dW, want)
+
+
+def test_linear_autograd(gpu):
+    """The autograd form gives the explicit form's gradients, and they agree with differences of
+    the forward: h = 2^-5 leaves h^2 / 6 of the third derivative and 2^-22 |L| / h of rounding."""
+    f = _randn(gpu, 9)
+    x, W, b, r, up = f(40, 30), f(50, 30, std=0.3), f(50), f(40, 50), f(40, 50)
+    ts = [t.requires_grad_() for t in (x, W, b, r)]
+    y = train.linear(x, W, b, act='gelu', residual=r)
+    grads = torch.autograd.grad(y, ts, up)
+    with torch.no_grad():
+        _, z = train.linear(x, W, b, act='gelu', residual=r, save=True)
+        want = train.linear_backward(up, x, W, z=z, act='gelu') + (up,)
+        assert all(torch.equal(p, q) for p, q in zip(grads, want))
+        h = 2.0 ** -5
+        for i, t in enumerate(ts):
+            d = torch.randn(t.shape, device=gpu, generator=torch.Generator(device=gpu).manual_seed(i))
+            d /= d.norm()
+            side = []
+            for s in (h, -h):
+                at = [u + s * d if j == i else u for j, u in enumerate(ts)]
+                side.append((train.linear(at[0], at[1], at[2], act='gelu', residual=at[3]).double()
+                             * up.double()).sum())
+            num = float((side[0] - side[1]) / (2 * h))
+            assert abs(num - float((grads[i].double() * d.double()).sum())) < \
+                2e-3 * float(grads[i].double().norm())
+
+
+def test_linear_refusals(gpu):
+    x, W = torch.zeros(4, 8, device=gpu), torch.zeros(6, 8, device=gpu)
+    for bad in (lambda: train.linear(x, W[:, :7]), lambda: train.linear(x, W, torch.zeros(5, device=gpu)),
+                lambda: train.linear(x, W.bfloat16()), lambda: train.linear(x, W, act='sigmoid'),
+                lambda: train.linear(x, W, residual=x), lambda: train.linear(x, W.cpu()),
+                lambda: train.linear_backward(x, x, W), lambda: train.linear_backward(x[:, :6], x, W, act='relu'),
+                lambda: train.linear_backward(x[:, :6], x, W, need=('y',))):
+        with pytest.raises(ValueError):
+            bad()
+    for to in (torch.float64, torch.float16):
+        with pytest.raises(NotImplementedError):
+            train.linear(x.to(to), W.to(to))
+
+
+# ----------------------------------------------------------------------- loss
+
+def _loss64(z, t, e, ignore):
+    """Row losses and their gradients in 64 bits; masked rows as the operator defines them."""
+    z = z.double()
+    V = z.shape[1]
+    keep, none = t != ignore, (z == -math.inf).all(1)
+    ok = (t >= 0) & (t < V)
+    at = torch.where(ok, t, 0).unsqueeze(1)
+    z = z - z.amax(1, keepdim=True)  # large beside their differences: even 64 bits would cancel
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    loss = lse - (1 - e) * z.gather(1, at)
+    if e:
+        loss = loss - e * z.mean(1, keepdim=True)
+    d = torch.exp(z - lse) - e / V
+    d.scatter_add_(1, at, torch.full_like(lse, e - 1))
+    loss = torch.where(none, math.inf, loss[:, 0])
+    d = torch.where(none.unsqueeze(1), 0.0, d)
+    loss, d = torch.where(ok, loss, math.nan), torch.where(ok.unsqueeze(1), d, math.nan)
+    return torch.where(keep, loss, 0.0), torch.where(keep.unsqueeze(1), d, 0.0)
+
+
+def _check_loss(z, t, e=0.0, ignore=-100):
+    """Every reduction against 64 bits: the sums of V exponentials carry (20 + V / 64) units of
+    2^-24, the exponentials |z - max| units."""
+    R, V = z.shape
+    lw, dw = _loss64(z, t, e, ignore)
+    fin = torch.where(z.isfinite(), z.double(), 0.0)
+    span = (fin.amax(1) - fin.amin(1)).clamp(min=1)
+    rel = (32 + V / 64 + 4 * span) * 2.0 ** -24
+    tol_l = rel * (1 + fin.abs().amax(1))
+    half = 2.0 ** -8 if z.dtype == BF16 else 0.0
+    n = int((t != ignore).sum())
+    for red, s in (('none', 1.0), ('sum', 1.0), ('mean', 1 / max(n, 1))):
+        loss, d = train.cross_entropy(z, t, reduction=red, smoothing=e, ignore_index=ignore)
+        assert torch.equal(d.isnan(), dw.isnan())
+        w = torch.where(dw.isnan(), 0.0, dw)
+        got = torch.where(dw.isnan(), 0.0, d.double())
+        _within(got, w * s, ((rel.unsqueeze(1) * (w.abs() + e / V + 2.0 ** -24) + half * w.abs()) * s
+                             + 1e-37), red)
+        if red == 'none':
+            fine = lw.isfinite()
+            assert torch.equal(loss.isnan(), lw.isnan()) and torch.equal(loss.isinf(), lw.isinf())
+            _within(loss[fine], lw[fine], tol_l[fine], 'loss')
+        elif n == 0 and red == 'mean':
+            assert loss.isnan()
+        elif lw.isnan().any():
+            assert loss.isnan()
+        elif lw.isinf().any():
+            assert loss.isinf()
+        else:
+            _within(loss, lw.sum() * s, tol_l.sum() * s + 2.0 ** -23 * lw.abs().sum() * s, red)
+        only, none = train.cross_entropy(z, t, reduction=red, smoothing=e, ignore_index=ignore,
+                                         grad=False)
+        assert none is None and torch.equal(only.nan_to_num(7.0), loss.nan_to_num(7.0))
+        buf = z.clone()
+        again, same = train.cross_entropy(buf, t, reduction=red, smoothing=e, ignore_index=ignore,
+                                          out=buf)
+        assert same is buf and torch.equal(buf.nan_to_num(7.0), d.nan_to_num(7.0))
+        assert torch.equal(again.nan_to_num(7.0), loss.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('R,V', [(1, 1), (1, 2), (5, 10), (512, 10), (70, 63), (33, 64), (9, 65),
+                                 (3000, 17), (7, 255), (4, 1000), (12, 1024), (3, 4097), (130, 8192),
+                                 (2, 16385), (3, 50021), (2, 65536), (2, 131072), (2, 150001),
+                                 (1, 300000)])
+@pytest.mark.parametrize('e', [0.0, 0.1])
+def test_cross_entropy(gpu, to, R, V, e):
+    f = _randn(gpu, R + V)
+    z = f(R, V, to=to, std=3.0)
+    t = torch.randint(0, V, (R,), device=gpu, generator=torch.Generator(device=gpu).manual_seed(V))
+    t[1::5] = -100
+    _check_loss(z, t, e)
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('V', [8, 300, 5000, 140000])
+def test_cross_entropy_masks(gpu, to, V):
+    """Masked classes, rows that masks leave empty, the type's lowest value, infinities, NaN,
+    targets that are masked, ignored or no class."""
+    z = _randn(gpu, V)(14, V, to=to, std=3.0)
+    t = torch.arange(14, device=gpu) % 4
+    z[:, V - 2:] = -math.inf
+    z[1, 4:] = -math.inf
+    z[2] = -math.inf                       # nothing left
+    z[3] = torch.finfo(to).min             # masked by the lowest value: uniform
+    z[4, 1:] = torch.finfo(to).min
+    t[5] = V - 1                           # a masked target: an infinite loss
+    z[6, 2] = math.nan
+    z[7, 3] = math.inf
+    t[8], t[9], t[10] = -100, V, -1        # ignored; no class
+    z[11] += 1e4
+    z[12] -= 1e4
+    z[13, 0], t[13] = 1e4, 1
+    for rows in ([0, 1, 3, 4, 8, 11, 12, 13], list(range(14)), [2, 8], [8]):
+        _check_loss(z[rows].contiguous(), t[rows].contiguous())
+    _check_loss(z[[0, 3, 8, 11]][:, :V - 2].contiguous(), t[[0, 3, 8, 11]], 0.2)
+    _check_loss(z[:2].contiguous(), t[:2].contiguous(), ignore=1)
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+def test_cross_entropy_strides(gpu, to):
+    """Rows apart at any offset, leading axes: what a contiguous copy gives."""
+    big = _randn(gpu, 3)(20, 3000, to=to)
+    t = torch.arange(20, device=gpu) * 7
+    for off, V in ((0, 2048), (1, 2048), (3, 999), (8, 2500)):
+        z = big[:, off:off + V]
+        got, want = train.cross_entropy(z, t), train.cross_entropy(z.contiguous(), t)
+        _close(got[0], want[0])
+        _close(got[1], want[1])
+    got, want = train.cross_entropy(big.view(4, 5, 3000), t.view(4, 5)), train.cross_entropy(big, t)
+    _close(got[0], want[0])
+    _close(got[1].view(20, 3000), want[1])
+    loss, d = train.cross_entropy(big[:0], t[:0], reduction='sum')
+    assert float(loss) == 0 and d.shape == (0, 3000)
+    assert train.cross_entropy(big[:0], t[:0], reduction='none')[0].shape == (0,)
+    assert train.cross_entropy(big[:0], t[:0])[0].isnan()
+
+
+def test_cross_entropy_long_offsets(gpu):
+    """Rows past 2^32 values, the gradient in the logits' place."""
+    V, R = 131072, 32768 + 3
+    z = torch.zeros(R, V, dtype=BF16, device=gpu)
+    z[-1, 5] = 8.0
+    t = torch.full((R,), 5, device=gpu)
+    loss, d = train.cross_entropy(z, t, reduction='none', out=z)
+    want, dw = _loss64(torch.zeros(2, V, device=gpu).index_put_(
+        (torch.tensor([1], device=gpu), torch.tensor([5], device=gpu)), torch.tensor(8.0, device=gpu)),
+        t[:2], 0.0, -100)
+    assert abs(float(loss[0]) - float(want[0])) < 1e-3 and abs(float(loss[-1]) - float(want[1])) < 1e-3
+    assert (d[-2:].double() - dw).abs().max() < 2.0 ** -8
+
+
+def test_cross_entropy_autograd(gpu):
+    """Through autograd, with the reductions' own factors, and against differences of the loss."""
+    f = _randn(gpu, 4)
+    z, t = f(6, 40), torch.arange(6, device=gpu)
+    z.requires_grad_()
+    for red in ('mean', 'sum', 'none'):
+        loss, d = train.cross_entropy(z, t, reduction=red, smoothing=0.1)
+        w = torch.arange(1.0, 7.0, device=gpu) if red == 'none' else torch.tensor(3.0, device=gpu)
+        got, = torch.autograd.grad(loss, z, w)
+        assert torch.equal(got, d * (w.unsqueeze(1) if red == 'none' else w))
+    loss, d = train.cross_entropy(z.detach(), t, reduction='sum')
+    step, h = f(6, 40), 2.0 ** -6
+    side = [train.cross_entropy(z.detach() + s * step, t, reduction='none')[0].double().sum()
+            for s in (h, -h)]
+    num = float((side[0] - side[1]) / (2 * h))
+    assert abs(num - float((d.double() * step.double()).sum())) < 2e-3 * float(d.norm() * step.norm())
+
+
+def test_cross_entropy_refusals(gpu):
+    z, t = torch.zeros(4, 8, device=gpu), torch.zeros(4, dtype=torch.int64, device=gpu)
+    for bad in (lambda: train.cross_entropy(z, t.int()), lambda: train.cross_entropy(z, t[:3]),
+                lambda: train.cross_entropy(z, t.cpu()), lambda: train.cross_entropy(z, t, reduction='max'),
+                lambda: train.cross_entropy(z, t, smoothing=2.0), lambda: train.cross_entropy(z[:, :0], t),
+                lambda: train.cross_entropy(z, t, out=z.bfloat16()),
+                lambda: train.cross_entropy(z, t, out=torch.zeros(8, 4, device=gpu).t())):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(NotImplementedError):
+        train.cross_entropy(z.half(), t)
+
+
+# ------------------------------------------------------------------ optimiser
+
+HYPER = dict(lr=3e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+
+
+def _adamw64(p, m, v, g, step, lr, betas, eps, weight_decay):
+    b1, b2 = betas
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    p = p * (1 - lr * weight_decay) - lr / (1 - b1 ** step) * m / (
+        (v / (1 - b2 ** step)).sqrt() + eps)
+    return p, m, v
+
+
+def _tensors(f, sizes, to, shift=0):
+    """Parameters of these sizes, each `shift` values into its own storage."""
+    return [f(n + shift, to=to)[shift:] for n in sizes]
+
+
+SETS = [[1], [255], [256, 257], [5 * 50, 50, 50 * 50, 50, 5], [0, 3, 4096, 0, 4099, 1 << 16],
+        [n % 700 for n in range(1, 2000, 11)]]
+
+
+@pytest.mark.parametrize('pt,gt', [(F32, F32), (F32, BF16), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize('sizes', SETS, ids=lambda s: str(len(s)) + 'x' + str(sum(s)))
+@pytest.mark.parametrize('shift', [0, 1])
+def test_adamw_32(gpu, pt, gt, sizes, shift):
+    """Three steps with states in 32 bits, tensors on and off a wide load's boundary.  A step's
+    moments carry four roundings of 2^-24; the update, under lr (1 + |m| / u), six; the parameter
+    one of its type."""
+    f = _randn(gpu, sum(sizes))
+    params, copies = _tensors(f, sizes, pt, shift), _tensors(f, sizes, BF16, shift)
+    state = train.adamw_state(params)
+    ref = [tuple(torch.zeros_like(p, dtype=F64) for _ in range(3)) for p in params]
+    for k in range(1, 4):
+        grads = _tensors(f, sizes, gt, shift)
+        start = [p.double() for p in params]
+        train.adamw_step(params, grads, state, k, copies=copies, **HYPER)
+        for i, (p, c, (m, v)) in enumerate(zip(params, copies, train.adamw_moments(params, state))):
+            pw, mw, vw = _adamw64(start[i], ref[i][0], ref[i][1], grads[i].double(), k, **HYPER)
+            seen = ref[i][2] + grads[i].double().abs()
+            ref[i] = (mw, vw, seen)
+            _within(m, mw, 4 * 2.0 ** -24 * seen, 'm')
+            _within(v, vw, 8 * k * 2.0 ** -24 * vw + 1e-37, 'v')
+            tol = 2.0 ** -23 * pw.abs() + HYPER['lr'] * 20 * 2.0 ** -22
+            half = 2.0 ** -8 * pw.abs()
+            _within(p, pw, tol + (half if pt == BF16 else 0), 'p')
+            _within(c, pw, tol + half, 'copy')
+
+
+def test_adamw_32_is_torchs(gpu):
+    """torch.optim.AdamW in 64 bits takes the same path: five steps' parameters within five steps'
+    roundings."""
+    f = _randn(gpu, 2)
+    ours = [f(1000), f(37, 11)]
+    params = [p.double().requires_grad_() for p in ours]
+    opt = torch.optim.AdamW(params, lr=1e-2, weight_decay=0.05)
+    state = train.adamw_state(ours)
+    for k in range(1, 6):
+        grads = [f(*p.shape) for p in params]
+        for p, g in zip(params, grads):
+            p.grad = g.double()
+        opt.step()
+        train.adamw_step(ours, grads, state, k, lr=1e-2, weight_decay=0.05)
+    for p, q in zip(params, ours):
+        _within(q, p.detach(), 5 * (2.0 ** -23 * p.detach().abs() + 1e-2 * 20 * 2.0 ** -22), 'p')
+
+
+def _grid(x):
+    """The spacing of e4m3 values at magnitude x (in units of the scale)."""
+    return torch.exp2(torch.floor(torch.log2(x.clamp(min=2.0 ** -6))) - 3)
+
+
+@pytest.mark.parametrize('pt,gt', [(F32, F32), (F32, BF16), (BF16, BF16)])
+@pytest.mark.parametrize('sizes', SETS, ids=lambda s: str(len(s)) + 'x' + str(sum(s)))
+@pytest.mark.parametrize('shift', [0, 1])
+def test_adamw_8(gpu, pt, gt, sizes, shift):
+    """States in 8 bits: from the state as stored, a step's parameters are the formula's, and each
+    stored moment is one of the two e4m3 values around the exact one (in units of its block's
+    scale, the largest / 448; 2^-18 of slack for the fp32 arithmetic)."""
+    f = _randn(gpu, sum(sizes) + 1)
+    params = _tensors(f, sizes, pt, shift)
+    state = train.adamw_state(params, bits=8)
+    for k in range(1, 4):
+        grads = [g * torch.exp(3 * f(g.numel())).to(gt) for g in _tensors(f, sizes, gt, shift)]
+        for g in grads:
+            g[::3] = 0
+        start, old = [p.double() for p in params], train.adamw_moments(params, state)
+        train.adamw_step(params, grads, state, k, **HYPER)
+        new, at = train.adamw_moments(params, state), 0
+        for i, p in enumerate(params):
+            pw, mw, vw = _adamw64(start[i], old[i][0].double(), old[i][1].double(),
+                                  grads[i].double(), k, **HYPER)
+            tol = 2.0 ** -22 * pw.abs() + HYPER['lr'] * 20 * 2.0 ** -20
+            _within(p, pw, tol + (2.0 ** -8 * pw.abs() if pt == BF16 else 0), 'p')
+            nb = (p.numel() + 255) // 256
+            for got, want, key in ((new[i][0].double(), mw, 'm_scale'),
+                                   (new[i][1].double().sqrt(), vw.sqrt(), 'v_scale')):
+                pad = torch.zeros(nb * 256, dtype=F64, device=gpu)
+                pad[:p.numel()] = want
+                top = pad.view(nb, 256).abs().amax(1)
+                sc = state[key][at:at + nb].double()
+                _within(sc, top / 448, 2.0 ** -20 * sc, key)
+                s = sc.repeat_interleave(256)[:p.numel()]
+                t = want.abs() / s.clamp(min=1e-300)
+                _within(got, want, s * _grid(t) * (1 + 2.0 ** -10) + 2.0 ** -16 * want.abs(), key)
+                if key == 'v_scale':
+                    assert not ((want > 0) & (got == 0)).any()
+            at += nb
+
+
+def test_adamw_8_moves_on_average(gpu):
+    """A gradient of constant size takes v to its square though every step moves it by less than
+    the grid's spacing, and the mean over many values comes within a few percent."""
+    n = 1 << 16
+    p, g = torch.zeros(n, device=gpu), torch.ones(n, device=gpu)
+    g[::256] = 16.0  # a larger value in every block, so that the others are not its scale
+    state = train.adamw_state([p], bits=8)
+    for k in range(1, 1501):
+        train.adamw_step([p], [g], state, k, betas=(0.9, 0.995))
+    (m, v), = train.adamw_moments([p], state)
+    keep = g == 1
+    assert abs(float(m[keep].mean()) - 1) < 0.02
+    assert abs(float(v[keep].sqrt().mean()) - 1) < 0.05
+
+
+@pytest.mark.parametrize('bits', [8, 32])
+def test_adamw_scale(gpu, bits):
+    """The gradients' factor on the device; where it is not finite nothing changes."""
+    f = _randn(gpu, 8)
+    p, g = f(1000), f(1000)
+    a, b = p.clone(), p.clone()
+    sa, sb = train.adamw_state([a], bits), train.adamw_state([b], bits)
+    train.adamw_step([a], [g], sa, 1, scale=torch.tensor([0.5], device=gpu))
+    train.adamw_step([b], [g * 0.5], sb, 1)
+    assert torch.equal(a, b) and all(torch.equal(sa[k], sb[k]) for k in sa if k != 'bits')
+    for bad in (math.inf, math.nan):
+        train.adamw_step([a], [g], sa, 2, scale=torch.tensor(bad, device=gpu))
+        assert torch.equal(a, b) and all(torch.equal(sa[k], sb[k]) for k in sa if k != 'bits')
+
+
+@pytest.mark.parametrize('bits', [8, 32])
+def test_adamw_not_finite(gpu, bits):
+    """A NaN or infinite gradient leaves a trace in its own value (32 bits) or block (8 bits) and
+    nowhere else."""
+    p = torch.ones(1024, device=gpu)
+    g = torch.ones(1024, device=gpu)
+    g[300], g[900] = math.nan, math.inf
+    state = train.adamw_state([p], bits)
+    train.adamw_step([p], [g], state, 1)
+    (m, v), = train.adamw_moments([p], state)
+    for t in (m, v):
+        assert not t[300].isfinite() and not t[900].isfinite()
+        assert t[:256].isfinite().all() and t[512:768].isfinite().all()
+    assert p[300].isnan() and p[:300].isfinite().all() and p[901:].isfinite().all()
+
+
+def test_adamw_long_offsets(gpu):
+    """A tensor of more than 2^32 values, states in 8 bits."""
+    n = (1 << 32) + 700
+    p = torch.zeros(n, dtype=BF16, device=gpu)
+    g = torch.zeros(n, dtype=BF16, device=gpu)
+    g[-3:], g[:3], g[1 << 31] = 1.0, -1.0, 1.0
+    state = train.adamw_state([p], bits=8)
+    train.adamw_step([p], [g], state, 1, lr=0.5, weight_decay=0.0)
+    assert torch.equal(p[-4:].float().cpu(), torch.tensor([0, -0.5, -0.5, -0.5]))
+    assert torch.equal(p[:4].float().cpu(), torch.tensor([0.5, 0.5, 0.5, 0]))
+    assert float(p[1 << 31]) == -0.5 and int((p != 0).sum()) == 7
+
+
+def test_adamw_refusals(gpu):
+    p, g = torch.zeros(10, device=gpu), torch.zeros(10, device=gpu)
+    s = train.adamw_state([p])
+    t = torch.zeros(10, 2, device=gpu)[:, 0]
+    for bad in (lambda: train.adamw_step([p], [], s, 1), lambda: train.adamw_step([p], [g[:5]], s, 1),
+                lambda: train.adamw_step([t], [g], s, 1), lambda: train.adamw_step([p, p.bfloat16()], [g, g], s, 1),
+                lambda: train.adamw_step([p], [g], train.adamw_state([torch.zeros(300, device=gpu)]), 1),
+                lambda: train.adamw_step([p], [g], dict(s, bits=8, m_scale=g, v_scale=g), 1),
+                lambda: train.adamw_step([p], [g], s, 0), lambda: train.adamw_step([p], [g], s, 1, betas=(1.0, 0.9)),
+                lambda: train.adamw_step([p], [g], s, 1, copies=[g]),
+                lambda: train.adamw_step([p], [g], s, 1, scale=g)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(NotImplementedError):
+        train.adamw_step([p.double()], [g.double()], s, 1)
+
+
+# ------------------------------------------------------------- used together
+
+def test_own_stream(gpu):
+    """A training step on a side stream, its workspaces freed while it runs: the bits of the same
+    step on the default stream."""
+    f = _randn(gpu, 6)
+    x, W, b = f(600, 300), f(200, 300, std=0.1), f(200)
+    t = torch.randint(0, 200, (600,), device=gpu)
+
+    def step():
+        w, c = W.clone(), b.clone()
+        y, z = train.linear(x, w, c, act='silu', save=True)
+        loss, d = train.cross_entropy(y, t)
+        grads = train.linear_backward(d, x, w, z=z, act='silu')
+        train.adamw_step([w, c], grads[1:], train.adamw_state([w, c], 8), 1)
+        return loss, w, c
+
+    want = step()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = step()
+    s.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))

@@ -5,7 +5,7 @@ Drop-in GPU implementations of the reference's bound primitives
 by hand-written HIP kernels for gfx950 in libvibecheck_amd.so (C ABI:
 include/vibecheck_amd.h).
 """
-from . import _lib, spec, workloads  # noqa: F401
+from . import _lib, spec, train, workloads  # noqa: F401
 
 __version__ = '0.1.0'
 

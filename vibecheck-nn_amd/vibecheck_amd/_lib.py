@@ -152,8 +152,20 @@ SIGNATURES = {
                          _P, _P, _L, _P, _P, _L, _L, _P, _P, _P, _P, _P, _P],
     'vc_widest_axis': [_P, _P, _L, _I, _P, _P, _P],
     'vc_bisect': [_P, _P, _P, _P, _L, _I, _P, _P, _P, _P, _P],
+    'vc_linear_workspace': [_I, _L, _I, _I],
+    'vc_linear': [_I, _P, _L, _I, _L, _P, _I, _P, _I, _P, _L, _P, _P, _P, _L, _P],
+    'vc_linear_backward_workspace': [_I, _L, _I, _I, _I, _I],
+    'vc_linear_backward': [_I, _P, _L, _P, _L, _P, _P, _L, _I, _L, _I, _I, _P, _P, _P, _P, _L,
+                           _P],
+    'vc_cross_entropy_workspace': [_L, _I],
+    'vc_cross_entropy': [_I, _P, _L, _L, _L, _P, _L, _F, _I, _P, _P, _L, _P, _L, _P],
+    'vc_adamw_step': [_P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _D, _D, _D, _D, _D, _L,
+                      _P, _P],
 }
 _RESTYPE = {'vc_compact_workspace': ctypes.c_int64,
+            'vc_linear_workspace': ctypes.c_int64,
+            'vc_linear_backward_workspace': ctypes.c_int64,
+            'vc_cross_entropy_workspace': ctypes.c_int64,
             'vc_conv_t_pack_floats': ctypes.c_int64,
             'vc_conv_split_pack_bytes': ctypes.c_int64,
             'vc_fc_split_pack_bytes': ctypes.c_int64,

@@ -1,0 +1,330 @@
+"""The network itself, next to its bounds: fc layers forward and backward, the
+classification loss with its gradient, and the optimiser's step, on the library's
+kernels (no reference counterpart).
+
+Tensors are fp32 or bf16 on the GPU; every function runs on the current stream,
+allocates its outputs and workspace from torch and waits for nothing.  CPU tensors
+raise RuntimeError, other types NotImplementedError, sizes that do not fit
+ValueError.
+"""
+import ctypes
+
+import torch
+
+
+from ._lib import call, load, stream
+
+ACTS = {None: 0, 'none': 0, 'relu': 1, 'gelu': 2, 'silu': 3}
+REDUCTIONS = {'none': 0, 'sum': 1, 'mean': 2}
+BLOCK = 256     # values of an optimiser state that share a scale
+E4M3_MAX = 448.0
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _type(t, what):
+    """The library's number for a GPU tensor's type."""
+    if not t.is_cuda:
+        raise RuntimeError(f'vibecheck_amd: {what} is not on the GPU '
+                           '(the HIP library is the only compute path)')
+    k = _TYPES.get(t.dtype)
+    if k is None:
+        raise NotImplementedError(f'vibecheck_amd: {what} is {t.dtype}; fp32 and bf16 are taken')
+    if t.device.index != torch._C._cuda_getDevice():
+        raise ValueError(f'vibecheck_amd: {what} is on {t.device}, not on the current device')
+    return k
+
+
+def _like(t, ref, shape, what):
+    if t.dtype != ref.dtype or t.device != ref.device:
+        raise ValueError(f'vibecheck_amd: {what} is {t.dtype} on {t.device}, '
+                         f'expected {ref.dtype} on {ref.device}')
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f'vibecheck_amd: {what} has shape {tuple(t.shape)}, '
+                         f'expected {tuple(shape)}')
+
+
+def _rows(t):
+    """t as rows of its last axis, values of a row side by side: (tensor to keep, row stride)."""
+    n = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, n)
+    if t.shape[0] <= 1 or n == 0:
+        return t.contiguous(), n
+    if t.stride(1) != 1 and n > 1 or t.stride(0) < n:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _work(nbytes, device):
+    if nbytes < 0:
+        raise ValueError('vibecheck_amd: sizes out of range')
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+# ------------------------------------------------------------------- fc layer
+
+def _act(act):
+    if act not in ACTS:
+        raise ValueError(f'vibecheck_amd: activation {act!r}; one of {list(ACTS)} is taken')
+    return ACTS[act]
+
+
+def _linear(x, W, bias, act, residual, save):
+    k = _type(x, 'x')
+    if x.dim() < 1 or W.dim() != 2:
+        raise ValueError('vibecheck_amd: x has at least one axis, W two')
+    N, K = W.shape
+    _like(W, x, (N, x.shape[-1]), 'W')
+    shape = x.shape[:-1] + (N,)
+    if bias is not None:
+        _like(bias, x, (N,), 'bias')
+        bias = bias.contiguous()
+    if residual is not None:
+        _like(residual, x, shape, 'residual')
+    x, ldx = _rows(x)
+    W = W.contiguous()
+    M = x.numel() // K if K else shape.numel() // max(1, N)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    # the sign of relu's output is its input's; another activation's input is kept
+    z = torch.empty_like(y) if save and act and (act != 1 or residual is not None) else None
+    if residual is not None:
+        residual, ldr = _rows(residual)
+    else:
+        ldr = 0
+    work = _work(load().vc_linear_workspace(k, M, K, N), x.device)
+    call('vc_linear', k, x.data_ptr(), M, K, ldx, W.data_ptr(), N, _ptr(bias), act,
+         _ptr(residual), ldr, y.data_ptr(), _ptr(z), _ptr(work), work.numel() if work is not None else 0,
+         stream())
+    return y, (y if save and act and z is None else z)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, W, bias, act, residual):
+        y, z = _linear(x, W, bias, act, residual, True)
+        ctx.save_for_backward(x, W, z)
+        ctx.act, ctx.bias, ctx.res = act, bias is not None, residual is not None
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, W, z = ctx.saved_tensors
+        needs = ctx.needs_input_grad
+        need = [n for n, on in zip(('x', 'W', 'bias'), needs) if on]
+        dx, dW, db = linear_backward(dy, x, W, z, ctx.act, need) if need else (None, None, None)
+        return dx, dW, db, None, dy if needs[4] else None
+
+
+def linear(x, W, bias=None, act=None, residual=None, save=False):
+    """act(x W^T + bias) + residual for x (..., K), W (N, K), bias (N), residual (..., N), all of
+    one type.  ``act``: None, 'relu', 'gelu' (the erf form) or 'silu'.
+
+    With ``save`` returns (y, z), z what linear_backward needs (None without an activation;
+    for relu without a residual it is y itself).  Differentiable through autograd for inputs
+    that require it; the saved tensors are then the node's own."""
+    a = _act(act)
+    if not save and torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, W, bias, residual)):
+        return _Linear.apply(x, W, bias, a, residual)
+    y, z = _linear(x, W, bias, a, residual, save)
+    return (y, z) if save else y
+
+
+def linear_backward(dy, x, W, z=None, act=None, need=('x', 'W', 'bias')):
+    """(dx, dW, db) of y = act(x W^T + bias) from dy (..., N): dz = dy act'(z), dx = dz W,
+    dW = dz^T x, db the sum of dz over rows; None for what ``need`` does not name.  ``z`` is
+    what linear(save=True) returned.  The residual's gradient is dy."""
+    a = act if isinstance(act, int) else _act(act)
+    k = _type(dy, 'dy')
+    if W.dim() != 2 or dy.dim() < 1:
+        raise ValueError('vibecheck_amd: dy has at least one axis, W two')
+    if not set(need) <= {'x', 'W', 'bias'}:
+        raise ValueError(f"vibecheck_amd: need names {need!r}; 'x', 'W' and 'bias' are taken")
+    N, K = W.shape
+    _like(W, dy, (dy.shape[-1], K), 'W')
+    lead = dy.shape[:-1]
+    _like(x, dy, lead + (K,), 'x')
+    if a:
+        if z is None:
+            raise ValueError('vibecheck_amd: an activation needs z')
+        _like(z, dy, dy.shape, 'z')
+        z, ldz = _rows(z)
+    else:
+        z, ldz = None, 0
+    M = lead.numel()
+    new = dict(dtype=dy.dtype, device=dy.device)
+    dx = torch.empty(lead + (K,), **new) if 'x' in need else None
+    dW = torch.empty(N, K, **new) if 'W' in need else None
+    # no row adds to it, no launch writes it
+    db = (torch.empty if M else torch.zeros)(N, **new) if 'bias' in need else None
+    dy, ldy = _rows(dy)
+    x, ldx = _rows(x)
+    W = W.contiguous()
+    which = (dx is not None) + 2 * (dW is not None) + 4 * (db is not None)
+    work = _work(load().vc_linear_backward_workspace(k, M, K, N, a, which), dy.device)
+    call('vc_linear_backward', k, dy.data_ptr(), ldy, x.data_ptr(), ldx, W.data_ptr(), _ptr(z), ldz,
+         a, M, K, N, _ptr(dx), _ptr(dW), _ptr(db), _ptr(work),
+         work.numel() if work is not None else 0, stream())
+    return dx, dW, db
+
+
+# ----------------------------------------------------------------------- loss
+
+class _Loss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, target, reduction, ignore_index, smoothing):
+        loss, d = _cross_entropy(logits, target, reduction, ignore_index, smoothing, True, None)
+        ctx.save_for_backward(d)
+        ctx.mark_non_differentiable(d)
+        return loss, d
+
+    @staticmethod
+    def backward(ctx, g, _):
+        d, = ctx.saved_tensors
+        return (d * g.unsqueeze(-1) if g.dim() else d * g).to(d.dtype), None, None, None, None
+
+
+def _cross_entropy(logits, target, reduction, ignore_index, smoothing, grad, out):
+    k = _type(logits, 'logits')
+    if reduction not in REDUCTIONS:
+        raise ValueError(f'vibecheck_amd: reduction {reduction!r}; one of {list(REDUCTIONS)} is taken')
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError('vibecheck_amd: logits have at least one class')
+    if not 0 <= smoothing <= 1:
+        raise ValueError(f'vibecheck_amd: smoothing {smoothing} is not in [0, 1]')
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if target.dtype != torch.int64 or target.device != logits.device or target.shape != lead:
+        raise ValueError(f'vibecheck_amd: target is {target.dtype} {tuple(target.shape)} on '
+                         f'{target.device}, expected int64 {tuple(lead)} on {logits.device}')
+    R, kind = lead.numel(), REDUCTIONS[reduction]
+    loss = torch.empty(lead if kind == 0 else (), dtype=torch.float32, device=logits.device)
+    if out is not None:
+        _like(out, logits, logits.shape, 'out')
+        if not out.is_contiguous():
+            raise ValueError('vibecheck_amd: out must be contiguous')
+        d = out
+    else:
+        d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None
+    z, ld = _rows(logits)
+    target = target.contiguous()
+    work = _work(load().vc_cross_entropy_workspace(R, kind), logits.device)
+    call('vc_cross_entropy', k, z.data_ptr(), R, V, ld, target.data_ptr(), ignore_index, smoothing,
+         kind, loss.data_ptr(), _ptr(d), V, _ptr(work), work.numel() if work is not None else 0,
+         stream())
+    return loss, d
+
+
+def cross_entropy(logits, target, reduction='mean', ignore_index=-100, smoothing=0.0, grad=True,
+                  out=None):
+    """(loss, dlogits) of softmax cross-entropy: logits (..., V), target int64 (...), loss fp32,
+    dlogits of the logits' type (None without ``grad``; written to ``out``, which may be the
+    logits, where that is given).
+
+    loss = lse - (1 - smoothing) z_t - smoothing mean(z) per row ('none'), summed, or averaged
+    over the rows whose target is not ``ignore_index``; dlogits is its gradient (per row for
+    'none').  A target that is no class gives NaN, a row without a logit above -inf an infinite
+    loss and no gradient.  The loss is differentiable where the logits require it."""
+    if torch.is_grad_enabled() and logits.requires_grad and grad and out is None:
+        return _Loss.apply(logits, target, reduction, ignore_index, smoothing)
+    return _cross_entropy(logits, target, reduction, ignore_index, smoothing, grad, out)
+
+
+# ------------------------------------------------------------------ optimiser
+
+def _blocks(params):
+    return sum((p.numel() + BLOCK - 1) // BLOCK for p in params)
+
+
+def adamw_state(params, bits=32):
+    """A new state for adamw_step over ``params``: {'bits', 'm', 'v'} of fp32 values, each tensor
+    padded to blocks of 256, or with ``bits`` 8 the bytes of e4m3 values ('m', and in 'v' the
+    square roots) and one scale per block ('m_scale', 'v_scale')."""
+    if bits not in (8, 32):
+        raise ValueError(f'vibecheck_amd: states of {bits} bits; 8 and 32 are taken')
+    params = list(params)
+    n = _blocks(params)
+    dev = params[0].device if params else 'cuda'
+    if bits == 32:
+        return {'bits': 32, 'm': torch.zeros(n * BLOCK, device=dev),
+                'v': torch.zeros(n * BLOCK, device=dev)}
+    return {'bits': 8, 'm': torch.zeros(n * BLOCK, dtype=torch.uint8, device=dev),
+            'v': torch.zeros(n * BLOCK, dtype=torch.uint8, device=dev),
+            'm_scale': torch.zeros(n, device=dev), 'v_scale': torch.zeros(n, device=dev)}
+
+
+def adamw_moments(params, state):
+    """[(m, v), ...] of each parameter in fp32, from a state of either kind."""
+    m, v = state['m'], state['v']
+    if state['bits'] == 8:
+        m, v = ((c.view(torch.float8_e4m3fn).float().view(-1, BLOCK) * s.unsqueeze(1)).view(-1)
+                for c, s in ((m, state['m_scale']), (v, state['v_scale'])))
+        v = v * v
+    out, at = [], 0
+    for p in params:
+        out.append(tuple(t[at:at + p.numel()].view(p.shape) for t in (m, v)))
+        at += (p.numel() + BLOCK - 1) // BLOCK * BLOCK
+    return out
+
+
+def _one_type(tensors, sizes, what):
+    """Type number and pointers of a list of contiguous GPU tensors of one type."""
+    k, kind, dev = _type(tensors[0], what), tensors[0].dtype, tensors[0].device
+    for t, n in zip(tensors, sizes):
+        if t.dtype != kind or t.device != dev or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f'vibecheck_amd: {what} are contiguous, of one type, on one device '
+                             f'and of their parameters\' sizes; got {t.dtype} {tuple(t.shape)} '
+                             f'on {t.device}')
+    return k, [t.data_ptr() for t in tensors]
+
+
+def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
+               weight_decay=0.01, copies=None, scale=None):
+    """One AdamW step in place, all tensors by one launch per 88: params (fp32 or bf16), grads
+    (fp32 or bf16), ``state`` from adamw_state, ``step`` counting from 1, with
+    torch.optim.AdamW's formula.  ``copies``: bf16 tensors that receive the new parameters.  ``scale``: one fp32
+    value on the GPU that multiplies the gradients (a clip, a loss scale); where it is not finite
+    the step changes nothing.
+
+    States of 8 bits are rounded up or down by a hash of the value's place and the step, so that
+    a step that moves a value by less than its grid does move it on average; the same inputs
+    give the same results."""
+    params, grads = list(params), list(grads)
+    if not params:
+        return
+    sizes = [p.numel() for p in params]
+    if len(grads) != len(params) or (copies is not None and len(copies) != len(params)):
+        raise ValueError('vibecheck_amd: one gradient (and copy) for each parameter')
+    kp, pp = _one_type(params, sizes, 'params')
+    kg, pg = _one_type(grads, sizes, 'grads')
+    if grads[0].device != params[0].device:
+        raise ValueError('vibecheck_amd: params and grads are on different devices')
+    n, cnt = sum((k + BLOCK - 1) // BLOCK for k in sizes), len(sizes)
+    bits = state['bits']
+    keys = ('m', 'v') if bits == 32 else ('m', 'v', 'm_scale', 'v_scale')
+    for key in keys:
+        t = state[key]
+        want = torch.float32 if bits == 32 or key[1:] else torch.uint8
+        if t.dtype != want or t.numel() != (n if key[1:] else n * BLOCK) or \
+                t.device != params[0].device or not t.is_contiguous():
+            raise ValueError(f'vibecheck_amd: state {key!r} does not fit these parameters')
+    array = ctypes.c_void_p * cnt
+    if copies is not None:
+        kc, pc = _one_type(copies, sizes, 'copies')
+        if kc != 1 or copies[0].device != params[0].device:
+            raise ValueError('vibecheck_amd: copies are bf16 tensors beside their parameters')
+        pc = array(*pc)
+    else:
+        pc = None
+    if scale is not None and (scale.dtype != torch.float32 or scale.numel() != 1 or
+                              scale.device != params[0].device):
+        raise ValueError('vibecheck_amd: scale is one fp32 value on the parameters\' device')
+    pp, pg, pn = array(*pp), array(*pg), (ctypes.c_int64 * cnt)(*sizes)
+    call('vc_adamw_step', ctypes.addressof(pp), ctypes.addressof(pg),
+         ctypes.addressof(pc) if pc is not None else None, ctypes.addressof(pn), cnt, kp, kg, bits,
+         state['m'].data_ptr(), state['v'].data_ptr(), _ptr(state.get('m_scale')),
+         _ptr(state.get('v_scale')), lr, betas[0], betas[1], eps, weight_decay, step, _ptr(scale),
+         stream())
