@@ -1,0 +1,169 @@
+// The fc layer's kernels share this: types, activations, what a product is and how
+// its sums are finished (bias, activation, residual, rounding, stores).
+#pragma once
+#include "vc_gemm_core.h"
+#include "vc_split.h"
+
+namespace vcl {
+
+using namespace vcs;
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+enum Act { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
+
+__device__ __forceinline__ float bf_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t w) {
+  return __builtin_bit_cast(float, w & 0xffff0000u);
+}
+// Two values rounded to nearest, the first in the low half.
+__device__ __forceinline__ uint32_t bf_pack(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2bf));
+}
+
+template <class T>
+__device__ __forceinline__ float get(const T* p) {
+  if constexpr (sizeof(T) == 4) return *p;
+  else return bf_lo(*p);
+}
+template <class T>
+__device__ __forceinline__ void put(T* p, float v) {
+  if constexpr (sizeof(T) == 4) *p = v;
+  else *p = (uint16_t)bf_pack(v, 0.f);
+}
+
+constexpr float kLog2e = 1.44269504088896341f;
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// The normal distribution's integral up to z, and e = exp(-z^2 / 2) on the way
+// (Abramowitz and Stegun 7.1.26, off by at most 7.5e-8): twenty instructions,
+// where the library's erff takes twice as many and the 134 million values of an
+// 8192 x 16384 output showed it (150 us of 1140).
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+  e = __builtin_amdgcn_exp2f(z * z * (-0.5f * kLog2e));
+  float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  p = __builtin_fmaf(p, t, 1.421413741f);
+  p = __builtin_fmaf(p, t, -0.284496736f);
+  p = __builtin_fmaf(p, t, 0.254829592f);
+  const float q = 0.5f * p * t * e;  // of -|z|
+  return z < 0.f ? q : 1.f - q;
+}
+
+__device__ __forceinline__ float activate(float z, int act) {
+  float e;
+  if (act == kRelu) return z > 0.f ? z : (z != z ? z : 0.f);
+  if (act == kGelu) return z * normal_cdf(z, e);
+  if (act == kSilu) return z * __builtin_amdgcn_rcpf(1.f + exp_of(-z));
+  return z;
+}
+
+__device__ __forceinline__ float slope(float z, int act) {
+  if (act == kRelu) return z > 0.f ? 1.f : 0.f;
+  if (act == kGelu) {
+    float e;
+    const float c = normal_cdf(z, e);
+    return __builtin_fmaf(z * e, 0.39894228040143268f, c);
+  }
+  const float s = __builtin_amdgcn_rcpf(1.f + exp_of(-z));
+  return s * (1.f + z * (1.f - s));
+}
+
+// An operand: `rows` of its free axis; (row, k) at p[row ld + k], across at
+// p[k ld + row].  vec: two rows' eight k may be read by its wide loads.
+template <class T>
+struct Operand {
+  const T* p;
+  int64_t ld;
+  int rows, vec;
+};
+
+template <class T>
+struct Product {
+  Operand<T> A, B;
+  int I, J, K;
+  int slices, steps;  // steps of a slice
+  float* part;        // slices > 1: (slices, I, J)
+  const T *bias, *res;
+  int64_t ldr;
+  T *out, *z;
+  int act, wide;      // wide: four columns of out, z, res and bias by one access
+  int64_t tiles;
+  vcg::FastDiv f_nj;
+  // as bf16 parts (an fp32 value is three): plane p of an operand starts p planes
+  // after the first
+  const uint16_t *pa, *pb;
+  int64_t lda, ldb, planeA, planeB;
+};
+
+// The tiled products of vc_linear_tile.hip: shape 0 is 256 x 256 (fp32: 256 x
+// 128), 1 is 128 x 128, 2 is 64 x 64.  Rows (across: k) lie lda, ldb values apart.
+// The caller has seen to it that every operand's base and ld are multiples of 16
+// bytes, that K is a multiple of eight (an operand whose k is contiguous) or its
+// rows are (one that is read across), and that 256 rows span less than 2^31 bytes.
+struct TileShape {
+  int bi, bj, bk, threads, lds;
+};
+TileShape tile_shape(int type, int shape);
+template <class T>
+void run_tiles(const Product<T>& a, int shape, bool xa, bool xb, hipStream_t st);
+
+// Four columns j .. j + 3 of row i: bias, activation, residual, stores.
+template <class T>
+__device__ __forceinline__ void finish(const Product<T>& a, int64_t i, int j, const float* s) {
+  const int n = min(4, a.J - j);
+  float v[4], b[4] = {0.f, 0.f, 0.f, 0.f}, r[4] = {0.f, 0.f, 0.f, 0.f};
+  T* const o = a.out + i * a.J + j;
+  if (a.wide) {  // J a multiple of four
+    if (a.bias) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) b[q] = get(a.bias + j + q);
+    }
+    if (a.res) {
+      const T* const p = a.res + i * a.ldr + j;
+      if constexpr (sizeof(T) == 4) {
+        const v4f w = *reinterpret_cast<const v4f*>(p);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) r[q] = w[q];
+      } else {
+        const u2 w = *reinterpret_cast<const u2*>(p);
+        r[0] = bf_lo(w.x), r[1] = bf_hi(w.x), r[2] = bf_lo(w.y), r[3] = bf_hi(w.y);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (q >= n) continue;
+      if (a.bias) b[q] = get(a.bias + j + q);
+      if (a.res) r[q] = get(a.res + i * a.ldr + j + q);
+    }
+  }
+  float z[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    z[q] = a.bias ? s[q] + b[q] : s[q];
+    v[q] = activate(z[q], a.act);
+    if (a.res) v[q] += r[q];
+  }
+  if (a.wide) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<v4f*>(o) = v4f{v[0], v[1], v[2], v[3]};
+      if (a.z) *reinterpret_cast<v4f*>(a.z + i * a.J + j) = v4f{z[0], z[1], z[2], z[3]};
+    } else {
+      *reinterpret_cast<u2*>(o) = u2{bf_pack(v[0], v[1]), bf_pack(v[2], v[3])};
+      if (a.z)
+        *reinterpret_cast<u2*>(a.z + i * a.J + j) = u2{bf_pack(z[0], z[1]), bf_pack(z[2], z[3])};
+    }
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (q >= n) continue;
+    put(o + q, v[q]);
+    if (a.z) put(a.z + i * a.J + j + q, z[q]);
+  }
+}
+
+}  // namespace vcl

@@ -11,78 +11,13 @@
 // largest starts from zero each step of 32 and is added in fp32.  Where the sum
 // is not finite the largest products' sum stands alone: with an infinity or NaN
 // among the values it is what the fp32 product gives, and the small ones are not.
-#include "vc_gemm_core.h"
-#include "vc_split.h"
+#include "vc_linear.h"
 
 namespace {
 
-using namespace vcs;
-
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+using namespace vcl;
 
 constexpr int LNT = 256;  // threads: four waves, 2 x 2 over the tile
-
-enum Act { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
-
-__device__ __forceinline__ float bf_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t w) {
-  return __builtin_bit_cast(float, w & 0xffff0000u);
-}
-// Two values rounded to nearest, the first in the low half.
-__device__ __forceinline__ uint32_t bf_pack(float a, float b) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2bf));
-}
-
-template <class T>
-__device__ __forceinline__ float get(const T* p) {
-  if constexpr (sizeof(T) == 4) return *p;
-  else return bf_lo(*p);
-}
-template <class T>
-__device__ __forceinline__ void put(T* p, float v) {
-  if constexpr (sizeof(T) == 4) *p = v;
-  else *p = (uint16_t)bf_pack(v, 0.f);
-}
-
-__device__ __forceinline__ float activate(float z, int act) {
-  if (act == kRelu) return z > 0.f ? z : (z != z ? z : 0.f);
-  if (act == kGelu) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-  if (act == kSilu) return z / (1.f + expf(-z));
-  return z;
-}
-
-__device__ __forceinline__ float slope(float z, int act) {
-  if (act == kRelu) return z > 0.f ? 1.f : 0.f;
-  if (act == kGelu)
-    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) +
-           z * expf(-0.5f * z * z) * 0.39894228040143268f;
-  const float s = 1.f / (1.f + expf(-z));
-  return s * (1.f + z * (1.f - s));
-}
-
-// An operand: `rows` of its free axis; (row, k) at p[row ld + k], across at
-// p[k ld + row].  vec: two rows' eight k may be read by its wide loads.
-template <class T>
-struct Operand {
-  const T* p;
-  int64_t ld;
-  int rows, vec;
-};
-
-template <class T>
-struct Product {
-  Operand<T> A, B;
-  int I, J, K;
-  int slices, steps;  // steps of a slice
-  float* part;        // slices > 1: (slices, I, J)
-  const T *bias, *res;
-  int64_t ldr;
-  T *out, *z;
-  int act, wide;      // wide: four columns of out, z, res and bias by one access
-  int64_t tiles;
-  vcg::FastDiv f_nj;
-};
 
 // Eight k of two rows, as loaded: of bf16 [row][k pair] or across [k] (both
 // rows), of fp32 [row][k] or across [k][row].
@@ -188,62 +123,6 @@ __device__ __forceinline__ void unit_row(const Raw<T>& v, int r, u4* o) {
       o[0][j] = ACROSS ? __builtin_amdgcn_perm(v.d[2 * j + 1], v.d[2 * j],
                                                r ? 0x07060302 : 0x05040100)
                        : v.d[4 * r + j];
-  }
-}
-
-// Four columns j .. j + 3 of row i: bias, activation, residual, stores.
-template <class T>
-__device__ __forceinline__ void finish(const Product<T>& a, int64_t i, int j, const float* s) {
-  const int n = min(4, a.J - j);
-  float v[4], b[4] = {0.f, 0.f, 0.f, 0.f}, r[4] = {0.f, 0.f, 0.f, 0.f};
-  T* const o = a.out + i * a.J + j;
-  if (a.wide) {  // J a multiple of four
-    if (a.bias) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) b[q] = get(a.bias + j + q);
-    }
-    if (a.res) {
-      const T* const p = a.res + i * a.ldr + j;
-      if constexpr (sizeof(T) == 4) {
-        const v4f w = *reinterpret_cast<const v4f*>(p);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) r[q] = w[q];
-      } else {
-        const u2 w = *reinterpret_cast<const u2*>(p);
-        r[0] = bf_lo(w.x), r[1] = bf_hi(w.x), r[2] = bf_lo(w.y), r[3] = bf_hi(w.y);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (q >= n) continue;
-      if (a.bias) b[q] = get(a.bias + j + q);
-      if (a.res) r[q] = get(a.res + i * a.ldr + j + q);
-    }
-  }
-  float z[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    z[q] = a.bias ? s[q] + b[q] : s[q];
-    v[q] = activate(z[q], a.act);
-    if (a.res) v[q] += r[q];
-  }
-  if (a.wide) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<v4f*>(o) = v4f{v[0], v[1], v[2], v[3]};
-      if (a.z) *reinterpret_cast<v4f*>(a.z + i * a.J + j) = v4f{z[0], z[1], z[2], z[3]};
-    } else {
-      *reinterpret_cast<u2*>(o) = u2{bf_pack(v[0], v[1]), bf_pack(v[2], v[3])};
-      if (a.z)
-        *reinterpret_cast<u2*>(a.z + i * a.J + j) = u2{bf_pack(z[0], z[1]), bf_pack(z[2], z[3])};
-    }
-    return;
-  }
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (q >= n) continue;
-    put(o + q, v[q]);
-    if (a.z) put(a.z + i * a.J + j + q, z[q]);
   }
 }
 
@@ -406,95 +285,231 @@ __global__ __launch_bounds__(LNT) void k_join(Product<T> a) {
   }
 }
 
-// dz = dy act'(z), and the columns' sums of each block of rows.
+// Eight values j .. j + 7 of a row of n, as floats; past the end zero.
+template <class T>
+__device__ __forceinline__ void load8(const T* p, int j, int n, bool wide, float* o) {
+  if (wide && j + 8 <= n) {
+    if constexpr (sizeof(T) == 4) {
+      const v4f a = *reinterpret_cast<const v4f*>(p + j), b = *reinterpret_cast<const v4f*>(p + j + 4);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] = a[q], o[4 + q] = b[q];
+    } else {
+      const u4 a = *reinterpret_cast<const u4*>(p + j);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[2 * q] = bf_lo(a[q]), o[2 * q + 1] = bf_hi(a[q]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) o[q] = j + q < n ? get(p + j + q) : 0.f;
+}
+
+// Eight values as 16 bytes of each part, part p at p planes.
+template <class T>
+__device__ __forceinline__ void store_parts(const float* v, uint16_t* to, int64_t plane) {
+  u4 h, m, l;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t a, b, c;
+      cut2(v[2 * q], v[2 * q + 1], a, b, c);
+      h[q] = a, m[q] = b, l[q] = c;
+    } else {
+      h[q] = bf_pack(v[2 * q], v[2 * q + 1]);
+    }
+  }
+  *reinterpret_cast<u4*>(to) = h;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<u4*>(to + plane) = m;
+    *reinterpret_cast<u4*>(to + 2 * plane) = l;
+  }
+}
+
+// Up to two matrices as parts for the tiled products, their lines padded with
+// zeros to a multiple of eight.
+template <class T>
+struct Pack {
+  const T* p;
+  int64_t ld, rows;
+  int n, np, wide;  // values of a line, and with its padding
+  uint16_t* to;
+};
+
+template <class T>
+__global__ __launch_bounds__(LNT) void k_pack(Pack<T> a, Pack<T> b, int64_t split) {
+  const bool second = blockIdx.x >= split;
+  const Pack<T> m = second ? b : a;
+  const int64_t t = (blockIdx.x - (second ? split : 0)) * (int64_t)LNT + threadIdx.x;
+  const int c = m.np / 8;
+  const int64_t row = t / c;
+  if (row >= m.rows) return;
+  const int j = (int)(t - row * c) * 8;
+  float v[8];
+  load8(m.p + row * m.ld, j, m.n, m.wide, v);
+  store_parts<T>(v, m.to + row * m.np + j, m.rows * m.np);
+}
+
+// dz = dy act'(z), and the columns' sums of each block of rows.  dz as values, or
+// as parts for the tiled products (lines of np values, zeros past N).
 template <class T>
 struct Slope {
   const T *dy, *z;
   int64_t ldy, ldz;
-  T* dz;        // null: sums only
-  float* sums;  // (blocks of rows, N), or null
+  T* dz;           // lines of N, or null
+  uint16_t* parts; // or null
+  float* sums;     // (blocks of rows, N), or null
   int64_t M;
-  int N, act, rows;
+  int N, np, act, rows, wide;
 };
 
-constexpr int kSlopeCols = 64;  // columns of a workgroup, its four waves take every fourth row
+constexpr int kSlopeCols = 256;  // of a workgroup: eight a thread, eight rows at a time
 
 template <class T>
 __global__ __launch_bounds__(LNT) void k_slope(Slope<T> a) {
-  __shared__ float part[4][kSlopeCols];
-  const int c = threadIdx.x & 63, y = threadIdx.x >> 6;
-  const int j = blockIdx.x * kSlopeCols + c;
+  __shared__ float part[8][kSlopeCols + 8];
+  const int c = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int j = blockIdx.x * kSlopeCols + 8 * c;
   const int64_t m0 = (int64_t)blockIdx.y * a.rows;
   const int64_t m1 = m0 + a.rows < a.M ? m0 + a.rows : a.M;
-  float sum = 0.f;
-  if (j < a.N)
-    for (int64_t m = m0 + y; m < m1; m += 4) {
-      float d = get(a.dy + m * a.ldy + j);
-      if (a.act != kNone) d *= slope(get(a.z + m * a.ldz + j), a.act);
-      if (a.dz) put(a.dz + m * a.N + j, d);
-      sum += d;
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (j < a.N) {
+    for (int64_t m = m0 + y; m < m1; m += 32) {  // four rows' loads before the first is used
+      float d[4][8], z[4][8];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t r = m + 8 * q < m1 ? m + 8 * q : m;
+        load8(a.dy + r * a.ldy, j, a.N, a.wide, d[q]);
+        if (a.act != kNone) load8(a.z + r * a.ldz, j, a.N, a.wide, z[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t r = m + 8 * q;
+        if (r >= m1) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (a.act != kNone) d[q][i] *= slope(z[q][i], a.act);
+          sum[i] += d[q][i];
+        }
+        if (a.parts) store_parts<T>(d[q], a.parts + r * a.np + j, a.M * a.np);
+        if (a.dz) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (j + i < a.N) put(a.dz + r * a.N + j + i, d[q][i]);
+        }
+      }
     }
-  part[y][c] = sum;
+  }
+  if (!a.sums) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[y][8 * c + i] = sum[i];
   __syncthreads();
-  if (a.sums && y == 0 && j < a.N)
-    a.sums[(int64_t)blockIdx.y * a.N + j] = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
+  const int k = blockIdx.x * kSlopeCols + threadIdx.x;
+  if (k >= a.N) return;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += part[i][threadIdx.x];
+  a.sums[(int64_t)blockIdx.y * a.N + k] = s;
 }
 
+// The blocks' sums joined: 32 columns a workgroup, eight threads a column.
 template <class T>
 __global__ __launch_bounds__(LNT) void k_slope_join(const float* sums, int blocks, int N, T* db) {
-  const int j = blockIdx.x * LNT + threadIdx.x;
-  if (j >= N) return;
+  __shared__ float part[8][32];
+  const int c = threadIdx.x & 31, y = threadIdx.x >> 5, j = blockIdx.x * 32 + c;
   float s = 0.f;
-  for (int b = 0; b < blocks; ++b) s += sums[(int64_t)b * N + j];
+  if (j < N)
+    for (int b = y; b < blocks; b += 8) s += sums[(int64_t)b * N + j];
+  part[y][c] = s;
+  __syncthreads();
+  if (y || j >= N) return;
+  for (int i = 1; i < 8; ++i) s += part[i][c];
   put(db + j, s);
 }
 
-int cu_count() {
-  static int n[16];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess) return 256;
-  const int at = dev & 15;
-  if (!n[at]) {
-    int v = 0;
-    if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v < 1)
-      v = 256;
-    n[at] = v;
-  }
-  return n[at];
-}
+int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
+constexpr int64_t kCus = 256;
 
-// How a product is cut: tiles of 128 where they fill the chip, else of 64, and
-// slices of k where those do not either.
+// How a product is cut: the kernel (shape -1: k_product, else k_tile's) and the
+// slices of k, by the time that they are expected to take.
 struct Cut {
-  int tile, slices, steps;
+  int shape, slices, steps;
   int64_t tiles, nj;
 };
 
-Cut cut(int type, int64_t I, int64_t J, int64_t K) {
-  const int kstep = type == VC_FP32 ? 32 : 64;
-  const int64_t all = (K + kstep - 1) / kstep, cus = 256;
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+Cut cut_general(int type, int64_t I, int64_t J, int64_t K) {
+  const int64_t all = div_up(K, type == VC_FP32 ? 32 : 64);
   Cut c;
-  const int64_t t128 = ((I + 127) / 128) * ((J + 127) / 128);
-  c.tile = t128 >= cus ? 128 : 64;
-  c.nj = (J + c.tile - 1) / c.tile;
-  c.tiles = ((I + c.tile - 1) / c.tile) * c.nj;
+  c.shape = -1;
+  c.nj = div_up(J, 64);
+  c.tiles = div_up(I, 64) * c.nj;
   int64_t s = 1;
-  if (c.tiles < cus && all >= 16) {
-    s = cus / c.tiles;
+  if (c.tiles < kCus && all >= 16) {
+    s = kCus / c.tiles;
     if (s > all / 8) s = all / 8;
     if (s > 64) s = 64;
   }
-  c.steps = (int)((all + s - 1) / s);
+  c.steps = (int)div_up(all, s);
   if (c.steps < 1) c.steps = 1;
-  c.slices = (int)((all + c.steps - 1) / c.steps);
+  c.slices = (int)div_up(all, c.steps);
   if (c.slices < 1) c.slices = 1;
   return c;
 }
 
-int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+// Of the tiled kernels: a step of one tile alone on a CU, and of each of several
+// that share one (us, measured on 264 x 328 and 8192 x 16384 outputs).
+constexpr float kStepAlone[2][3] = {{2.0f, 1.5f, 0.50f}, {2.1f, 1.0f, 0.45f}};
+constexpr float kStepShared[2][3] = {{2.7f, 1.54f, 0.46f}, {2.2f, 0.55f, 0.21f}};
+constexpr int kShare[2][3] = {{1, 1, 3}, {1, 2, 4}};
+
+Cut cut_tiles(int type, int64_t I, int64_t J, int64_t K) {
+  Cut best = {};
+  float least = 1e30f;
+  for (int shape = 0; shape < 3; ++shape) {
+    const TileShape t = tile_shape(type, shape);
+    const int b = type == VC_FP32 ? 0 : 1;
+    const int64_t all = div_up(K, t.bk), nj = div_up(J, t.bj), tiles = div_up(I, t.bi) * nj;
+    for (int64_t want = 1; want <= 16 && want <= all; want *= 2) {
+      const int64_t steps = div_up(all, want), slices = div_up(all, steps);
+      const int64_t load = div_up(tiles * slices, kCus);
+      const float alone = kStepAlone[b][shape] * div_up(load, kShare[b][shape]);
+      const float shared = kStepShared[b][shape] * load;
+      float us = steps * (alone > shared ? alone : shared);
+      // the slices' sums written, read again and joined by a launch
+      if (slices > 1) us += 4.f + 8.f * slices * I * J / 4e6f;
+      if (us < least) {
+        least = us;
+        best = {shape, (int)slices, (int)steps, tiles, nj};
+      }
+    }
+  }
+  return best;
+}
+
+// Which products are tiled: those whose time the tiles cut by more than their
+// parts' pass and its launch cost.
+bool tiled(int type, int64_t M, int64_t K, int64_t N) {
+  return K > 0 && (double)M * K * N >= (type == VC_FP32 ? 3e8 : 1.5e8) && K < (1 << 21) &&
+         N < (1 << 21);
+}
+
+Cut cut(int type, int64_t I, int64_t J, int64_t K, bool tiles) {
+  return tiles ? cut_tiles(type, I, J, K) : cut_general(type, I, J, K);
+}
 
 int64_t part_bytes(const Cut& c, int64_t I, int64_t J) {
   return c.slices > 1 ? up256(4 * c.slices * I * J) : 0;
+}
+
+// A matrix of `rows` lines as parts, and whether it has to be made into them.
+template <class T>
+bool as_it_is(const T* p, int64_t ld, int64_t n) {
+  return sizeof(T) == 2 && aligned16(p) && ld % 8 == 0 && n % 8 == 0 && ld < (1 << 21);
+}
+int64_t parts_bytes(int type, int64_t rows, int64_t n) {
+  return up256((type == VC_FP32 ? 6 : 2) * rows * up8(n));
 }
 
 template <class T>
@@ -511,41 +526,70 @@ bool quads(const void* p, int64_t ld) {
 }
 
 template <class T, bool XA, bool XB>
-int run_product(Product<T> a, void* work, int64_t work_bytes, hipStream_t st) {
-  constexpr int type = sizeof(T) == 4 ? VC_FP32 : VC_BF16;
+int run_product(Product<T> a, const Cut& c, void* work, int64_t work_bytes, hipStream_t st) {
   if (a.I == 0 || a.J == 0) return VC_OK;
-  const Cut c = cut(type, a.I, a.J, a.K);
   if (c.tiles > (1ll << 23)) return VC_ERR_UNSUPPORTED;  // threads of a grid axis: below 2^32
   if (part_bytes(c, a.I, a.J) > work_bytes) return VC_ERR_OOM;
-  a.A.vec = XA ? wide_across(a.A.p, a.A.ld, a.A.rows) : wide_rows(a.A.p, a.A.ld, a.K);
-  a.B.vec = XB ? wide_across(a.B.p, a.B.ld, a.B.rows) : wide_rows(a.B.p, a.B.ld, a.K);
   a.wide = a.J % 4 == 0 && quads<T>(a.out, a.J) && quads<T>(a.z, a.J) && quads<T>(a.res, a.ldr);
   a.slices = c.slices;
   a.steps = c.steps;
   a.part = (float*)work;
   a.tiles = c.tiles;
   a.f_nj = vcg::FastDiv::make((uint32_t)c.nj);
-  const dim3 grid((unsigned)c.tiles, (unsigned)c.slices);
-  if (c.tile == 128) k_product<T, XA, XB, 128, 128><<<grid, LNT, 0, st>>>(a);
-  else k_product<T, XA, XB, 64, 64><<<grid, LNT, 0, st>>>(a);
+  if (c.shape >= 0) {
+    run_tiles<T>(a, c.shape, XA, XB, st);
+  } else {
+    a.A.vec = XA ? wide_across(a.A.p, a.A.ld, a.A.rows) : wide_rows(a.A.p, a.A.ld, a.K);
+    a.B.vec = XB ? wide_across(a.B.p, a.B.ld, a.B.rows) : wide_rows(a.B.p, a.B.ld, a.K);
+    k_product<T, XA, XB, 64, 64><<<dim3((unsigned)c.tiles, (unsigned)c.slices), LNT, 0, st>>>(a);
+  }
   if (c.slices > 1) {
     const int64_t n = (int64_t)a.I * ((a.J + 3) / 4);
-    int64_t blocks = (n + LNT - 1) / LNT;
-    if (blocks > 4096) blocks = 4096;
-    k_join<T><<<(unsigned)blocks, LNT, 0, st>>>(a);
+    const int64_t blocks = div_up(n, LNT);
+    k_join<T><<<(unsigned)(blocks < 4096 ? blocks : 4096), LNT, 0, st>>>(a);
   }
   VC_LAUNCH_CHECK();
   return VC_OK;
+}
+
+template <class T>
+void run_pack(Pack<T> a, Pack<T> b, hipStream_t st) {
+  const int64_t na = a.to ? div_up(a.rows * (a.np / 8), LNT) : 0;
+  const int64_t nb = b.to ? div_up(b.rows * (b.np / 8), LNT) : 0;
+  a.wide = aligned16(a.p) && a.ld % (16 / (int)sizeof(T)) == 0;
+  b.wide = aligned16(b.p) && b.ld % (16 / (int)sizeof(T)) == 0;
+  if (na + nb > 0) k_pack<T><<<(unsigned)(na + nb), LNT, 0, st>>>(a, b, na);
 }
 
 bool sizes_ok(int64_t M, int K, int N) {
   return M >= 0 && M <= 0x7fffff00 && K >= 0 && K <= 0x7fffff00 && N >= 0 && N <= 0x7fffff00;
 }
 
+struct ForwardPlan {
+  bool tiles;
+  Cut c;
+  int64_t x, W, part, bytes;  // offsets in the workspace, and its size
+};
+
+ForwardPlan plan_forward(int type, int64_t M, int K, int N) {
+  ForwardPlan p;
+  p.tiles = tiled(type, M, K, N);
+  p.c = cut(type, M, N, K, p.tiles);
+  p.x = 0;
+  p.W = p.tiles ? parts_bytes(type, M, K) : 0;
+  p.part = p.W + (p.tiles ? parts_bytes(type, N, K) : 0);
+  p.bytes = p.part + part_bytes(p.c, M, N);
+  return p;
+}
+
 template <class T>
 int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, const void* bias,
             int act, const void* res, int64_t ldr, void* y, void* z, void* work,
             int64_t work_bytes, hipStream_t st) {
+  constexpr int type = sizeof(T) == 4 ? VC_FP32 : VC_BF16;
+  const ForwardPlan p = plan_forward(type, M, K, N);
+  if (p.bytes > work_bytes || (p.bytes && !work)) return VC_ERR_OOM;
+  char* const base = (char*)work;
   Product<T> a = {};
   a.A = {(const T*)x, ldx, (int)M, 0};
   a.B = {(const T*)W, K, N, 0};
@@ -558,35 +602,57 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
   a.out = (T*)y;
   a.z = (T*)z;
   a.act = act;
-  return run_product<T, false, false>(a, work, work_bytes, st);
+  if (p.tiles) {
+    const int kp = (int)up8(K);
+    Pack<T> px = {}, pw = {};
+    if (!as_it_is((const T*)x, ldx, K)) px = {(const T*)x, ldx, M, K, kp, 0, (uint16_t*)(base + p.x)};
+    if (!as_it_is((const T*)W, K, K)) pw = {(const T*)W, K, N, K, kp, 0, (uint16_t*)(base + p.W)};
+    run_pack(px, pw, st);
+    a.pa = px.to ? px.to : (const uint16_t*)x;
+    a.lda = px.to ? kp : ldx;
+    a.planeA = M * kp;
+    a.pb = pw.to ? pw.to : (const uint16_t*)W;
+    a.ldb = kp;
+    a.planeB = (int64_t)N * kp;
+    a.K = kp;
+  }
+  return run_product<T, false, false>(a, p.c, base + p.part, work_bytes - p.part, st);
 }
 
 // Rows of a block of k_slope: at most 256 blocks.
 int slope_rows(int64_t M) {
-  int64_t r = (M + 255) / 256;
+  const int64_t r = (M + 255) / 256;
   return (int)(r < 64 ? 64 : r);
 }
 
 struct BackwardPlan {
+  bool tiles;
+  Cut cx, cw;
   int rows, blocks;
-  int64_t dz, sums, part, bytes;  // offsets in the workspace, and its size
+  int64_t dz, W, x, sums, part, bytes;  // offsets in the workspace, and its size
 };
 
 BackwardPlan plan_backward(int type, int64_t M, int K, int N, int act, int need) {
   BackwardPlan p;
   const int64_t e = type == VC_FP32 ? 4 : 2;
+  p.tiles = tiled(type, M, K, N);
+  p.cx = cut(type, M, K, N, p.tiles);
+  p.cw = cut(type, N, K, M, p.tiles);
   p.rows = slope_rows(M);
-  p.blocks = (int)((M + p.rows - 1) / p.rows);
+  p.blocks = (int)div_up(M, p.rows);
   p.dz = 0;
-  p.sums = act != kNone && (need & 3) ? up256(e * M * N) : 0;
-  p.part = p.sums + (need & 4 ? up256(4ll * p.blocks * N) : 0);
-  int64_t most = 0;
-  if (need & 1) most = part_bytes(cut(type, M, K, N), M, K);
-  if (need & 2) {
-    const int64_t b = part_bytes(cut(type, N, K, M), N, K);
-    if (b > most) most = b;
-  }
-  p.bytes = p.part + most;
+  int64_t at = 0;
+  if (need & 3) at += p.tiles ? parts_bytes(type, M, N) : act != kNone ? up256(e * M * N) : 0;
+  p.W = at;
+  if ((need & 1) && p.tiles) at += parts_bytes(type, N, K);
+  p.x = at;
+  if ((need & 2) && p.tiles) at += parts_bytes(type, M, K);
+  p.sums = at;
+  if (need & 4) at += up256(4ll * p.blocks * N);
+  p.part = at;
+  int64_t most = need & 1 ? part_bytes(p.cx, M, K) : 0;
+  const int64_t b = need & 2 ? part_bytes(p.cw, N, K) : 0;
+  p.bytes = at + (b > most ? b : most);
   return p;
 }
 
@@ -599,43 +665,85 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
   const BackwardPlan p = plan_backward(type, M, K, N, act, need);
   if (p.bytes > work_bytes || (p.bytes && !work)) return VC_ERR_OOM;
   char* const base = (char*)work;
-  const T* dz = (const T*)dy;
-  int64_t ldd = ldy;
-  const bool write = act != kNone && (need & 3);
-  if (N > 0 && M > 0 && (write || db)) {
-    Slope<T> s = {(const T*)dy, (const T*)z, ldy, ldz, write ? (T*)(base + p.dz) : nullptr,
-                  db ? (float*)(base + p.sums) : nullptr, M, N, act, p.rows};
-    k_slope<T><<<dim3((unsigned)((N + kSlopeCols - 1) / kSlopeCols), (unsigned)p.blocks), LNT, 0, st>>>(s);
+  const int np = (int)up8(N), kp = (int)up8(K);
+  // dy itself is dz where nothing is between them and the products can read it
+  const bool made = (need & 3) && (act != kNone || (p.tiles && !as_it_is((const T*)dy, ldy, N)));
+  if (N > 0 && M > 0 && (made || db)) {
+    Slope<T> s = {};
+    s.dy = (const T*)dy;
+    s.z = (const T*)z;
+    s.ldy = ldy;
+    s.ldz = ldz;
+    if (made && p.tiles) s.parts = (uint16_t*)(base + p.dz);
+    else if (made) s.dz = (T*)(base + p.dz);
+    s.sums = db ? (float*)(base + p.sums) : nullptr;
+    s.M = M;
+    s.N = N;
+    s.np = np;
+    s.act = act;
+    s.rows = p.rows;
+    const int per = 16 / (int)sizeof(T);
+    s.wide = aligned16(dy) && ldy % per == 0 && (act == kNone || (aligned16(z) && ldz % per == 0));
+    k_slope<T><<<dim3((unsigned)div_up(N, kSlopeCols), (unsigned)p.blocks), LNT, 0, st>>>(s);
   }
   if (db && N > 0)
-    k_slope_join<T><<<(unsigned)((N + LNT - 1) / LNT), LNT, 0, st>>>((float*)(base + p.sums), p.blocks,
-                                                                   N, (T*)db);
+    k_slope_join<T><<<(unsigned)div_up(N, 32), LNT, 0, st>>>((float*)(base + p.sums), p.blocks, N,
+                                                             (T*)db);
   VC_LAUNCH_CHECK();
-  if (write) {
-    dz = (const T*)(base + p.dz);
-    ldd = N;
+  Product<T> a = {};
+  if (p.tiles && (need & 3)) {
+    Pack<T> pw = {}, px = {};
+    if (dx && !as_it_is((const T*)W, K, K)) pw = {(const T*)W, K, N, K, kp, 0, (uint16_t*)(base + p.W)};
+    if (dW && !as_it_is((const T*)x, ldx, K)) px = {(const T*)x, ldx, M, K, kp, 0, (uint16_t*)(base + p.x)};
+    run_pack(pw, px, st);
+    a.pa = made ? (const uint16_t*)(base + p.dz) : (const uint16_t*)dy;
+    a.lda = made ? np : ldy;
+    a.planeA = M * np;
+    if (dx) {
+      a.pb = pw.to ? pw.to : (const uint16_t*)W;
+      a.ldb = kp;
+      a.planeB = (int64_t)N * kp;
+    }
+    if (dx) {
+      a.I = (int)M;
+      a.J = K;
+      a.K = N;
+      a.out = (T*)dx;
+      const int rc = run_product<T, false, true>(a, p.cx, base + p.part, work_bytes - p.part, st);
+      if (rc != VC_OK) return rc;
+    }
+    if (dW) {
+      a.pb = px.to ? px.to : (const uint16_t*)x;
+      a.ldb = px.to ? kp : ldx;
+      a.planeB = M * kp;
+      a.I = N;
+      a.J = K;
+      a.K = (int)M;
+      a.out = (T*)dW;
+      return run_product<T, true, true>(a, p.cw, base + p.part, work_bytes - p.part, st);
+    }
+    return VC_OK;
   }
-  const int64_t left = work_bytes - p.part;
+  const T* const dz = made ? (const T*)(base + p.dz) : (const T*)dy;
+  const int64_t ldd = made ? N : ldy;
   if (dx) {
-    Product<T> a = {};
     a.A = {dz, ldd, (int)M, 0};
     a.B = {(const T*)W, K, K, 0};
     a.I = (int)M;
     a.J = K;
     a.K = N;
     a.out = (T*)dx;
-    const int rc = run_product<T, false, true>(a, base + p.part, left, st);
+    const int rc = run_product<T, false, true>(a, p.cx, base + p.part, work_bytes - p.part, st);
     if (rc != VC_OK) return rc;
   }
   if (dW) {
-    Product<T> a = {};
     a.A = {dz, ldd, N, 0};
     a.B = {(const T*)x, ldx, K, 0};
     a.I = N;
     a.J = K;
     a.K = (int)M;
     a.out = (T*)dW;
-    return run_product<T, true, true>(a, base + p.part, left, st);
+    return run_product<T, true, true>(a, p.cw, base + p.part, work_bytes - p.part, st);
   }
   return VC_OK;
 }
@@ -649,7 +757,7 @@ bool known(int type, int act) {
 extern "C" int64_t vc_linear_workspace(int type, int64_t M, int K, int N) {
   if (!known(type, kNone) || !sizes_ok(M, K, N)) return -1;
   if (M == 0 || N == 0) return 0;
-  return part_bytes(cut(type, M, N, K), M, N);
+  return plan_forward(type, M, K, N).bytes;
 }
 
 extern "C" int vc_linear(int type, const void* x, int64_t M, int K, int64_t ldx, const void* W,

@@ -1,0 +1,307 @@
+// The fc layer's large products: tiles of up to 256 x 256, both operands as bf16
+// (an fp32 value as three parts, vc_linear.hip) brought into LDS by loads that
+// pass no register.
+//
+// A step of BK goes into one of two LDS buffers while the other is multiplied;
+// one barrier a step.  A load instruction writes 1 KB of LDS in lane order, so
+// the order that spreads a fragment's reads over the banks is made by which
+// address each lane reads from:
+//   k contiguous: [row][BK], 16-byte chunk c of row r at c ^ (r mod 8) (BK 64) or
+//     c ^ (r / 2 mod 4) (BK 32); a lane's fragment is one 16-byte read;
+//   read across: [k][row], 32-byte chunk c of line k at c ^ f(k), f = k mod 4 + 4
+//     (k / 8 mod 2); two 8-byte transposing reads give a lane its eight k.
+// 256 x 256 by eight waves of 128 x 64: a step of 64 is 1,024 cycles of a wave's
+// matrix instructions against 192 KB of fragment reads a workgroup.
+#include "vc_linear.h"
+
+namespace {
+
+using namespace vcl;
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef uint32_t u8w __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) char LdsChar;
+typedef __attribute__((address_space(3))) v4s LdsV4s;
+
+// Tile w of ni x nj, eight tile rows at a time, so that tiles close in time share
+// both operands in an XCD's L2.
+__device__ __forceinline__ void tile_of(int64_t w, int ni, int nj, int& ti, int& tj) {
+  const int64_t per = 8ll * nj;
+  const int band = (int)(w / per), r = (int)(w - band * per), rows = min(8, ni - 8 * band);
+  tj = r / rows;
+  ti = 8 * band + r - tj * rows;
+}
+
+// One operand's side of a tile: R rows, NW waves.
+template <bool X, int R, int BK, int NW>
+struct Side {
+  static constexpr int kGroups = R * BK * 2 / 1024;  // load instructions of one plane's step
+  static constexpr int kOwn = kGroups / NW;
+  static constexpr int kBytes = R * BK * 2;
+  static_assert(kGroups % NW == 0, "every wave issues as many loads");
+  const uint16_t* base;  // of the tile's first row and k
+  uint32_t off[kOwn];    // bytes
+
+  static __device__ __forceinline__ int fold(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) & (R / 16 - 1); }
+
+  // Which chunk of which row (across: of which line k) the lane brings in by its i-th load.
+  static __device__ __forceinline__ void at(int i, int wv, int lane, int& line, int& chunk) {
+    const int n = i * NW + wv;
+    if (X) {
+      constexpr int CR = R / 8;
+      line = n * (64 / CR) + lane / CR;
+      const int pos = lane % CR;
+      chunk = ((pos >> 1) ^ fold(line)) * 2 + (pos & 1);
+    } else {
+      constexpr int CR = BK / 8;
+      line = n * (64 / CR) + lane / CR;
+      const int pos = lane % CR;
+      chunk = pos ^ (BK == 64 ? line & 7 : (line >> 1) & 3);
+    }
+  }
+
+  __device__ __forceinline__ void init(const uint16_t* p, int64_t ld, int rows, int r0, int64_t k0,
+                                       int wv, int lane) {
+    base = X ? p + k0 * ld + r0 : p + (int64_t)r0 * ld + k0;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      int line, chunk;
+      at(i, wv, lane, line, chunk);
+      // past the last row the last again: its products are not stored
+      if (X) off[i] = (uint32_t)(line * ld * 2) + min(chunk * 8, rows - 8 - r0) * 2;
+      else off[i] = (uint32_t)(min(line, rows - 1 - r0) * ld * 2) + chunk * 16;
+    }
+  }
+
+  // Whole steps: straight into LDS.
+  __device__ __forceinline__ void issue(const uint16_t* from, char* lds, int wv) const {
+    const Buf b = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(from), 0, 0x7fffffff,
+                                                    0x00027000);
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          b, (__attribute__((address_space(3))) void*)(lds + (i * NW + wv) * 1024), 16, (int)off[i],
+          0, 0, 0);
+  }
+
+  // The last step where K does not fill it (left < BK of it): zeros past the end.
+  __device__ __forceinline__ void tail(const uint16_t* from, char* lds, int wv, int lane,
+                                       int left) const {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      int line, chunk;
+      at(i, wv, lane, line, chunk);
+      const bool in = X ? line < left : chunk * 8 < left;
+      u4 v = u4{0, 0, 0, 0};
+      if (in) v = *reinterpret_cast<const u4*>(reinterpret_cast<const char*>(from) + off[i]);
+      *reinterpret_cast<u4*>(lds + (i * NW + wv) * 1024 + lane * 16) = v;
+    }
+  }
+
+  // The fragment of 16 rows from row0 (a multiple of 16), k = 32 ks + 8 g + 0 .. 7.
+  static __device__ __forceinline__ v8bf frag(const char* lds, int row0, int ks, int lane) {
+    const int g = lane >> 4, r = lane & 15;
+    if (X) {
+      const int k = ks * 32 + 8 * g + (r >> 2);
+      const char* const p = lds + k * (R * 2) + ((row0 >> 4) ^ fold(k)) * 32 + (r & 3) * 8;
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(LdsChar*)p);
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(LdsChar*)(p + 4 * R * 2));
+      return __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    const int c = (ks * 4 + g) ^ (BK == 64 ? r & 7 : (r >> 1) & 3);
+    return *reinterpret_cast<const v8bf*>(lds + (row0 + r) * (BK * 2) + c * 16);
+  }
+};
+
+template <class T, int NP, bool XA, bool XB, int BI, int BJ, int WI, int WJ, int BK>
+__global__ __launch_bounds__(64 * WI * WJ, 2) void k_tile(Product<T> a) {
+  constexpr int NW = WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16;
+  typedef Side<XA, BI, BK, NW> SA;
+  typedef Side<XB, BJ, BK, NW> SB;
+  constexpr int kStage = NP * (SA::kBytes + SB::kBytes);
+  extern __shared__ __align__(1024) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ni = (a.I + BI - 1) / BI, nj = (a.J + BJ - 1) / BJ;
+  int ti, tj;
+  tile_of(vcg::xcd_tile(blockIdx.x, a.tiles), ni, nj, ti, tj);
+  const int i0 = ti * BI, j0 = tj * BJ;
+  const int64_t k0 = (int64_t)blockIdx.y * a.steps * BK;
+  const int left = (int)min((int64_t)a.steps * BK, a.K - k0);
+  const int full = left / BK;
+  const int wi = wv / WJ, wj = wv % WJ;
+
+  SA sa;
+  SB sb;
+  // a line that is read across is padded to whole chunks
+  sa.init(a.pa, a.lda, XA ? (a.I + 7) & ~7 : a.I, i0, k0, wv, lane);
+  sb.init(a.pb, a.ldb, XB ? (a.J + 7) & ~7 : a.J, j0, k0, wv, lane);
+
+  v4f acc[MI][MJ], small[NP == 3 ? MI : 1][NP == 3 ? MJ : 1];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) {
+      acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+      if (NP == 3) small[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+
+  const auto load = [&](int s, char* to) {
+    const uint16_t* const fa = sa.base + (XA ? (int64_t)s * BK * a.lda : (int64_t)s * BK);
+    const uint16_t* const fb = sb.base + (XB ? (int64_t)s * BK * a.ldb : (int64_t)s * BK);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      sa.issue(fa + p * a.planeA, to + p * SA::kBytes, wv);
+      sb.issue(fb + p * a.planeB, to + NP * SA::kBytes + p * SB::kBytes, wv);
+    }
+  };
+  const auto multiply = [&](const char* from) {
+#pragma unroll
+    for (int ks = 0; ks < BK / 32; ++ks) {
+      v8bf fb[MJ][NP], fa[NP == 3 ? 1 : MI][NP];
+#pragma unroll
+      for (int j = 0; j < MJ; ++j)
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          fb[j][p] = SB::frag(from + NP * SA::kBytes + p * SB::kBytes, (wj * MJ + j) * 16, ks, lane);
+      if (NP == 1) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[i][0] = SA::frag(from, (wi * MI + i) * 16, ks, lane);
+      }
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        v8bf f[NP];
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          f[p] = NP == 1 ? fa[i][0] : SA::frag(from + p * SA::kBytes, (wi * MI + i) * 16, ks, lane);
+        if constexpr (NP == 1) {
+#pragma unroll
+          for (int j = 0; j < MJ; ++j) acc[i][j] = mfma_bf16(fb[j][0], f[0], acc[i][j]);
+        } else {
+#pragma unroll
+          for (int p = 0; p < 5; ++p)
+#pragma unroll
+            for (int j = 0; j < MJ; ++j)
+              small[i][j] = mfma_bf16(fb[j][kPartA[p]], f[kPartB[p]], small[i][j]);
+#pragma unroll
+          for (int j = 0; j < MJ; ++j)
+            acc[i][j] += mfma_bf16(fb[j][0], f[0], v4f{0.f, 0.f, 0.f, 0.f});
+        }
+      }
+    }
+  };
+  if (full > 0) {
+    load(0, lds);
+#pragma unroll 1
+    for (int s = 0;; s += 2) {
+      __syncthreads();  // this step has arrived, the buffer of the one before is read
+      if (s + 1 < full) load(s + 1, lds + kStage);
+      multiply(lds);
+      if (s + 1 >= full) break;
+      __syncthreads();
+      if (s + 2 < full) load(s + 2, lds);
+      multiply(lds + kStage);
+      if (s + 2 >= full) break;
+    }
+  }
+  if (left > full * BK) {
+    const uint16_t* const fa = sa.base + (XA ? (int64_t)full * BK * a.lda : (int64_t)full * BK);
+    const uint16_t* const fb = sb.base + (XB ? (int64_t)full * BK * a.ldb : (int64_t)full * BK);
+    __syncthreads();
+#pragma unroll 1
+    for (int p = 0; p < NP; ++p) {
+      sa.tail(fa + p * a.planeA, lds + p * SA::kBytes, wv, lane, left - full * BK);
+      sb.tail(fb + p * a.planeB, lds + NP * SA::kBytes + p * SB::kBytes, wv, lane, left - full * BK);
+    }
+    __syncthreads();
+    multiply(lds);
+  }
+
+  const int g = lane >> 4, r = lane & 15;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int64_t row = i0 + (wi * MI + i) * 16 + r;
+    if (row >= a.I) continue;
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) {
+      const int col = j0 + (wj * MJ + j) * 16 + 4 * g;
+      if (col >= a.J) continue;
+      float v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        v[q] = acc[i][j][q];
+        if (NP == 3) {
+          const float t = v[q] + small[i][j][q];
+          v[q] = finite(t) ? t : v[q];
+        }
+      }
+      if (a.slices == 1) {
+        finish(a, row, col, v);
+        continue;
+      }
+      float* const o = a.part + ((int64_t)blockIdx.y * a.I + row) * a.J + col;
+      if (a.J % 4 == 0) {
+        *reinterpret_cast<v4f*>(o) = v4f{v[0], v[1], v[2], v[3]};
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (col + q < a.J) o[q] = v[q];
+      }
+    }
+  }
+}
+
+template <class T, bool XA, bool XB, int SHAPE>
+struct Form {
+  static constexpr int NP = sizeof(T) == 4 ? 3 : 1;
+  static constexpr int BI = SHAPE == 0 ? 256 : SHAPE == 1 ? 128 : 64;
+  static constexpr int BJ = SHAPE == 0 ? (NP == 3 ? 128 : 256) : BI;
+  static constexpr int WI = SHAPE == 0 ? (NP == 3 ? 4 : 2) : 2;
+  static constexpr int WJ = SHAPE == 0 ? (NP == 3 ? 2 : 4) : 2;
+  static constexpr int BK = NP == 3 ? 32 : 64;
+  static constexpr int kThreads = 64 * WI * WJ;
+  static constexpr int kLds = 2 * NP * (BI + BJ) * BK * 2;
+  static void run(const Product<T>& a, hipStream_t st) {
+    const auto k = k_tile<T, NP, XA, XB, BI, BJ, WI, WJ, BK>;
+    static bool set[16];
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    if (!set[dev & 15]) {
+      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+      set[dev & 15] = true;
+    }
+    k<<<dim3((unsigned)a.tiles, (unsigned)a.slices), kThreads, kLds, st>>>(a);
+  }
+};
+
+template <class T, int SHAPE>
+void run_shape(const Product<T>& a, bool xa, bool xb, hipStream_t st) {
+  if (xa) Form<T, true, true, SHAPE>::run(a, st);
+  else if (xb) Form<T, false, true, SHAPE>::run(a, st);
+  else Form<T, false, false, SHAPE>::run(a, st);
+}
+
+}  // namespace
+
+namespace vcl {
+
+TileShape tile_shape(int type, int shape) {
+  const bool f = type == VC_FP32;
+  switch (shape) {
+    case 0: return f ? TileShape{256, 128, 32, 512, 0} : TileShape{256, 256, 64, 512, 0};
+    case 1: return {128, 128, f ? 32 : 64, 256, 0};
+    default: return {64, 64, f ? 32 : 64, 256, 0};
+  }
+}
+
+template <class T>
+void run_tiles(const Product<T>& a, int shape, bool xa, bool xb, hipStream_t st) {
+  if (shape == 0) run_shape<T, 0>(a, xa, xb, st);
+  else if (shape == 1) run_shape<T, 1>(a, xa, xb, st);
+  else run_shape<T, 2>(a, xa, xb, st);
+}
+template void run_tiles<float>(const Product<float>&, int, bool, bool, hipStream_t);
+template void run_tiles<uint16_t>(const Product<uint16_t>&, int, bool, bool, hipStream_t);
+
+}  // namespace vcl
