@@ -9,11 +9,11 @@
 // gradient is -S / (S + exp(z_t - m)) + e - e / V and the loss log(S + exp(z_t -
 // m)) + (m - z_t): nothing cancels where the target's probability is near one,
 // or where the logits are large beside their differences.
+#include <type_traits>
+
 #include "vc_common.h"
 
 namespace {
-
-constexpr int CNT = 256;  // threads of a row
 
 struct Rows {
   const void* z;
@@ -21,12 +21,15 @@ struct Rows {
   const int64_t* t;
   int64_t ignore;
   float smooth;
-  int mean;
-  const float* scale;  // mean: one over the rows that count
+  int mean;            // the gradient is of the mean over the rows that count
+  const float* scale;  // mean: one over their number; null: counted here
   float* loss;         // (R)
   void* dz;            // null: no gradient
   int64_t ldd;
+  float* joined;       // k_loss_few: the sum or mean, or null
 };
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ float load1(const uint16_t* p) {
@@ -36,6 +39,45 @@ __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(uint16_t* p, float v) {
   *p = __builtin_bit_cast(uint16_t, (__bf16)v);
 }
+
+typedef uint32_t u4at4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u4at2 __attribute__((ext_vector_type(4), aligned(2)));
+
+// Sixteen bytes of a row, at any alignment of its type.
+template <class T>
+struct Chunk {
+  static constexpr int kN = 16 / sizeof(T);
+  typedef std::conditional_t<sizeof(T) == 4, u4at4, u4at2> Any;
+  static __device__ __forceinline__ u4 load(const T* p) { return *reinterpret_cast<const Any*>(p); }
+  static __device__ __forceinline__ void store(T* p, u4 v) { *reinterpret_cast<Any*>(p) = v; }
+  static __device__ __forceinline__ float value(u4 w, int i) {
+    const uint32_t u = sizeof(T) == 4 ? w[i % 4] : i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16;
+    return __builtin_bit_cast(float, u);
+  }
+  static __device__ __forceinline__ u4 pack(const float* v) {
+    u4 w;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(uint32_t, v[i]);
+    } else {
+      typedef float v2f __attribute__((ext_vector_type(2)));
+      typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{v[2 * i], v[2 * i + 1]}, v2bf));
+    }
+    return w;
+  }
+  static __device__ __forceinline__ void set(u4& w, int i, uint32_t bits) {  // bits of a T
+#pragma unroll
+    for (int k = 0; k < kN; ++k) {
+      if (k != i) continue;
+      if constexpr (sizeof(T) == 4) w[k] = bits;
+      else w[k / 2] = k & 1 ? (w[k / 2] & 0xffffu) | bits << 16 : (w[k / 2] & 0xffff0000u) | bits;
+    }
+  }
+  static constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80u;  // -inf
+};
 
 constexpr float kLog2e = 1.44269504088896341f;
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
@@ -51,67 +93,295 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   m = top;
 }
 
-// others: the sum without the target's term et; half: half the logits' mean, which
-// rounding cannot take past the largest value.
-__device__ __forceinline__ float row_loss(float m, float others, float et, float zt, float half,
-                                          float e) {
-  if (m == -INFINITY && others == 0.f) return INFINITY;
-  float v = log1pf(others + (et - 1.f));
+// others: the sum without the target's term et, in units of em, the largest
+// logit's own term; half: half the logits' mean, which rounding cannot take past
+// the largest value.
+__device__ __forceinline__ float row_loss(float m, float others, float et, float em, float zt,
+                                          float half, float e) {
+  const float v = log1pf((others + (et - em)) / em);
   if (e == 0.f) return v + (m - zt);
   return v + ((1.f - e) * (m - zt) + e * (2.f * (0.5f * m - half)));
 }
 
-// One workgroup a row: a pass for the running maximum and sum, one for the
-// gradient.
-template <class T>
-__global__ __launch_bounds__(CNT) void k_loss_rows(Rows a) {
-  __shared__ float sh[3][CNT / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int64_t row = blockIdx.x;
-  const T* const z = (const T*)a.z + row * a.ld;
-  T* const dz = a.dz ? (T*)a.dz + row * a.ldd : nullptr;
-  const int64_t t = a.t[row];
-  if (t == a.ignore) {
-    if (tid == 0) a.loss[row] = 0.f;
-    if (dz)
-      for (int64_t j = tid; j < a.V; j += CNT) store1(dz + j, 0.f);
-    return;
+// Rows that one wavefront or a workgroup of W waves takes: sums and maxima over
+// its threads, each wave's part through LDS where there are several.
+template <int W>
+struct Team {
+  float (*sh)[W];
+  int lane, wv;
+  __device__ __forceinline__ float max_of(float v) {
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    if (W == 1) return v;
+    if (lane == 0) sh[0][wv] = v;
+    __syncthreads();
+    v = sh[0][0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) v = fmaxf(v, sh[0][i]);
+    return v;
   }
+  __device__ __forceinline__ void sums(float& a, float& b, bool two) {
+    a = wave_sum(a);
+    if (two) b = wave_sum(b);
+    if (W == 1) return;
+    if (lane == 0) {
+      sh[1][wv] = a;
+      sh[2][wv] = b;
+    }
+    __syncthreads();
+    a = sh[1][0];
+    b = sh[2][0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) a += sh[1][i], b += sh[2][i];
+  }
+};
+
+// One over the rows that count, by every wave for itself (few rows).
+__device__ __forceinline__ float scale_of(const Rows& a, int lane) {
+  if (!a.mean) return 1.f;
+  if (a.scale) return *a.scale;
+  int n = 0;
+  for (int64_t i = lane; i < a.R; i += 64) n += a.t[i] != a.ignore;
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+  return 1.f / (float)n;
+}
+
+// A row of any values, two passes over memory: rows without a finite largest
+// logit, or one so large that its exponent's product would not be.
+template <class T, int W>
+__device__ void plain_row(const Rows& a, const T* z, T* dz, int64_t t, float zt, int tid, float w,
+                          float* loss, Team<W> team) {
+  const float iv = 0.5f / (float)a.V;
   const bool valid = t >= 0 && t < a.V;
-  const float zt = load1(z + (valid ? t : 0)), iv = 0.5f / (float)a.V;
   float m = -INFINITY, s = 0.f, half = 0.f;
-  for (int64_t j = tid; j < a.V; j += CNT) {
+  for (int64_t j = tid; j < a.V; j += 64 * W) {
     const float v = load1(z + j);
     join(m, s, v, v == -INFINITY || j == t ? 0.f : 1.f);
     half += v * iv;
   }
-  for (int o = 32; o > 0; o >>= 1) {
-    join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
-    half += __shfl_xor(half, o, 64);
-  }
-  if (lane == 0) {
-    sh[0][wv] = m;
-    sh[1][wv] = s;
-    sh[2][wv] = half;
-  }
-  __syncthreads();  // and dz may be z: the target's logit is read
-  m = sh[0][0];
-  s = sh[1][0];
-  half = sh[2][0];
-  for (int i = 1; i < CNT / 64; ++i) {
-    join(m, s, sh[0][i], sh[1][i]);
-    half += sh[2][i];
-  }
-  const float et = exp_of(zt - m);
-  if (tid == 0) a.loss[row] = valid ? row_loss(m, s, et, zt, half, a.smooth) : NAN;
-  if (!dz) return;
+  if (W > 1) __syncthreads();
+  const float top = team.max_of(m);
+  s = top == -INFINITY ? s : s * exp_of(m - top);
+  m = top;
+  team.sums(s, half, true);  // after its barrier the target's logit may be overwritten
   const bool none = m == -INFINITY && s == 0.f;
-  const float w = a.mean ? *a.scale : 1.f;
+  const float et = exp_of(zt - m);
+  if (tid == 0) *loss = !valid ? NAN : none ? INFINITY : row_loss(m, s, et, 1.f, zt, half, a.smooth);
+  if (!dz) return;
   const float inv = 1.f / (s + et), ev = a.smooth / (float)a.V;
-  for (int64_t j = tid; j < a.V; j += CNT) {
+  for (int64_t j = tid; j < a.V; j += 64 * W) {
     const float p = j == t ? a.smooth - s * inv : exp_of(load1(z + j) - m) * inv;
     store1(dz + j, !valid ? NAN : none ? 0.f : (p - ev) * w);
   }
+}
+
+// A row is read once: its chunks stay in the team's registers, NV a thread, or
+// (NV 0, rows that do not fit) are read again for the gradient.
+//
+// While chunks arrive a thread keeps r, a whole number not below its largest
+// logit times log2 e, and the sum of 2^(z log2 e - r): one fma and one
+// exponential a value, and moving to another r multiplies by a power of two,
+// which rounds nothing.  What the rounding of log2 e does to large logits is in
+// every term, the largest's own (em) too, and cancels.  The target's term is kept
+// apart (its place holds -inf meanwhile).
+//
+// 8,192 x 131,072 bf16: see the measured times at the entry point below.
+template <class T, int W, int NV, bool SMOOTH>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
+  typedef Chunk<T> C;
+  typedef std::conditional_t<NV != 0, int, int64_t> Index;  // held rows: 32 bits beside the row's base
+  constexpr int N = C::kN, TH = 64 * W, NB = NV ? NV : 4;
+  __shared__ float sh[3][W];
+  const int tid = W == 1 ? threadIdx.x & 63 : threadIdx.x, lane = threadIdx.x & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = W == 1 ? blockIdx.x * 4ll + wv : blockIdx.x;
+  if (row >= a.R) return;
+  Team<W> team{sh, lane, wv};
+  const T* const z = (const T*)a.z + row * a.ld;
+  T* const dz = a.dz ? (T*)a.dz + row * a.ldd : nullptr;
+  const int64_t t = a.t[row];
+  // chunks; what is left over belongs to chunk `whole`
+  const Index whole = (Index)(a.V / N), chunks = (Index)((a.V + N - 1) / N);
+  if (t == a.ignore) {
+    if (tid == 0) a.loss[row] = 0.f;
+    if (dz) {
+      for (int64_t c = tid; c < whole; c += TH) C::store(dz + c * N, u4{0, 0, 0, 0});
+      for (int64_t j = whole * N + tid; j < a.V; j += TH) store1(dz + j, 0.f);
+    }
+    return;
+  }
+  const bool valid = t >= 0 && t < a.V;
+  const float zt = load1(z + (valid ? t : 0)), iv = 0.5f / (float)a.V;
+  const Index ct = valid ? (Index)(t / N) : -1;
+  const auto at = [](auto* p, Index c) {
+    typedef std::remove_pointer_t<decltype(p)> P;
+    if constexpr (NV != 0) return p + (uint32_t)c * (uint32_t)N;
+    else return (P*)p + c * N;
+  };
+  const auto fetch = [&](Index c) {
+    if (c < whole) return C::load(at(z, c));
+    u4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = sizeof(T) == 4 ? C::kNone : C::kNone | C::kNone << 16;
+    if (c == whole)
+      for (int64_t j = (int64_t)c * N; j < a.V; ++j) {
+        if constexpr (sizeof(T) == 4) C::set(w, (int)(j - (int64_t)c * N), __builtin_bit_cast(uint32_t, z[j]));
+        else C::set(w, (int)(j - (int64_t)c * N), z[j]);
+      }
+    return w;
+  };
+  float m = -INFINITY, r = -1e37f, s = 0.f, half = 0.f;
+  const auto take = [&](u4& w, Index c) {
+    if (SMOOTH) {
+      if (c < whole) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) half += C::value(w, i) * iv;
+      } else if (c == whole) {
+        for (int64_t j = (int64_t)c * N; j < a.V; ++j) half += load1(z + j) * iv;
+      }
+    }
+    if (c == ct) C::set(w, (int)(t - (int64_t)ct * N), C::kNone);
+    float top = C::value(w, 0);
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, C::value(w, i));
+    if (top > m) {
+      m = top;
+      const float to = fmaxf(ceilf(m * kLog2e), r);
+      s *= __builtin_amdgcn_exp2f(r - to);
+      r = to;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      s += __builtin_amdgcn_exp2f(__builtin_fmaf(C::value(w, i), kLog2e, -r));
+  };
+  u4 v[NB];
+  if (NV) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) v[k] = fetch(tid + k * TH);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      take(v[k], tid + k * TH);
+      __builtin_amdgcn_sched_barrier(0);  // one chunk's floats at a time
+    }
+  } else {
+    for (Index c = tid; c < chunks; c += NB * TH) {
+#pragma unroll
+      for (int k = 0; k < NB; ++k) v[k] = fetch(c + k * TH);
+#pragma unroll
+      for (int k = 0; k < NB; ++k) take(v[k], c + k * TH);
+    }
+  }
+  const float w = scale_of(a, lane);
+  const float top = team.max_of(fmaxf(m, zt));
+  if (!(fabsf(top) < 1e38f)) {  // the same in every thread of the row
+    plain_row<T, W>(a, z, dz, t, zt, tid, w, a.loss + row, team);
+    return;
+  }
+  const float to = ceilf(top * kLog2e);
+  s *= __builtin_amdgcn_exp2f(r - to);
+  r = to;
+  team.sums(s, half, SMOOTH);
+  const float em = __builtin_amdgcn_exp2f(__builtin_fmaf(top, kLog2e, -r));
+  const float et = __builtin_amdgcn_exp2f(__builtin_fmaf(zt, kLog2e, -r));
+  if (tid == 0) a.loss[row] = valid ? row_loss(top, s, et, em, zt, half, a.smooth) : NAN;
+  if (!dz) return;
+  const float inv = valid ? w / (s + et) : NAN, ev = a.smooth / (float)a.V * w;
+  const float at_t = a.smooth * w - s * inv - ev;
+  const auto give = [&](u4 x, Index c) {
+    asm volatile("" : "+v"(x));  // unpacked again here, not kept from before: twice the registers
+    float g[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(C::value(x, i), kLog2e, -r));
+      g[i] = SMOOTH ? __builtin_fmaf(p, inv, -ev) : p * inv;
+    }
+    if (c < whole) {
+      C::store(at(dz, c), C::pack(g));
+    } else if (c == whole) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if ((int64_t)c * N + i < a.V) store1(dz + (int64_t)c * N + i, g[i]);
+    }
+    if (c == ct) store1(dz + t, at_t);
+  };
+  if (NV) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      give(v[k], tid + k * TH);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  } else {
+    for (Index c = tid; c < chunks; c += NB * TH) {
+#pragma unroll
+      for (int k = 0; k < NB; ++k) v[k] = fetch(c + k * TH);
+#pragma unroll
+      for (int k = 0; k < NB; ++k) give(v[k], c + k * TH);
+    }
+  }
+}
+
+// Few classes: a thread a row, its values from the caches for each of its passes.
+// With ONE the whole call is this workgroup: the rows are counted and their
+// losses added here too.
+constexpr int kFew = 32;
+
+template <class T, int TH, bool ONE>
+__global__ __launch_bounds__(TH) void k_loss_few(Rows a) {
+  __shared__ double sums[TH / 64];
+  __shared__ int counts[TH / 64];
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x * (int64_t)TH + tid;
+  const bool in = row < a.R;
+  const int64_t t = in ? a.t[row] : 0;
+  const bool on = in && t != a.ignore, valid = t >= 0 && t < a.V;
+  float w = 1.f;
+  int count = 0;
+  if (ONE) {
+    const int n = __popcll(__ballot(on));
+    if ((tid & 63) == 0) counts[tid >> 6] = n;
+    __syncthreads();
+    for (int i = 0; i < TH / 64; ++i) count += counts[i];
+    if (a.mean) w = 1.f / (float)count;
+  } else if (a.mean) {
+    w = *a.scale;
+  }
+  float loss = 0.f;
+  const int V = (int)a.V;
+  if (on) {
+    const T* const z = (const T*)a.z + row * a.ld;
+    T* const dz = a.dz ? (T*)a.dz + row * a.ldd : nullptr;
+    const float zt = load1(z + (valid ? t : 0)), iv = 0.5f / (float)V;
+    float m = -INFINITY, s = 0.f, half = 0.f;
+    for (int j = 0; j < V; ++j) m = fmaxf(m, load1(z + j));
+    const bool none = m == -INFINITY;
+    for (int j = 0; j < V; ++j) {
+      const float v = load1(z + j);
+      half += v * iv;
+      if (j != t) s += none && v == m ? 0.f : exp_of(v - m);
+    }
+    const float et = exp_of(zt - m);
+    const bool empty = none && s == 0.f;
+    loss = !valid ? NAN : empty ? INFINITY : row_loss(m, s, et, 1.f, zt, half, a.smooth);
+    if (dz) {
+      const float inv = 1.f / (s + et), ev = a.smooth / (float)V;
+      for (int j = 0; j < V; ++j) {
+        const float p = j == t ? a.smooth - s * inv : exp_of(load1(z + j) - m) * inv;
+        store1(dz + j, !valid ? NAN : empty ? 0.f : (p - ev) * w);
+      }
+    }
+  } else if (in && a.dz) {
+    for (int j = 0; j < V; ++j) store1((T*)a.dz + row * a.ldd + j, 0.f);
+  }
+  if (!ONE || !a.joined) {
+    if (in) a.loss[row] = loss;
+    return;
+  }
+  const double sum = wave_sum_f64((double)loss);
+  if ((tid & 63) == 0) sums[tid >> 6] = sum;
+  __syncthreads();
+  if (tid) return;
+  double all = 0.0;
+  for (int i = 0; i < TH / 64; ++i) all += sums[i];
+  *a.joined = (float)(a.mean ? all / (double)count : all);
 }
 
 // scale[0] = one over the number of rows that count.
@@ -119,29 +389,73 @@ __global__ __launch_bounds__(1024) void k_loss_count(const int64_t* t, int64_t R
                                                      float* scale) {
   __shared__ int sh[16];
   int n = 0;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < R; i += 1024) n += t[i] != ignore;
   for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = n;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) n += sh[i];
-    *scale = n ? 1.f / (float)n : NAN;
+    *scale = 1.f / (float)n;
   }
 }
 
-// The rows' losses added in a fixed order, in 64 bits.
-__global__ __launch_bounds__(1024) void k_loss_sum(const float* loss, int64_t R, const float* scale,
-                                                   float* out) {
+// The rows' losses added in a fixed order, in 64 bits; averaged over the rows
+// that count.
+__global__ __launch_bounds__(1024) void k_loss_sum(const float* loss, int64_t R, const int64_t* t,
+                                                   int64_t ignore, int mean, float* out) {
   __shared__ double sh[16];
+  __shared__ int shn[16];
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < R; i += 1024) s += (double)loss[i];
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+  int n = 0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < R; i += 1024) {
+    s += (double)loss[i];
+    if (mean) n += t[i] != ignore;
+  }
+  for (int o = 32; o > 0; o >>= 1) {
+    s += __shfl_xor(s, o, 64);
+    n += __shfl_xor(n, o, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    sh[threadIdx.x >> 6] = s;
+    shn[threadIdx.x >> 6] = n;
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 16; ++i) s += sh[i];
-    *out = (float)(scale ? s * (double)*scale : s);
+    for (int i = 1; i < 16; ++i) s += sh[i], n += shn[i];
+    *out = (float)(mean ? s / (double)n : s);
   }
+}
+
+template <class T, int W, int NV>
+void run_rows(const Rows& a, hipStream_t st) {
+  const unsigned grid = (unsigned)(W == 1 ? (a.R + 3) / 4 : a.R);
+  const int threads = W == 1 ? 256 : 64 * W;
+  if (a.smooth != 0.f) k_loss_rows<T, W, NV, true><<<grid, threads, 0, st>>>(a);
+  else k_loss_rows<T, W, NV, false><<<grid, threads, 0, st>>>(a);
+}
+
+constexpr int64_t kOneRows = 1024;    // of k_loss_few by one workgroup
+constexpr int64_t kCountRows = 1024;  // that every wave counts by itself
+
+// The team of a row: as many waves as hold it in at most 16 chunks a thread.
+template <class T>
+void run_loss(const Rows& a, hipStream_t st) {
+  const int64_t c = (a.V + Chunk<T>::kN - 1) / Chunk<T>::kN;
+  if (a.V <= kFew) {
+    if (a.R <= kOneRows) k_loss_few<T, kOneRows, true><<<1, kOneRows, 0, st>>>(a);
+    else k_loss_few<T, 256, false><<<(unsigned)((a.R + 255) / 256), 256, 0, st>>>(a);
+  } else if (c <= 64) run_rows<T, 1, 1>(a, st);
+  else if (c <= 128) run_rows<T, 1, 2>(a, st);
+  else if (c <= 256) run_rows<T, 1, 4>(a, st);
+  else if (c <= 1024) run_rows<T, 4, 4>(a, st);
+  else if (c <= 2048) run_rows<T, 4, 8>(a, st);
+  else if (c <= 4096) run_rows<T, 8, 8>(a, st);
+  else if (c <= 8192) run_rows<T, 16, 8>(a, st);
+  else if (c <= 13312) run_rows<T, 16, 13>(a, st);
+  else if (c <= 16384) run_rows<T, 16, 16>(a, st);
+  else run_rows<T, 16, 0>(a, st);
 }
 
 }  // namespace
@@ -164,16 +478,20 @@ extern "C" int vc_cross_entropy(int type, const void* logits, int64_t R, int64_t
   const int64_t need = vc_cross_entropy_workspace(R, reduction);
   if (need > work_bytes || (need && !work)) return VC_ERR_OOM;
   hipStream_t st = (hipStream_t)stream;
-  float* const scale = (float*)work;
   const bool mean = reduction == VC_REDUCE_MEAN, joined = reduction != VC_REDUCE_NONE;
-  Rows a = {logits, R,    V,     ld, target, ignore, smoothing, mean, scale,
-            joined ? (float*)work + 64 : loss, dlogits, ldd};
-  if (mean) k_loss_count<<<1, 1024, 0, st>>>(target, R, ignore, scale);
-  if (R > 0) {
-    if (type == VC_FP32) k_loss_rows<float><<<(unsigned)R, CNT, 0, st>>>(a);
-    else k_loss_rows<uint16_t><<<(unsigned)R, CNT, 0, st>>>(a);
+  // with few rows of few classes one workgroup is the whole call; with few rows
+  // their number is counted by every wave, which spares a launch
+  const bool one = V <= kFew && R <= kOneRows;
+  float* const scale = mean && !one && (R > kCountRows || V <= kFew) ? (float*)work : nullptr;
+  Rows a = {logits, R,  V,    ld, target, ignore, smoothing, mean && (one || dlogits), scale,
+            joined ? (float*)work + 64 : loss, dlogits, ldd, one && joined ? loss : nullptr};
+  if (scale && dlogits) k_loss_count<<<1, 1024, 0, st>>>(target, R, ignore, scale);
+  if (R > 0 || one) {
+    if (type == VC_FP32) run_loss<float>(a, st);
+    else run_loss<uint16_t>(a, st);
   }
-  if (joined) k_loss_sum<<<1, 1024, 0, st>>>(a.loss, R, mean ? scale : nullptr, loss);
+  if (joined && !one)
+    k_loss_sum<<<1, 1024, 0, st>>>(a.loss, R, target, ignore, mean, loss);
   VC_LAUNCH_CHECK();
   return VC_OK;
 }
