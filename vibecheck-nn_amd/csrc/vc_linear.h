@@ -11,6 +11,15 @@ using namespace vcs;
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
+typedef uint32_t u4at4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u4at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u2at4 __attribute__((ext_vector_type(2), aligned(4)));
+typedef uint32_t u1at2 __attribute__((aligned(2)));
+
+// Sixteen bytes at any alignment of the type.
+__device__ __forceinline__ u4 load16(const float* p) { return *reinterpret_cast<const u4at4*>(p); }
+__device__ __forceinline__ u4 load16(const uint16_t* p) { return *reinterpret_cast<const u4at2*>(p); }
+
 enum Act { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
 
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
@@ -20,6 +29,16 @@ __device__ __forceinline__ float bf_hi(uint32_t w) {
 // Two values rounded to nearest, the first in the low half.
 __device__ __forceinline__ uint32_t bf_pack(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2bf));
+}
+
+// Two values' parts, the first cut: h + m + l is the value.
+__device__ __forceinline__ void cut2(float x0, float x1, uint32_t& h, uint32_t& m, uint32_t& l) {
+  const uint32_t b0 = __builtin_bit_cast(uint32_t, x0), b1 = __builtin_bit_cast(uint32_t, x1);
+  h = __builtin_amdgcn_perm(b1, b0, 0x07060302);
+  const float a0 = x0 - __builtin_bit_cast(float, b0 & 0xffff0000u);
+  const float a1 = x1 - __builtin_bit_cast(float, b1 & 0xffff0000u);
+  m = bf_pack(a0, a1);
+  l = bf_pack(a0 - bf_lo(m), a1 - bf_hi(m));
 }
 
 template <class T>
@@ -72,12 +91,12 @@ __device__ __forceinline__ float slope(float z, int act) {
 }
 
 // An operand: `rows` of its free axis; (row, k) at p[row ld + k], across at
-// p[k ld + row].  vec: two rows' eight k may be read by its wide loads.
+// p[k ld + row].
 template <class T>
 struct Operand {
   const T* p;
   int64_t ld;
-  int rows, vec;
+  int rows;
 };
 
 template <class T>
@@ -98,13 +117,14 @@ struct Product {
   int64_t lda, ldb, planeA, planeB;
 };
 
-// The tiled products of vc_linear_tile.hip: shape 0 is 256 x 256 (fp32: 256 x
-// 128), 1 is 128 x 128, 2 is 64 x 64.  Rows (across: k) lie lda, ldb values apart.
-// The caller has seen to it that every operand's base and ld are multiples of 16
-// bytes, that K is a multiple of eight (an operand whose k is contiguous) or its
-// rows are (one that is read across), and that 256 rows span less than 2^31 bytes.
+// The tiled products of vc_linear_tile.hip, shape 0 the largest (bf16 256 x 256,
+// 128 x 128, 64 x 64; fp32 128 x 128, 64 x 64).  Rows (across: k) lie lda, ldb
+// values apart.  The caller has seen to it that every operand's base and ld are
+// multiples of 16 bytes, that K is a multiple of eight (an operand whose k is
+// contiguous) or its lines are padded to one (read across), and that 256 of them
+// span less than 2^31 bytes.
 struct TileShape {
-  int bi, bj, bk, threads, lds;
+  int bi, bj, bk;
 };
 TileShape tile_shape(int type, int shape);
 template <class T>

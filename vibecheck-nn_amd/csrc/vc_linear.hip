@@ -11,6 +11,8 @@
 // largest starts from zero each step of 32 and is added in fp32.  Where the sum
 // is not finite the largest products' sum stands alone: with an infinity or NaN
 // among the values it is what the fp32 product gives, and the small ones are not.
+#include <type_traits>
+
 #include "vc_linear.h"
 
 namespace {
@@ -26,81 +28,60 @@ struct Raw {
   uint32_t d[sizeof(T) == 4 ? 16 : 8];
 };
 
+// Values k .. k + 7 of a row of K; past the end zero.
+template <class T>
+__device__ __forceinline__ void load_k8(const T* p, int k, int K, uint32_t* d) {
+  constexpr bool F = sizeof(T) == 4;
+  if (k + 8 <= K) {
+    const u4 a = load16(p + k);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d[j] = a[j];
+    if (F) {
+      const u4 b = load16(p + k + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[(4 + j) % (F ? 8 : 4)] = b[j];
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < (F ? 8 : 4); ++j) d[j] = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (k + j >= K) continue;
+    if constexpr (F) d[j] = __builtin_bit_cast(uint32_t, p[k + j]);
+    else d[j / 2] |= (uint32_t)p[k + j] << 16 * (j & 1);
+  }
+}
+
 template <class T, bool ACROSS>
 __device__ __forceinline__ void load_unit(const Operand<T>& o, int row, int k, int K, Raw<T>& v) {
   constexpr bool F = sizeof(T) == 4;
   const int r0 = min(row, o.rows - 1), r1 = min(row + 1, o.rows - 1);
   if (!ACROSS) {
-    const T* const p0 = o.p + (int64_t)r0 * o.ld + k;
-    const T* const p1 = o.p + (int64_t)r1 * o.ld + k;
-    if (o.vec) {  // K a multiple of eight
-      u4 a[F ? 4 : 2];
-      const u4 zero = u4{0, 0, 0, 0};
-      const bool in = k < K;
-      const u4* const q0 = reinterpret_cast<const u4*>(in ? p0 : p0 - k);
-      const u4* const q1 = reinterpret_cast<const u4*>(in ? p1 : p1 - k);
-      a[0] = q0[0];
-      if (F) a[1] = q0[1];
-      a[F ? 2 : 1] = q1[0];
-      if (F) a[F ? 3 : 1] = q1[1];
-#pragma unroll
-      for (int i = 0; i < (F ? 4 : 2); ++i) {
-        a[i] = in ? a[i] : zero;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v.d[4 * i + j] = a[i][j];
-      }
-      return;
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const T* const p = r ? p1 : p0;
-      uint32_t w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        w[j] = 0;
-        if (k + j < K) {
-          if (F) w[j] = __builtin_bit_cast(uint32_t, (float)get(p + j));
-          else w[j] = (uint32_t)p[j];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (F) v.d[8 * r + j] = w[j];
-        else if (j & 1) v.d[4 * r + j / 2] = w[j - 1] | w[j] << 16;
-      }
-    }
+    load_k8(o.p + (int64_t)r0 * o.ld, k, K, v.d);
+    load_k8(o.p + (int64_t)r1 * o.ld, k, K, v.d + (F ? 8 : 4));
     return;
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const bool in = k + j < K;
     const T* const p = o.p + (int64_t)(in ? k + j : 0) * o.ld;
-    if (o.vec) {  // rows and ld even
-      if (F) {
-        const u2 w = *reinterpret_cast<const u2*>(p + min(row, o.rows - 2));
+    if (row + 1 < o.rows) {
+      if constexpr (F) {
+        const u2 w = *reinterpret_cast<const u2at4*>(p + row);
         v.d[2 * j] = in ? w.x : 0;
-        v.d[(2 * j + 1) % (F ? 16 : 8)] = in ? w.y : 0;
+        v.d[2 * j + 1] = in ? w.y : 0;
       } else {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(p + min(row, o.rows - 2));
+        const uint32_t w = *reinterpret_cast<const u1at2*>(p + row);
         v.d[j] = in ? w : 0;
       }
-    } else if (F) {
-      v.d[(2 * j) % (F ? 16 : 8)] = in ? __builtin_bit_cast(uint32_t, (float)get(p + r0)) : 0;
-      v.d[(2 * j + 1) % (F ? 16 : 8)] = in ? __builtin_bit_cast(uint32_t, (float)get(p + r1)) : 0;
+    } else if constexpr (F) {
+      v.d[2 * j] = in ? __builtin_bit_cast(uint32_t, p[r0]) : 0;
+      v.d[2 * j + 1] = v.d[2 * j];
     } else {
-      v.d[j] = in ? (uint32_t)p[r0] | (uint32_t)p[r1] << 16 : 0;
+      v.d[j] = in ? (uint32_t)p[r0] * 0x10001u : 0;
     }
   }
-}
-
-// Two values' parts, the first cut: h + m + l is the value.
-__device__ __forceinline__ void cut2(float x0, float x1, uint32_t& h, uint32_t& m, uint32_t& l) {
-  const uint32_t b0 = __builtin_bit_cast(uint32_t, x0), b1 = __builtin_bit_cast(uint32_t, x1);
-  h = __builtin_amdgcn_perm(b1, b0, 0x07060302);
-  const float a0 = x0 - __builtin_bit_cast(float, b0 & 0xffff0000u);
-  const float a1 = x1 - __builtin_bit_cast(float, b1 & 0xffff0000u);
-  m = bf_pack(a0, a1);
-  l = bf_pack(a0 - bf_lo(m), a1 - bf_hi(m));
 }
 
 // The 16-byte operands of row r (0, 1) of a unit, one per part.
@@ -266,6 +247,127 @@ __global__ __launch_bounds__(LNT, 2) void k_product(Product<T> a) {
   }
 }
 
+// Few rows, or few steps: 16 MB rows x 16 NB columns by eight waves that share the
+// k, each reading its fragments straight from memory (64 of k at a time, UN of
+// these requested together) and, in fp32, taking its values apart itself: no LDS,
+// no barrier until the waves' sums are joined, in their order.  One token through
+// 4096 x 4096 bf16 is 256 workgroups with 64 KB on its way to each CU.
+constexpr int kDirectWaves = 8;
+
+template <class T>
+__device__ __forceinline__ void parts_of(const uint32_t* d, u4* o) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t h, m, l;
+      cut2(__builtin_bit_cast(float, d[2 * j]), __builtin_bit_cast(float, d[2 * j + 1]), h, m, l);
+      o[0][j] = h, o[1][j] = m, o[2][j] = l;
+    } else {
+      o[0][j] = d[j];
+    }
+  }
+}
+
+template <class T, int NB, int MB, int UN>
+__global__ __launch_bounds__(64 * kDirectWaves, 2) void k_direct(Product<T> a) {
+  constexpr bool F = sizeof(T) == 4;
+  constexpr int NP = F ? 3 : 1, D = F ? 8 : 4, NW = kDirectWaves;
+  __shared__ __align__(16) v4f part[NW][NB * MB][64];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, r = lane & 15;
+  const int64_t w = vcg::xcd_tile(blockIdx.x, a.tiles);
+  const int ti = (int)a.f_nj.div((uint32_t)w), tj = (int)(w - (int64_t)ti * a.f_nj.d);
+  const int i0 = ti * 16 * MB, j0 = tj * 16 * NB;
+  const T *pa[MB], *pb[NB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i) pa[i] = a.A.p + (int64_t)min(i0 + 16 * i + r, a.I - 1) * a.A.ld;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) pb[j] = a.B.p + (int64_t)min(j0 + 16 * j + r, a.J - 1) * a.B.ld;
+  v4f acc[MB][NB], small[F ? MB : 1][F ? NB : 1];
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+      if (F) small[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+  // slices: workgroups, then waves, take every 64-deep piece in turn
+  const int each = NW * gridDim.y;
+  const auto pieces = [&](int c, auto whole) {
+    uint32_t da[UN][2][MB][D], db[UN][2][NB][D];
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = (c + u * each) * 64 + 32 * h + 8 * g, K = whole ? 0x7fffffff : a.K;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) load_k8(pb[j], k, K, db[u][h][j]);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) load_k8(pa[i], k, K, da[u][h][i]);
+      }
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u4 fb[NB][NP];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) parts_of<T>(db[u][h][j], fb[j]);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+          u4 fa[NP];
+          parts_of<T>(da[u][h][i], fa);
+#pragma unroll
+          for (int j = 0; j < NB; ++j) {
+            if constexpr (F) {
+#pragma unroll
+              for (int p = 0; p < 5; ++p)
+                small[i][j] = mfma_bf16(fb[j][kPartA[p]], fa[kPartB[p]], small[i][j]);
+              acc[i][j] += mfma_bf16(fb[j][0], fa[0], v4f{0.f, 0.f, 0.f, 0.f});
+            } else {
+              acc[i][j] = mfma_bf16(fb[j][0], fa[0], acc[i][j]);
+            }
+          }
+        }
+      }
+  };
+  for (int c = blockIdx.y * NW + wv; c * 64 < a.K; c += UN * each) {
+    if ((c + (UN - 1) * each) * 64 + 64 <= a.K) pieces(c, std::true_type{});
+    else pieces(c, std::false_type{});
+  }
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      v4f s = acc[i][j];
+      if (F) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float t = s[q] + small[i][j][q];
+          s[q] = finite(t) ? t : s[q];
+        }
+      }
+      part[wv][i * NB + j][lane] = s;
+    }
+  __syncthreads();
+  for (int b = wv; b < NB * MB; b += NW) {
+    v4f s = part[0][b][lane];
+#pragma unroll
+    for (int k = 1; k < NW; ++k) s += part[k][b][lane];
+    const int64_t row = i0 + 16 * (b / NB) + r;
+    const int col = j0 + 16 * (b % NB) + 4 * g;
+    if (row >= a.I || col >= a.J) continue;
+    const float v[4] = {s[0], s[1], s[2], s[3]};
+    if (a.slices == 1) {
+      finish(a, row, col, v);
+    } else {
+      float* const o = a.part + ((int64_t)blockIdx.y * a.I + row) * a.J + col;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (col + q < a.J) o[q] = v[q];
+    }
+  }
+}
+
 // The slices' sums joined in their order.
 template <class T>
 __global__ __launch_bounds__(LNT) void k_join(Product<T> a) {
@@ -287,21 +389,13 @@ __global__ __launch_bounds__(LNT) void k_join(Product<T> a) {
 
 // Eight values j .. j + 7 of a row of n, as floats; past the end zero.
 template <class T>
-__device__ __forceinline__ void load8(const T* p, int j, int n, bool wide, float* o) {
-  if (wide && j + 8 <= n) {
-    if constexpr (sizeof(T) == 4) {
-      const v4f a = *reinterpret_cast<const v4f*>(p + j), b = *reinterpret_cast<const v4f*>(p + j + 4);
+__device__ __forceinline__ void load8(const T* p, int j, int n, float* o) {
+  uint32_t d[sizeof(T) == 4 ? 8 : 4];
+  load_k8(p, j, n, d);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) o[q] = a[q], o[4 + q] = b[q];
-    } else {
-      const u4 a = *reinterpret_cast<const u4*>(p + j);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) o[2 * q] = bf_lo(a[q]), o[2 * q + 1] = bf_hi(a[q]);
-    }
-    return;
-  }
-#pragma unroll
-  for (int q = 0; q < 8; ++q) o[q] = j + q < n ? get(p + j + q) : 0.f;
+  for (int q = 0; q < 8; ++q)
+    o[q] = sizeof(T) == 4 ? __builtin_bit_cast(float, d[q % (sizeof(T) * 2)])
+                          : q & 1 ? bf_hi(d[q / 2]) : bf_lo(d[q / 2]);
 }
 
 // Eight values as 16 bytes of each part, part p at p planes.
@@ -331,7 +425,7 @@ template <class T>
 struct Pack {
   const T* p;
   int64_t ld, rows;
-  int n, np, wide;  // values of a line, and with its padding
+  int n, np;  // values of a line, and with its padding
   uint16_t* to;
 };
 
@@ -345,7 +439,7 @@ __global__ __launch_bounds__(LNT) void k_pack(Pack<T> a, Pack<T> b, int64_t spli
   if (row >= m.rows) return;
   const int j = (int)(t - row * c) * 8;
   float v[8];
-  load8(m.p + row * m.ld, j, m.n, m.wide, v);
+  load8(m.p + row * m.ld, j, m.n, v);
   store_parts<T>(v, m.to + row * m.np + j, m.rows * m.np);
 }
 
@@ -359,7 +453,7 @@ struct Slope {
   uint16_t* parts; // or null
   float* sums;     // (blocks of rows, N), or null
   int64_t M;
-  int N, np, act, rows, wide;
+  int N, np, act, rows;
 };
 
 constexpr int kSlopeCols = 256;  // of a workgroup: eight a thread, eight rows at a time
@@ -378,8 +472,8 @@ __global__ __launch_bounds__(LNT) void k_slope(Slope<T> a) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int64_t r = m + 8 * q < m1 ? m + 8 * q : m;
-        load8(a.dy + r * a.ldy, j, a.N, a.wide, d[q]);
-        if (a.act != kNone) load8(a.z + r * a.ldz, j, a.N, a.wide, z[q]);
+        load8(a.dy + r * a.ldy, j, a.N, d[q]);
+        if (a.act != kNone) load8(a.z + r * a.ldz, j, a.N, z[q]);
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -430,74 +524,92 @@ int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
 constexpr int64_t kCus = 256;
 
-// How a product is cut: the kernel (shape -1: k_product, else k_tile's) and the
-// slices of k, by the time that they are expected to take.
+// How a product is cut: the kernel, its shape, and the slices of k, by the time
+// that they are expected to take (us).
+enum Kernel { kProduct, kDirect, kTile };
 struct Cut {
+  Kernel kernel;
   int shape, slices, steps;
   int64_t tiles, nj;
+  float us;
 };
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-Cut cut_general(int type, int64_t I, int64_t J, int64_t K) {
-  const int64_t all = div_up(K, type == VC_FP32 ? 32 : 64);
-  Cut c;
-  c.shape = -1;
-  c.nj = div_up(J, 64);
-  c.tiles = div_up(I, 64) * c.nj;
-  int64_t s = 1;
-  if (c.tiles < kCus && all >= 16) {
-    s = kCus / c.tiles;
-    if (s > all / 8) s = all / 8;
-    if (s > 64) s = 64;
+// A grid of `tiles` workgroups of `all` steps, cut into more slices while that
+// helps: `alone` us a step for as many workgroups as share a CU, `shared` us for
+// each of them.
+void slice(Cut& best, Kernel kernel, int shape, int64_t I, int64_t J, int bi, int bj, int64_t all,
+           float alone, float shared, int share) {
+  const int64_t nj = div_up(J, bj), tiles = div_up(I, bi) * nj;
+  for (int64_t want = 1; want <= 32 && (want == 1 || 4 * want <= all); want *= 2) {
+    const int64_t steps = div_up(all, want) > 0 ? div_up(all, want) : 1;
+    const int64_t slices = div_up(all, steps) > 0 ? div_up(all, steps) : 1;
+    const int64_t load = div_up(tiles * slices, kCus);
+    const float a = alone * div_up(load, share), s = shared * load;
+    // the slices' sums are written, read again and joined by a launch
+    const float us = 4.f + steps * (a > s ? a : s) +
+                     (slices > 1 ? 4.f + 8.f * slices * I * J / 4e6f : 0.f);
+    if (us < best.us) best = {kernel, shape, (int)slices, (int)steps, tiles, nj, us};
   }
-  c.steps = (int)div_up(all, s);
-  if (c.steps < 1) c.steps = 1;
-  c.slices = (int)div_up(all, c.steps);
-  if (c.slices < 1) c.slices = 1;
+}
+
+// The kernel of 64 x 64 tiles by registers: steps of 32 (bf16: 64).
+Cut cut_product(int type, int64_t I, int64_t J, int64_t K) {
+  Cut c = {};
+  c.us = 1e30f;
+  const bool f = type == VC_FP32;
+  slice(c, kProduct, 0, I, J, 64, 64, div_up(K, f ? 32 : 64), f ? 1.0f : 0.9f, f ? 0.9f : 0.5f, 2);
   return c;
 }
 
-// Of the tiled kernels: a step of one tile alone on a CU, and of each of several
-// that share one (us, measured on 264 x 328 and 8192 x 16384 outputs).
-constexpr float kStepAlone[2][3] = {{2.0f, 1.5f, 0.50f}, {2.1f, 1.0f, 0.45f}};
-constexpr float kStepShared[2][3] = {{2.7f, 1.54f, 0.46f}, {2.2f, 0.55f, 0.21f}};
-constexpr int kShare[2][3] = {{1, 1, 3}, {1, 2, 4}};
+// The tiled kernels: a step of one tile alone on a CU, and of each of several that
+// share one (measured on 264 x 328 and 512 x 512 outputs, and on 8192 x 16384 and
+// 4096 x 4096).
+constexpr float kStepAlone[2][3] = {{1.15f, 0.50f, 0.f}, {1.45f, 1.0f, 0.45f}};
+constexpr float kStepShared[2][3] = {{1.39f, 0.46f, 0.f}, {1.95f, 0.55f, 0.21f}};
+constexpr int kShare[2][3] = {{1, 3, 1}, {1, 2, 4}};
 
 Cut cut_tiles(int type, int64_t I, int64_t J, int64_t K) {
-  Cut best = {};
-  float least = 1e30f;
-  for (int shape = 0; shape < 3; ++shape) {
+  Cut c = {};
+  c.us = 1e30f;
+  const int b = type == VC_FP32 ? 0 : 1;
+  for (int shape = 0; shape < (b ? 3 : 2); ++shape) {
     const TileShape t = tile_shape(type, shape);
-    const int b = type == VC_FP32 ? 0 : 1;
-    const int64_t all = div_up(K, t.bk), nj = div_up(J, t.bj), tiles = div_up(I, t.bi) * nj;
-    for (int64_t want = 1; want <= 16 && want <= all; want *= 2) {
-      const int64_t steps = div_up(all, want), slices = div_up(all, steps);
-      const int64_t load = div_up(tiles * slices, kCus);
-      const float alone = kStepAlone[b][shape] * div_up(load, kShare[b][shape]);
-      const float shared = kStepShared[b][shape] * load;
-      float us = steps * (alone > shared ? alone : shared);
-      // the slices' sums written, read again and joined by a launch
-      if (slices > 1) us += 4.f + 8.f * slices * I * J / 4e6f;
-      if (us < least) {
-        least = us;
-        best = {shape, (int)slices, (int)steps, tiles, nj};
-      }
-    }
+    slice(c, kTile, shape, I, J, t.bi, t.bj, div_up(K, t.bk), kStepAlone[b][shape],
+          kStepShared[b][shape], kShare[b][shape]);
   }
-  return best;
+  return c;
 }
 
-// Which products are tiled: those whose time the tiles cut by more than their
-// parts' pass and its launch cost.
-bool tiled(int type, int64_t M, int64_t K, int64_t N) {
-  return K > 0 && (double)M * K * N >= (type == VC_FP32 ? 3e8 : 1.5e8) && K < (1 << 21) &&
-         N < (1 << 21);
+// The direct kernel: 16 rows by 16 columns, 32 by 16, 64 by 16, 64 by 32.  A
+// workgroup's operands come at about 45 GB/s a CU, all of them together at no
+// more than the memory's rate.
+constexpr int kDirectRows[4] = {16, 32, 64, 64}, kDirectCols[4] = {16, 16, 16, 32};
+
+Cut cut_direct(int type, int64_t I, int64_t J, int64_t K) {
+  Cut c = {};
+  c.us = 1e30f;
+  const float e = type == VC_FP32 ? 4.f : 2.f;
+  for (int shape = 0; shape < 4; ++shape) {
+    const int bi = kDirectRows[shape], bj = kDirectCols[shape];
+    const int64_t nj = div_up(J, bj), tiles = div_up(I, bi) * nj;
+    int64_t s = 1;
+    while (tiles * s < kCus && 1024 * s < K && s < 16) s *= 2;
+    const float own = e * ((I < bi ? I : bi) + bj) * (float)K / s;
+    const float l2 = div_up(tiles * s, kCus) * own / 45e3f;
+    const float hbm = e * (I + J) * (float)K / 4.5e6f;
+    const float us = 5.f + (l2 > hbm ? l2 : hbm) + (s > 1 ? 4.f + 8.f * s * I * J / 4e6f : 0.f);
+    if (us < c.us) c = {kDirect, shape, (int)s, 0, tiles, nj, us};
+  }
+  return c;
 }
 
-Cut cut(int type, int64_t I, int64_t J, int64_t K, bool tiles) {
-  return tiles ? cut_tiles(type, I, J, K) : cut_general(type, I, J, K);
-}
+// Whether tiles can be made of matrices with lines of this length at all.
+bool tile_lines(int64_t n) { return n > 0 && n < (1 << 21); }
+
+// The pass that makes `n` values into parts.
+float pack_us(int type, int64_t n) { return 4.f + n * (type == VC_FP32 ? 10.f : 4.f) / 4e6f; }
 
 int64_t part_bytes(const Cut& c, int64_t I, int64_t J) {
   return c.slices > 1 ? up256(4 * c.slices * I * J) : 0;
@@ -512,14 +624,6 @@ int64_t parts_bytes(int type, int64_t rows, int64_t n) {
   return up256((type == VC_FP32 ? 6 : 2) * rows * up8(n));
 }
 
-template <class T>
-bool wide_rows(const T* p, int64_t ld, int64_t K) {
-  return aligned16(p) && ld % (16 / (int)sizeof(T)) == 0 && K % 8 == 0;
-}
-template <class T>
-bool wide_across(const T* p, int64_t ld, int64_t rows) {
-  return ((uintptr_t)p & (2 * sizeof(T) - 1)) == 0 && ld % 2 == 0 && rows % 2 == 0;
-}
 template <class T>
 bool quads(const void* p, int64_t ld) {
   return !p || (((uintptr_t)p & (4 * sizeof(T) - 1)) == 0 && ld % 4 == 0);
@@ -536,12 +640,18 @@ int run_product(Product<T> a, const Cut& c, void* work, int64_t work_bytes, hipS
   a.part = (float*)work;
   a.tiles = c.tiles;
   a.f_nj = vcg::FastDiv::make((uint32_t)c.nj);
-  if (c.shape >= 0) {
+  const dim3 grid((unsigned)c.tiles, (unsigned)c.slices);
+  if (c.kernel == kTile) {
     run_tiles<T>(a, c.shape, XA, XB, st);
+  } else if constexpr (XB) {
+    k_product<T, XA, XB, 64, 64><<<grid, LNT, 0, st>>>(a);
   } else {
-    a.A.vec = XA ? wide_across(a.A.p, a.A.ld, a.A.rows) : wide_rows(a.A.p, a.A.ld, a.K);
-    a.B.vec = XB ? wide_across(a.B.p, a.B.ld, a.B.rows) : wide_rows(a.B.p, a.B.ld, a.K);
-    k_product<T, XA, XB, 64, 64><<<dim3((unsigned)c.tiles, (unsigned)c.slices), LNT, 0, st>>>(a);
+    constexpr bool F = sizeof(T) == 4;
+    const int threads = 64 * kDirectWaves;
+    if (c.shape == 0) k_direct<T, 1, 1, 4><<<grid, threads, 0, st>>>(a);
+    else if (c.shape == 1) k_direct<T, 1, 2, F ? 2 : 4><<<grid, threads, 0, st>>>(a);
+    else if (c.shape == 2) k_direct<T, 1, 4, F ? 1 : 2><<<grid, threads, 0, st>>>(a);
+    else k_direct<T, 2, 4, F ? 1 : 2><<<grid, threads, 0, st>>>(a);
   }
   if (c.slices > 1) {
     const int64_t n = (int64_t)a.I * ((a.J + 3) / 4);
@@ -556,28 +666,30 @@ template <class T>
 void run_pack(Pack<T> a, Pack<T> b, hipStream_t st) {
   const int64_t na = a.to ? div_up(a.rows * (a.np / 8), LNT) : 0;
   const int64_t nb = b.to ? div_up(b.rows * (b.np / 8), LNT) : 0;
-  a.wide = aligned16(a.p) && a.ld % (16 / (int)sizeof(T)) == 0;
-  b.wide = aligned16(b.p) && b.ld % (16 / (int)sizeof(T)) == 0;
   if (na + nb > 0) k_pack<T><<<(unsigned)(na + nb), LNT, 0, st>>>(a, b, na);
 }
 
 bool sizes_ok(int64_t M, int K, int N) {
-  return M >= 0 && M <= 0x7fffff00 && K >= 0 && K <= 0x7fffff00 && N >= 0 && N <= 0x7fffff00;
+  return M >= 0 && M <= 0x7fffff00 && K >= 0 && K <= (1 << 30) && N >= 0 && N <= (1 << 30);
 }
 
 struct ForwardPlan {
-  bool tiles;
   Cut c;
   int64_t x, W, part, bytes;  // offsets in the workspace, and its size
 };
 
 ForwardPlan plan_forward(int type, int64_t M, int K, int N) {
   ForwardPlan p;
-  p.tiles = tiled(type, M, K, N);
-  p.c = cut(type, M, N, K, p.tiles);
+  p.c = cut_direct(type, M, N, K);
+  if (tile_lines(K)) {
+    const Cut t = cut_tiles(type, M, N, K);
+    const float pack = type == VC_FP32 || K % 8 ? pack_us(type, (M + N) * K) : 0.f;
+    if (t.us + pack < p.c.us) p.c = t;
+  }
+  const bool tiles = p.c.kernel == kTile;
   p.x = 0;
-  p.W = p.tiles ? parts_bytes(type, M, K) : 0;
-  p.part = p.W + (p.tiles ? parts_bytes(type, N, K) : 0);
+  p.W = tiles ? parts_bytes(type, M, K) : 0;
+  p.part = p.W + (tiles ? parts_bytes(type, N, K) : 0);
   p.bytes = p.part + part_bytes(p.c, M, N);
   return p;
 }
@@ -591,8 +703,8 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
   if (p.bytes > work_bytes || (p.bytes && !work)) return VC_ERR_OOM;
   char* const base = (char*)work;
   Product<T> a = {};
-  a.A = {(const T*)x, ldx, (int)M, 0};
-  a.B = {(const T*)W, K, N, 0};
+  a.A = {(const T*)x, ldx, (int)M};
+  a.B = {(const T*)W, K, N};
   a.I = (int)M;
   a.J = N;
   a.K = K;
@@ -602,11 +714,11 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
   a.out = (T*)y;
   a.z = (T*)z;
   a.act = act;
-  if (p.tiles) {
+  if (p.c.kernel == kTile) {
     const int kp = (int)up8(K);
     Pack<T> px = {}, pw = {};
-    if (!as_it_is((const T*)x, ldx, K)) px = {(const T*)x, ldx, M, K, kp, 0, (uint16_t*)(base + p.x)};
-    if (!as_it_is((const T*)W, K, K)) pw = {(const T*)W, K, N, K, kp, 0, (uint16_t*)(base + p.W)};
+    if (!as_it_is((const T*)x, ldx, K)) px = {(const T*)x, ldx, M, K, kp, (uint16_t*)(base + p.x)};
+    if (!as_it_is((const T*)W, K, K)) pw = {(const T*)W, K, N, K, kp, (uint16_t*)(base + p.W)};
     run_pack(px, pw, st);
     a.pa = px.to ? px.to : (const uint16_t*)x;
     a.lda = px.to ? kp : ldx;
@@ -635,9 +747,16 @@ struct BackwardPlan {
 BackwardPlan plan_backward(int type, int64_t M, int K, int N, int act, int need) {
   BackwardPlan p;
   const int64_t e = type == VC_FP32 ? 4 : 2;
-  p.tiles = tiled(type, M, K, N);
-  p.cx = cut(type, M, K, N, p.tiles);
-  p.cw = cut(type, N, K, M, p.tiles);
+  p.cx = cut_product(type, M, K, N);
+  p.cw = cut_product(type, N, K, M);
+  p.tiles = false;
+  if (tile_lines(K) && tile_lines(N)) {
+    const Cut x = cut_tiles(type, M, K, N), w = cut_tiles(type, N, K, M);
+    const float pack = type == VC_FP32 || K % 8 ? pack_us(type, (M + N) * K) : 0.f;
+    p.tiles = (need & 1 ? x.us : 0.f) + (need & 2 ? w.us : 0.f) + pack <
+              (need & 1 ? p.cx.us : 0.f) + (need & 2 ? p.cw.us : 0.f);
+    if (p.tiles) p.cx = x, p.cw = w;
+  }
   p.rows = slope_rows(M);
   p.blocks = (int)div_up(M, p.rows);
   p.dz = 0;
@@ -682,8 +801,6 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
     s.np = np;
     s.act = act;
     s.rows = p.rows;
-    const int per = 16 / (int)sizeof(T);
-    s.wide = aligned16(dy) && ldy % per == 0 && (act == kNone || (aligned16(z) && ldz % per == 0));
     k_slope<T><<<dim3((unsigned)div_up(N, kSlopeCols), (unsigned)p.blocks), LNT, 0, st>>>(s);
   }
   if (db && N > 0)
@@ -693,8 +810,8 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
   Product<T> a = {};
   if (p.tiles && (need & 3)) {
     Pack<T> pw = {}, px = {};
-    if (dx && !as_it_is((const T*)W, K, K)) pw = {(const T*)W, K, N, K, kp, 0, (uint16_t*)(base + p.W)};
-    if (dW && !as_it_is((const T*)x, ldx, K)) px = {(const T*)x, ldx, M, K, kp, 0, (uint16_t*)(base + p.x)};
+    if (dx && !as_it_is((const T*)W, K, K)) pw = {(const T*)W, K, N, K, kp, (uint16_t*)(base + p.W)};
+    if (dW && !as_it_is((const T*)x, ldx, K)) px = {(const T*)x, ldx, M, K, kp, (uint16_t*)(base + p.x)};
     run_pack(pw, px, st);
     a.pa = made ? (const uint16_t*)(base + p.dz) : (const uint16_t*)dy;
     a.lda = made ? np : ldy;
@@ -727,8 +844,8 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
   const T* const dz = made ? (const T*)(base + p.dz) : (const T*)dy;
   const int64_t ldd = made ? N : ldy;
   if (dx) {
-    a.A = {dz, ldd, (int)M, 0};
-    a.B = {(const T*)W, K, K, 0};
+    a.A = {dz, ldd, (int)M};
+    a.B = {(const T*)W, K, K};
     a.I = (int)M;
     a.J = K;
     a.K = N;
@@ -737,8 +854,8 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
     if (rc != VC_OK) return rc;
   }
   if (dW) {
-    a.A = {dz, ldd, N, 0};
-    a.B = {(const T*)x, ldx, K, 0};
+    a.A = {dz, ldd, N};
+    a.B = {(const T*)x, ldx, K};
     a.I = N;
     a.J = K;
     a.K = (int)M;

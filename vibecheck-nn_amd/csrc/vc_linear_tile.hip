@@ -1,17 +1,21 @@
-// The fc layer's large products: tiles of up to 256 x 256, both operands as bf16
+// The fc layer's large products: tiles of 64 x 64 to 256 x 256 (fp32 128 x 128), both operands as bf16
 // (an fp32 value as three parts, vc_linear.hip) brought into LDS by loads that
 // pass no register.
 //
-// A step of BK goes into one of two LDS buffers while the other is multiplied;
-// one barrier a step.  A load instruction writes 1 KB of LDS in lane order, so
-// the order that spreads a fragment's reads over the banks is made by which
-// address each lane reads from:
+// A step of BK goes into one of two or three LDS buffers while another is
+// multiplied.  A load instruction writes 1 KB of LDS in lane order, so the order
+// that spreads a fragment's reads over the banks is made by which address each
+// lane reads from:
 //   k contiguous: [row][BK], 16-byte chunk c of row r at c ^ (r mod 8) (BK 64) or
 //     c ^ (r / 2 mod 4) (BK 32); a lane's fragment is one 16-byte read;
 //   read across: [k][row], 32-byte chunk c of line k at c ^ f(k), f = k mod 4 + 4
 //     (k / 8 mod 2); two 8-byte transposing reads give a lane its eight k.
-// 256 x 256 by eight waves of 128 x 64: a step of 64 is 1,024 cycles of a wave's
-// matrix instructions against 192 KB of fragment reads a workgroup.
+//
+// Shapes of eight waves take turns: while four multiply, the other four, one on
+// each SIMD, read their next fragments; a barrier ends each turn.  256 x 256 by
+// waves of 128 x 64: a turn of 32 products deep is 512 cycles of matrix
+// instructions on each SIMD beside 48 KB of fragment reads and 16 KB of loads into
+// LDS, at 128 bytes a cycle 512 as well.
 #include "vc_linear.h"
 
 namespace {
@@ -113,7 +117,24 @@ struct Side {
   }
 };
 
-template <class T, int NP, bool XA, bool XB, int BI, int BJ, int WI, int WJ, int BK>
+// Up to n vector memory operations of this wave may still run (and any LDS ones,
+// with lds none).
+template <int N, bool LDS>
+__device__ __forceinline__ void wait_for() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (LDS ? 0 : 15) << 8 | (N >> 4) << 14);
+}
+// A workgroup barrier that waits for nothing else, and that nothing is moved over.
+__device__ __forceinline__ void turn() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
+// NBUF: LDS buffers.  TURNS: the waves take turns, one for each 32 of k.
+template <class T, int NP, bool XA, bool XB, int BI, int BJ, int WI, int WJ, int BK, int NBUF,
+          bool TURNS>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void k_tile(Product<T> a) {
   constexpr int NW = WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16;
   typedef Side<XA, BI, BK, NW> SA;
@@ -146,7 +167,14 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void k_tile(Product<T> a) {
       if (NP == 3) small[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
     }
 
-  const auto load = [&](int s, char* to) {
+  // A step of an operand whose k is contiguous is 64 or 128 bytes of each of its
+  // rows, and rows a power of two apart lie in one channel of the L2: with two such
+  // operands the tiles of an XCD start at eight places 256 bytes apart and wrap
+  // (8192 x 16384 x 4096 1137 -> 1007 us; with one, 262 -> 283, the tiles then no
+  // longer share what they read).
+  const int first = XA || XB || full == 0 ? 0 : (int)(blockIdx.x >> 3) % 8 * (128 / BK) % full;
+  const auto load = [&](int step, char* to) {
+    const int s = step + first < full ? step + first : step + first - full;
     const uint16_t* const fa = sa.base + (XA ? (int64_t)s * BK * a.lda : (int64_t)s * BK);
     const uint16_t* const fb = sb.base + (XB ? (int64_t)s * BK * a.ldb : (int64_t)s * BK);
 #pragma unroll
@@ -155,53 +183,97 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void k_tile(Product<T> a) {
       sb.issue(fb + p * a.planeB, to + NP * SA::kBytes + p * SB::kBytes, wv);
     }
   };
-  const auto multiply = [&](const char* from) {
+  v8bf fb[MJ][NP], fa[MI][NP];
+  const auto read = [&](const char* from, int ks) {
 #pragma unroll
-    for (int ks = 0; ks < BK / 32; ++ks) {
-      v8bf fb[MJ][NP], fa[NP == 3 ? 1 : MI][NP];
+    for (int j = 0; j < MJ; ++j)
 #pragma unroll
-      for (int j = 0; j < MJ; ++j)
+      for (int p = 0; p < NP; ++p)
+        fb[j][p] = SB::frag(from + NP * SA::kBytes + p * SB::kBytes, (wj * MJ + j) * 16, ks, lane);
 #pragma unroll
-        for (int p = 0; p < NP; ++p)
-          fb[j][p] = SB::frag(from + NP * SA::kBytes + p * SB::kBytes, (wj * MJ + j) * 16, ks, lane);
-      if (NP == 1) {
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int i = 0; i < MI; ++i) fa[i][0] = SA::frag(from, (wi * MI + i) * 16, ks, lane);
-      }
+      for (int p = 0; p < NP; ++p)
+        fa[i][p] = SA::frag(from + p * SA::kBytes, (wi * MI + i) * 16, ks, lane);
+  };
+  const auto multiply = [&]() {
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        v8bf f[NP];
+    for (int i = 0; i < MI; ++i) {
+      if constexpr (NP == 1) {
 #pragma unroll
-        for (int p = 0; p < NP; ++p)
-          f[p] = NP == 1 ? fa[i][0] : SA::frag(from + p * SA::kBytes, (wi * MI + i) * 16, ks, lane);
-        if constexpr (NP == 1) {
+        for (int j = 0; j < MJ; ++j) acc[i][j] = mfma_bf16(fb[j][0], fa[i][0], acc[i][j]);
+      } else {
+        v4f z[MJ];  // the largest products, from zero
 #pragma unroll
-          for (int j = 0; j < MJ; ++j) acc[i][j] = mfma_bf16(fb[j][0], f[0], acc[i][j]);
-        } else {
+        for (int j = 0; j < MJ; ++j) z[j] = mfma_bf16(fb[j][0], fa[i][0], v4f{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-          for (int p = 0; p < 5; ++p)
-#pragma unroll
-            for (int j = 0; j < MJ; ++j)
-              small[i][j] = mfma_bf16(fb[j][kPartA[p]], f[kPartB[p]], small[i][j]);
+        for (int p = 0; p < 5; ++p)
 #pragma unroll
           for (int j = 0; j < MJ; ++j)
-            acc[i][j] += mfma_bf16(fb[j][0], f[0], v4f{0.f, 0.f, 0.f, 0.f});
-        }
+            small[i][j] = mfma_bf16(fb[j][kPartA[p]], fa[i][kPartB[p]], small[i][j]);
+#pragma unroll
+        for (int j = 0; j < MJ; ++j) acc[i][j] += z[j];
       }
     }
   };
+  constexpr int kLoads = NP * (SA::kOwn + SB::kOwn), AHEAD = NBUF - 1;
   if (full > 0) {
-    load(0, lds);
+    if constexpr (!TURNS) {
+      static_assert(NBUF == 2);
+      load(0, lds);
 #pragma unroll 1
-    for (int s = 0;; s += 2) {
-      __syncthreads();  // this step has arrived, the buffer of the one before is read
-      if (s + 1 < full) load(s + 1, lds + kStage);
-      multiply(lds);
-      if (s + 1 >= full) break;
-      __syncthreads();
-      if (s + 2 < full) load(s + 2, lds);
-      multiply(lds + kStage);
-      if (s + 2 >= full) break;
+      for (int s = 0; s < full; ++s) {
+        __syncthreads();  // this step has arrived, the buffer of the one before is read
+        if (s + 1 < full) load(s + 1, lds + ((s + 1) & 1) * kStage);
+#pragma unroll
+        for (int ks = 0; ks < BK / 32; ++ks) {
+          read(lds + (s & 1) * kStage, ks);
+          multiply();
+        }
+      }
+    } else {
+      // Waves wv and wv + 4 share a SIMD; the later ones run a turn behind.  A
+      // step's loads are issued in its wave's first reading turn, into the buffer
+      // whose last reader was waited for at the turn's barrier, and waited for at
+      // the barrier before the turn that reads them first.
+      static_assert(NW == 8);
+      constexpr int PH = BK / 32;
+      const bool late = wv >= 4;
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s)
+        if (s < full) load(s, lds + s * kStage);
+      if (full >= AHEAD) wait_for<(AHEAD - 1) * kLoads, false>();
+      else wait_for<0, false>();
+      turn();
+      if (late) turn();
+      int at = 0;  // this step's buffer
+#pragma unroll 1
+      for (int s = 0; s < full; ++s) {
+        const char* const from = lds + at * kStage;
+        const int before = at == 0 ? NBUF - 1 : at - 1;
+#pragma unroll
+        for (int ph = 0; ph < PH; ++ph) {
+          read(from, ph);
+          if (ph == 0 && s + AHEAD < full) load(s + AHEAD, lds + before * kStage);
+          if (ph == PH - 1 && late) {
+            if (s + AHEAD < full) wait_for<(AHEAD - 1) * kLoads, true>();
+            else wait_for<0, true>();
+          } else {
+            __builtin_amdgcn_s_waitcnt(63 & 15 | 7 << 4 | 0 << 8 | 3 << 14);  // fragments only
+          }
+          turn();
+          __builtin_amdgcn_s_setprio(1);
+          multiply();
+          __builtin_amdgcn_s_setprio(0);
+          if (ph == PH - 1 && !late) {
+            if (s + AHEAD < full) wait_for<(AHEAD - 1) * kLoads, false>();
+            else wait_for<0, false>();
+          }
+          turn();
+        }
+        at = at == NBUF - 1 ? 0 : at + 1;
+      }
+      if (!late) turn();
     }
   }
   if (left > full * BK) {
@@ -214,7 +286,11 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void k_tile(Product<T> a) {
       sb.tail(fb + p * a.planeB, lds + NP * SA::kBytes + p * SB::kBytes, wv, lane, left - full * BK);
     }
     __syncthreads();
-    multiply(lds);
+#pragma unroll
+    for (int ks = 0; ks < BK / 32; ++ks) {
+      read(lds, ks);
+      multiply();
+    }
   }
 
   const int g = lane >> 4, r = lane & 15;
@@ -253,16 +329,17 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void k_tile(Product<T> a) {
 
 template <class T, bool XA, bool XB, int SHAPE>
 struct Form {
-  static constexpr int NP = sizeof(T) == 4 ? 3 : 1;
-  static constexpr int BI = SHAPE == 0 ? 256 : SHAPE == 1 ? 128 : 64;
-  static constexpr int BJ = SHAPE == 0 ? (NP == 3 ? 128 : 256) : BI;
-  static constexpr int WI = SHAPE == 0 ? (NP == 3 ? 4 : 2) : 2;
-  static constexpr int WJ = SHAPE == 0 ? (NP == 3 ? 2 : 4) : 2;
-  static constexpr int BK = NP == 3 ? 32 : 64;
+  static constexpr bool F = sizeof(T) == 4;
+  static constexpr int NP = F ? 3 : 1;
+  static constexpr int BI = (SHAPE == 0 ? 256 : SHAPE == 1 ? 128 : 64) / (F && SHAPE < 2 ? 2 : 1);
+  static constexpr int BJ = BI, WI = 2, WJ = SHAPE == 0 ? 4 : 2;
+  static constexpr int BK = F ? 32 : 64;
+  static constexpr int NBUF = F && SHAPE == 0 ? 3 : 2;
+  static constexpr int TURNS = SHAPE == 0;
   static constexpr int kThreads = 64 * WI * WJ;
-  static constexpr int kLds = 2 * NP * (BI + BJ) * BK * 2;
+  static constexpr int kLds = NBUF * NP * (BI + BJ) * BK * 2;
   static void run(const Product<T>& a, hipStream_t st) {
-    const auto k = k_tile<T, NP, XA, XB, BI, BJ, WI, WJ, BK>;
+    const auto k = k_tile<T, NP, XA, XB, BI, BJ, WI, WJ, BK, NBUF, TURNS>;
     static bool set[16];
     int dev = 0;
     (void)hipGetDevice(&dev);
@@ -287,19 +364,16 @@ void run_shape(const Product<T>& a, bool xa, bool xb, hipStream_t st) {
 namespace vcl {
 
 TileShape tile_shape(int type, int shape) {
-  const bool f = type == VC_FP32;
-  switch (shape) {
-    case 0: return f ? TileShape{256, 128, 32, 512, 0} : TileShape{256, 256, 64, 512, 0};
-    case 1: return {128, 128, f ? 32 : 64, 256, 0};
-    default: return {64, 64, f ? 32 : 64, 256, 0};
-  }
+  if (type == VC_FP32) return shape == 0 ? TileShape{128, 128, 32} : TileShape{64, 64, 32};
+  return shape == 0 ? TileShape{256, 256, 64}
+                    : shape == 1 ? TileShape{128, 128, 64} : TileShape{64, 64, 64};
 }
 
 template <class T>
 void run_tiles(const Product<T>& a, int shape, bool xa, bool xb, hipStream_t st) {
   if (shape == 0) run_shape<T, 0>(a, xa, xb, st);
   else if (shape == 1) run_shape<T, 1>(a, xa, xb, st);
-  else run_shape<T, 2>(a, xa, xb, st);
+  else if constexpr (sizeof(T) == 2) run_shape<T, 2>(a, xa, xb, st);
 }
 template void run_tiles<float>(const Product<float>&, int, bool, bool, hipStream_t);
 template void run_tiles<uint16_t>(const Product<uint16_t>&, int, bool, bool, hipStream_t);
