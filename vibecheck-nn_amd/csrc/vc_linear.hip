@@ -376,12 +376,22 @@ __global__ __launch_bounds__(LNT) void k_join(Product<T> a) {
        t += (int64_t)gridDim.x * LNT) {
     const int64_t i = t / nq;
     const int j = (int)(t - i * nq) * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.slices; ++s) {
-      const float* const p = a.part + ((int64_t)s * a.I + i) * a.J + j;
+    float v[4] = {-0.f, -0.f, -0.f, -0.f};  // adds nothing, not even a sign
+    const int64_t step = (int64_t)a.I * a.J;
+    const float* p = a.part + (int64_t)i * a.J + j;
+    if (a.J % 4 == 0) {
+#pragma unroll 8
+      for (int s = 0; s < a.slices; ++s, p += step) {
+        const v4f w = *reinterpret_cast<const v4f*>(p);
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (j + q < a.J) v[q] = s ? v[q] + p[q] : p[q];
+        for (int q = 0; q < 4; ++q) v[q] += w[q];
+      }
+    } else {
+#pragma unroll 4
+      for (int s = 0; s < a.slices; ++s, p += step)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (j + q < a.J) v[q] += p[q];
     }
     finish(a, i, j, v);
   }
@@ -536,20 +546,26 @@ struct Cut {
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// The slices' sums written, read again and joined by a launch.
+float join_us(int64_t slices, int64_t I, int64_t J) {
+  return slices > 1 ? 4.f + 0.1f * slices + 8.f * slices * I * J / 4e6f : 0.f;
+}
+
 // A grid of `tiles` workgroups of `all` steps, cut into more slices while that
 // helps: `alone` us a step for as many workgroups as share a CU, `shared` us for
 // each of them.
-void slice(Cut& best, Kernel kernel, int shape, int64_t I, int64_t J, int bi, int bj, int64_t all,
-           float alone, float shared, int share) {
+void slice(Cut& best, Kernel kernel, int shape, int type, int64_t I, int64_t J, int64_t K, int bi,
+           int bj, int bk, float alone, float shared, int share) {
+  const int64_t all = div_up(K, bk);
+  const float hbm = (type == VC_FP32 ? 6.f : 2.f) * (I + J) * K / 4.5e6f;
   const int64_t nj = div_up(J, bj), tiles = div_up(I, bi) * nj;
   for (int64_t want = 1; want <= 32 && (want == 1 || 4 * want <= all); want *= 2) {
     const int64_t steps = div_up(all, want) > 0 ? div_up(all, want) : 1;
     const int64_t slices = div_up(all, steps) > 0 ? div_up(all, steps) : 1;
     const int64_t load = div_up(tiles * slices, kCus);
-    const float a = alone * div_up(load, share), s = shared * load;
-    // the slices' sums are written, read again and joined by a launch
-    const float us = 4.f + steps * (a > s ? a : s) +
-                     (slices > 1 ? 4.f + 8.f * slices * I * J / 4e6f : 0.f);
+    const float a = steps * alone * div_up(load, share), s = steps * shared * load;
+    const float work = a > s ? a : s;
+    const float us = 4.f + (work > hbm ? work : hbm) + join_us(slices, I, J);
     if (us < best.us) best = {kernel, shape, (int)slices, (int)steps, tiles, nj, us};
   }
 }
@@ -559,7 +575,7 @@ Cut cut_product(int type, int64_t I, int64_t J, int64_t K) {
   Cut c = {};
   c.us = 1e30f;
   const bool f = type == VC_FP32;
-  slice(c, kProduct, 0, I, J, 64, 64, div_up(K, f ? 32 : 64), f ? 1.0f : 0.9f, f ? 0.9f : 0.5f, 2);
+  slice(c, kProduct, 0, type, I, J, K, 64, 64, f ? 32 : 64, f ? 1.0f : 0.9f, f ? 0.9f : 0.5f, 2);
   return c;
 }
 
@@ -576,14 +592,15 @@ Cut cut_tiles(int type, int64_t I, int64_t J, int64_t K) {
   const int b = type == VC_FP32 ? 0 : 1;
   for (int shape = 0; shape < (b ? 3 : 2); ++shape) {
     const TileShape t = tile_shape(type, shape);
-    slice(c, kTile, shape, I, J, t.bi, t.bj, div_up(K, t.bk), kStepAlone[b][shape],
+    slice(c, kTile, shape, type, I, J, K, t.bi, t.bj, t.bk, kStepAlone[b][shape],
           kStepShared[b][shape], kShare[b][shape]);
   }
   return c;
 }
 
 // The direct kernel: 16 rows by 16 columns, 32 by 16, 64 by 16, 64 by 32.  A
-// workgroup's operands come at about 45 GB/s a CU, all of them together at no
+// workgroup's operands come at about 25 GB/s a CU (sixteen rows a load, 16 bytes a
+// lane), all of them together at no
 // more than the memory's rate.
 constexpr int kDirectRows[4] = {16, 32, 64, 64}, kDirectCols[4] = {16, 16, 16, 32};
 
@@ -597,9 +614,9 @@ Cut cut_direct(int type, int64_t I, int64_t J, int64_t K) {
     int64_t s = 1;
     while (tiles * s < kCus && 1024 * s < K && s < 16) s *= 2;
     const float own = e * ((I < bi ? I : bi) + bj) * (float)K / s;
-    const float l2 = div_up(tiles * s, kCus) * own / 45e3f;
+    const float l2 = div_up(tiles * s, kCus) * own / 25e3f;
     const float hbm = e * (I + J) * (float)K / 4.5e6f;
-    const float us = 5.f + (l2 > hbm ? l2 : hbm) + (s > 1 ? 4.f + 8.f * s * I * J / 4e6f : 0.f);
+    const float us = 3.f + (l2 > hbm ? l2 : hbm) + join_us(s, I, J);
     if (us < c.us) c = {kDirect, shape, (int)s, 0, tiles, nj, us};
   }
   return c;
@@ -648,7 +665,7 @@ int run_product(Product<T> a, const Cut& c, void* work, int64_t work_bytes, hipS
   } else {
     constexpr bool F = sizeof(T) == 4;
     const int threads = 64 * kDirectWaves;
-    if (c.shape == 0) k_direct<T, 1, 1, 4><<<grid, threads, 0, st>>>(a);
+    if (c.shape == 0) k_direct<T, 1, 1, F ? 2 : 8><<<grid, threads, 0, st>>>(a);
     else if (c.shape == 1) k_direct<T, 1, 2, F ? 2 : 4><<<grid, threads, 0, st>>>(a);
     else if (c.shape == 2) k_direct<T, 1, 4, F ? 1 : 2><<<grid, threads, 0, st>>>(a);
     else k_direct<T, 2, 4, F ? 1 : 2><<<grid, threads, 0, st>>>(a);

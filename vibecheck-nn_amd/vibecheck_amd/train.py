@@ -8,6 +8,7 @@ raise RuntimeError, other types NotImplementedError, sizes that do not fit
 ValueError.
 """
 import ctypes
+import math
 
 import torch
 
@@ -29,16 +30,16 @@ def _type(t, what):
     k = _TYPES.get(t.dtype)
     if k is None:
         raise NotImplementedError(f'vibecheck_amd: {what} is {t.dtype}; fp32 and bf16 are taken')
-    if t.device.index != torch._C._cuda_getDevice():
+    if t.get_device() != torch._C._cuda_getDevice():
         raise ValueError(f'vibecheck_amd: {what} is on {t.device}, not on the current device')
     return k
 
 
 def _like(t, ref, shape, what):
-    if t.dtype != ref.dtype or t.device != ref.device:
+    if t.dtype != ref.dtype or t.get_device() != ref.get_device():
         raise ValueError(f'vibecheck_amd: {what} is {t.dtype} on {t.device}, '
                          f'expected {ref.dtype} on {ref.device}')
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f'vibecheck_amd: {what} has shape {tuple(t.shape)}, '
                          f'expected {tuple(shape)}')
 
@@ -46,6 +47,8 @@ def _like(t, ref, shape, what):
 def _rows(t):
     """t as rows of its last axis, values of a row side by side: (tensor to keep, row stride)."""
     n = t.shape[-1]
+    if t.is_contiguous():
+        return t, n
     if t.dim() != 2:
         t = t.reshape(-1, n)
     if t.shape[0] <= 1 or n == 0:
@@ -59,10 +62,23 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _work(nbytes, device):
-    if nbytes < 0:
-        raise ValueError('vibecheck_amd: sizes out of range')
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+_sizes = {}  # (function, its arguments): the bytes it gave
+
+
+def _work(like, name, *args):
+    """(tensor to keep or None, its pointer, its bytes) of a call's workspace."""
+    n = _sizes.get((name, args))
+    if n is None:
+        n = getattr(load(), name)(*args)
+        if n < 0:
+            raise ValueError('vibecheck_amd: sizes out of range')
+        if len(_sizes) > 4096:
+            _sizes.clear()
+        _sizes[name, args] = n
+    if n == 0:
+        return None, None, 0
+    t = torch.empty(n, dtype=torch.uint8, device=like.device)
+    return t, t.data_ptr(), n
 
 
 # ------------------------------------------------------------------- fc layer
@@ -79,7 +95,7 @@ def _linear(x, W, bias, act, residual, save):
         raise ValueError('vibecheck_amd: x has at least one axis, W two')
     N, K = W.shape
     _like(W, x, (N, x.shape[-1]), 'W')
-    shape = x.shape[:-1] + (N,)
+    shape = (*x.shape[:-1], N)
     if bias is not None:
         _like(bias, x, (N,), 'bias')
         bias = bias.contiguous()
@@ -87,18 +103,17 @@ def _linear(x, W, bias, act, residual, save):
         _like(residual, x, shape, 'residual')
     x, ldx = _rows(x)
     W = W.contiguous()
-    M = x.numel() // K if K else shape.numel() // max(1, N)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    M = math.prod(shape[:-1])
+    y = x.new_empty(shape)
     # the sign of relu's output is its input's; another activation's input is kept
     z = torch.empty_like(y) if save and act and (act != 1 or residual is not None) else None
     if residual is not None:
         residual, ldr = _rows(residual)
     else:
         ldr = 0
-    work = _work(load().vc_linear_workspace(k, M, K, N), x.device)
+    work, at, nbytes = _work(x, 'vc_linear_workspace', k, M, K, N)
     call('vc_linear', k, x.data_ptr(), M, K, ldx, W.data_ptr(), N, _ptr(bias), act,
-         _ptr(residual), ldr, y.data_ptr(), _ptr(z), _ptr(work), work.numel() if work is not None else 0,
-         stream())
+         _ptr(residual), ldr, y.data_ptr(), _ptr(z), at, nbytes, stream())
     return y, (y if save and act and z is None else z)
 
 
@@ -146,7 +161,7 @@ def linear_backward(dy, x, W, z=None, act=None, need=('x', 'W', 'bias')):
         raise ValueError(f"vibecheck_amd: need names {need!r}; 'x', 'W' and 'bias' are taken")
     N, K = W.shape
     _like(W, dy, (dy.shape[-1], K), 'W')
-    lead = dy.shape[:-1]
+    lead = tuple(dy.shape[:-1])
     _like(x, dy, lead + (K,), 'x')
     if a:
         if z is None:
@@ -155,20 +170,18 @@ def linear_backward(dy, x, W, z=None, act=None, need=('x', 'W', 'bias')):
         z, ldz = _rows(z)
     else:
         z, ldz = None, 0
-    M = lead.numel()
-    new = dict(dtype=dy.dtype, device=dy.device)
-    dx = torch.empty(lead + (K,), **new) if 'x' in need else None
-    dW = torch.empty(N, K, **new) if 'W' in need else None
+    M = math.prod(lead)
+    dx = dy.new_empty(lead + (K,)) if 'x' in need else None
+    dW = dy.new_empty((N, K)) if 'W' in need else None
     # no row adds to it, no launch writes it
-    db = (torch.empty if M else torch.zeros)(N, **new) if 'bias' in need else None
+    db = (dy.new_empty if M else dy.new_zeros)(N) if 'bias' in need else None
     dy, ldy = _rows(dy)
     x, ldx = _rows(x)
     W = W.contiguous()
     which = (dx is not None) + 2 * (dW is not None) + 4 * (db is not None)
-    work = _work(load().vc_linear_backward_workspace(k, M, K, N, a, which), dy.device)
+    work, at, nbytes = _work(dy, 'vc_linear_backward_workspace', k, M, K, N, a, which)
     call('vc_linear_backward', k, dy.data_ptr(), ldy, x.data_ptr(), ldx, W.data_ptr(), _ptr(z), ldz,
-         a, M, K, N, _ptr(dx), _ptr(dW), _ptr(db), _ptr(work),
-         work.numel() if work is not None else 0, stream())
+         a, M, K, N, _ptr(dx), _ptr(dW), _ptr(db), at, nbytes, stream())
     return dx, dW, db
 
 
@@ -197,7 +210,7 @@ def _cross_entropy(logits, target, reduction, ignore_index, smoothing, grad, out
     if not 0 <= smoothing <= 1:
         raise ValueError(f'vibecheck_amd: smoothing {smoothing} is not in [0, 1]')
     lead, V = logits.shape[:-1], logits.shape[-1]
-    if target.dtype != torch.int64 or target.device != logits.device or target.shape != lead:
+    if target.dtype != torch.int64 or target.get_device() != logits.get_device() or target.shape != lead:
         raise ValueError(f'vibecheck_amd: target is {target.dtype} {tuple(target.shape)} on '
                          f'{target.device}, expected int64 {tuple(lead)} on {logits.device}')
     R, kind = lead.numel(), REDUCTIONS[reduction]
@@ -208,13 +221,12 @@ def _cross_entropy(logits, target, reduction, ignore_index, smoothing, grad, out
             raise ValueError('vibecheck_amd: out must be contiguous')
         d = out
     else:
-        d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None
+        d = logits.new_empty(logits.shape) if grad else None
     z, ld = _rows(logits)
     target = target.contiguous()
-    work = _work(load().vc_cross_entropy_workspace(R, kind), logits.device)
+    work, at, nbytes = _work(logits, 'vc_cross_entropy_workspace', R, kind)
     call('vc_cross_entropy', k, z.data_ptr(), R, V, ld, target.data_ptr(), ignore_index, smoothing,
-         kind, loss.data_ptr(), _ptr(d), V, _ptr(work), work.numel() if work is not None else 0,
-         stream())
+         kind, loss.data_ptr(), _ptr(d), V, at, nbytes, stream())
     return loss, d
 
 
@@ -272,9 +284,9 @@ def adamw_moments(params, state):
 
 def _one_type(tensors, sizes, what):
     """Type number and pointers of a list of contiguous GPU tensors of one type."""
-    k, kind, dev = _type(tensors[0], what), tensors[0].dtype, tensors[0].device
+    k, kind, dev = _type(tensors[0], what), tensors[0].dtype, tensors[0].get_device()
     for t, n in zip(tensors, sizes):
-        if t.dtype != kind or t.device != dev or t.numel() != n or not t.is_contiguous():
+        if t.dtype is not kind or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
             raise ValueError(f'vibecheck_amd: {what} are contiguous, of one type, on one device '
                              f'and of their parameters\' sizes; got {t.dtype} {tuple(t.shape)} '
                              f'on {t.device}')
@@ -300,8 +312,7 @@ def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8
         raise ValueError('vibecheck_amd: one gradient (and copy) for each parameter')
     kp, pp = _one_type(params, sizes, 'params')
     kg, pg = _one_type(grads, sizes, 'grads')
-    if grads[0].device != params[0].device:
-        raise ValueError('vibecheck_amd: params and grads are on different devices')
+    dev = params[0].get_device()  # the current one, as the gradients' and copies' is
     n, cnt = sum((k + BLOCK - 1) // BLOCK for k in sizes), len(sizes)
     bits = state['bits']
     keys = ('m', 'v') if bits == 32 else ('m', 'v', 'm_scale', 'v_scale')
@@ -309,18 +320,18 @@ def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8
         t = state[key]
         want = torch.float32 if bits == 32 or key[1:] else torch.uint8
         if t.dtype != want or t.numel() != (n if key[1:] else n * BLOCK) or \
-                t.device != params[0].device or not t.is_contiguous():
+                t.get_device() != dev or not t.is_contiguous():
             raise ValueError(f'vibecheck_amd: state {key!r} does not fit these parameters')
     array = ctypes.c_void_p * cnt
     if copies is not None:
         kc, pc = _one_type(copies, sizes, 'copies')
-        if kc != 1 or copies[0].device != params[0].device:
+        if kc != 1:
             raise ValueError('vibecheck_amd: copies are bf16 tensors beside their parameters')
         pc = array(*pc)
     else:
         pc = None
     if scale is not None and (scale.dtype != torch.float32 or scale.numel() != 1 or
-                              scale.device != params[0].device):
+                              scale.get_device() != dev):
         raise ValueError('vibecheck_amd: scale is one fp32 value on the parameters\' device')
     pp, pg, pn = array(*pp), array(*pg), (ctypes.c_int64 * cnt)(*sizes)
     call('vc_adamw_step', ctypes.addressof(pp), ctypes.addressof(pg),
