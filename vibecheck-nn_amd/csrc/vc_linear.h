@@ -127,8 +127,22 @@ struct TileShape {
   int bi, bj, bk;
 };
 TileShape tile_shape(int type, int shape);
+
+// The blocks' sums of dz's columns, joined: 32 columns a workgroup.
 template <class T>
-void run_tiles(const Product<T>& a, int shape, bool xa, bool xb, hipStream_t st);
+struct Columns {
+  const float* sums;  // (blocks, N)
+  int blocks, N;
+  T* db;
+};
+
+// The forward's product.
+template <class T>
+void run_tile(const Product<T>& a, int shape, hipStream_t st);
+// The backward's two and the columns' sums, in one launch of `grid` workgroups.
+template <class T>
+void run_tiles(const Product<T>& w, const Product<T>& x, const Columns<T>& c, int shape,
+               unsigned grid, hipStream_t st);
 
 // Four columns j .. j + 3 of row i: bias, activation, residual, stores.
 template <class T>
@@ -184,6 +198,38 @@ __device__ __forceinline__ void finish(const Product<T>& a, int64_t i, int j, co
     put(o + q, v[q]);
     if (a.z) put(a.z + i * a.J + j + q, z[q]);
   }
+}
+
+// Four columns of row i of a slice: finished, or left for the join.
+template <class T>
+__device__ __forceinline__ void deliver(const Product<T>& a, int64_t slice, int64_t i, int j,
+                                        const float* v) {
+  if (a.slices == 1) {
+    finish(a, i, j, v);
+    return;
+  }
+  float* const o = a.part + (slice * a.I + i) * a.J + j;
+  if (a.J % 4 == 0) {
+    *reinterpret_cast<v4f*>(o) = v4f{v[0], v[1], v[2], v[3]};
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (j + q < a.J) o[q] = v[q];
+  }
+}
+
+// lds: 32 floats for every 32 threads.
+template <class T>
+__device__ __forceinline__ void add_columns(const Columns<T>& a, int block, float* lds) {
+  const int c = threadIdx.x & 31, y = threadIdx.x >> 5, ny = blockDim.x >> 5, j = block * 32 + c;
+  float s = 0.f;
+  if (j < a.N)
+    for (int b = y; b < a.blocks; b += ny) s += a.sums[(int64_t)b * a.N + j];
+  lds[y * 32 + c] = s;
+  __syncthreads();
+  if (y || j >= a.N) return;
+  for (int i = 1; i < ny; ++i) s += lds[i * 32 + c];
+  put(a.db + j, s);
 }
 
 }  // namespace vcl

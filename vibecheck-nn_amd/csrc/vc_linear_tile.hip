@@ -135,19 +135,22 @@ __device__ __forceinline__ void turn() {
 // NBUF: LDS buffers.  TURNS: the waves take turns, one for each 32 of k.
 template <class T, int NP, bool XA, bool XB, int BI, int BJ, int WI, int WJ, int BK, int NBUF,
           bool TURNS>
-__global__ __launch_bounds__(64 * WI * WJ, 2) void k_tile(Product<T> a) {
+__device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* lds) {
   constexpr int NW = WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16;
   typedef Side<XA, BI, BK, NW> SA;
   typedef Side<XB, BJ, BK, NW> SB;
   constexpr int kStage = NP * (SA::kBytes + SB::kBytes);
-  extern __shared__ __align__(1024) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ni = (a.I + BI - 1) / BI, nj = (a.J + BJ - 1) / BJ;
   int ti, tj;
-  tile_of(vcg::xcd_tile(blockIdx.x, a.tiles), ni, nj, ti, tj);
+  // in scalar registers, as the bases of the loads into LDS have to be
+  const int slice = __builtin_amdgcn_readfirstlane(block / (uint32_t)a.tiles);
+  tile_of(vcg::xcd_tile(block - slice * (uint32_t)a.tiles, a.tiles), ni, nj, ti, tj);
+  ti = __builtin_amdgcn_readfirstlane(ti);
+  tj = __builtin_amdgcn_readfirstlane(tj);
   const int i0 = ti * BI, j0 = tj * BJ;
-  const int64_t k0 = (int64_t)blockIdx.y * a.steps * BK;
+  const int64_t k0 = (int64_t)slice * a.steps * BK;
   const int left = (int)min((int64_t)a.steps * BK, a.K - k0);
   const int full = left / BK;
   const int wi = wv / WJ, wj = wv % WJ;
@@ -172,7 +175,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void k_tile(Product<T> a) {
   // operands the tiles of an XCD start at eight places 256 bytes apart and wrap
   // (8192 x 16384 x 4096 1137 -> 1007 us; with one, 262 -> 283, the tiles then no
   // longer share what they read).
-  const int first = XA || XB || full == 0 ? 0 : (int)(blockIdx.x >> 3) % 8 * (128 / BK) % full;
+  const int first = XA || XB || full == 0 ? 0 : (int)(block >> 3) % 8 * (128 / BK) % full;
   const auto load = [&](int step, char* to) {
     const int s = step + first < full ? step + first : step + first - full;
     const uint16_t* const fa = sa.base + (XA ? (int64_t)s * BK * a.lda : (int64_t)s * BK);
@@ -293,70 +296,105 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void k_tile(Product<T> a) {
     }
   }
 
+  // The sums go through LDS, as many rows as fit: what follows them (bias,
+  // activation, residual, stores of whole lines) is one short loop.  Four columns
+  // c of row i at c ^ (i mod 16).
+  constexpr int Q = BJ / 4, kFit = NBUF * kStage / (BJ * 4), ROWS = kFit < BI ? BI / WI : BI;
+  static_assert(ROWS <= kFit && Q >= 16);
+  v4f* const sums = reinterpret_cast<v4f*>(lds);
   const int g = lane >> 4, r = lane & 15;
+#pragma unroll 1
+  for (int p = 0; p < BI / ROWS; ++p) {
+    __syncthreads();
+    if (ROWS == BI || p == wi) {
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int64_t row = i0 + (wi * MI + i) * 16 + r;
-    if (row >= a.I) continue;
+      for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < MJ; ++j) {
-      const int col = j0 + (wj * MJ + j) * 16 + 4 * g;
-      if (col >= a.J) continue;
-      float v[4];
+        for (int j = 0; j < MJ; ++j) {
+          v4f v = acc[i][j];
+          if constexpr (NP == 3) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        v[q] = acc[i][j][q];
-        if (NP == 3) {
-          const float t = v[q] + small[i][j][q];
-          v[q] = finite(t) ? t : v[q];
+            for (int q = 0; q < 4; ++q) {
+              const float t = v[q] + small[i][j][q];
+              v[q] = finite(t) ? t : v[q];
+            }
+          }
+          const int row = ((ROWS == BI ? wi * MI : 0) + i) * 16 + r;
+          sums[row * Q + (((wj * MJ + j) * 4 + g) ^ (row & 15))] = v;
         }
-      }
-      if (a.slices == 1) {
-        finish(a, row, col, v);
-        continue;
-      }
-      float* const o = a.part + ((int64_t)blockIdx.y * a.I + row) * a.J + col;
-      if (a.J % 4 == 0) {
-        *reinterpret_cast<v4f*>(o) = v4f{v[0], v[1], v[2], v[3]};
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (col + q < a.J) o[q] = v[q];
-      }
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int t = tid; t < ROWS * Q; t += 64 * NW) {
+      const int row = t / Q, q = t % Q;
+      const int64_t i = i0 + p * ROWS + row;
+      const int j = j0 + 4 * q;
+      if (i >= a.I || j >= a.J) continue;
+      const v4f w = sums[row * Q + (q ^ (row & 15))];
+      const float v[4] = {w[0], w[1], w[2], w[3]};
+      deliver(a, slice, i, j, v);
     }
   }
 }
 
-template <class T, bool XA, bool XB, int SHAPE>
+template <class T, int SHAPE>
 struct Form {
   static constexpr bool F = sizeof(T) == 4;
   static constexpr int NP = F ? 3 : 1;
   static constexpr int BI = (SHAPE == 0 ? 256 : SHAPE == 1 ? 128 : 64) / (F && SHAPE < 2 ? 2 : 1);
-  static constexpr int BJ = BI, WI = 2, WJ = SHAPE == 0 ? 4 : 2;
+  static constexpr int WI = 2, WJ = SHAPE == 0 ? 4 : 2;
   static constexpr int BK = F ? 32 : 64;
   static constexpr int NBUF = F && SHAPE == 0 ? 3 : 2;
-  static constexpr int TURNS = SHAPE == 0;
   static constexpr int kThreads = 64 * WI * WJ;
-  static constexpr int kLds = NBUF * NP * (BI + BJ) * BK * 2;
-  static void run(const Product<T>& a, hipStream_t st) {
-    const auto k = k_tile<T, NP, XA, XB, BI, BJ, WI, WJ, BK, NBUF, TURNS>;
-    static bool set[16];
-    int dev = 0;
-    (void)hipGetDevice(&dev);
-    if (!set[dev & 15]) {
-      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k),
-                                hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-      set[dev & 15] = true;
-    }
-    k<<<dim3((unsigned)a.tiles, (unsigned)a.slices), kThreads, kLds, st>>>(a);
+  static constexpr int kLds = NBUF * NP * 2 * BI * BK * 2;
+  template <bool XA, bool XB>
+  static __device__ __forceinline__ void run(const Product<T>& a, uint32_t block, char* lds) {
+    tile<T, NP, XA, XB, BI, BI, WI, WJ, BK, NBUF, SHAPE == 0>(a, block, lds);
   }
 };
 
 template <class T, int SHAPE>
-void run_shape(const Product<T>& a, bool xa, bool xb, hipStream_t st) {
-  if (xa) Form<T, true, true, SHAPE>::run(a, st);
-  else if (xb) Form<T, false, true, SHAPE>::run(a, st);
-  else Form<T, false, false, SHAPE>::run(a, st);
+__global__ __launch_bounds__((Form<T, SHAPE>::kThreads), 2) void k_tile(Product<T> a) {
+  extern __shared__ __align__(1024) char lds[];
+  Form<T, SHAPE>::template run<false, false>(a, blockIdx.x, lds);
+}
+
+// Workgroups of dW (the longer sums), then of dx, then of the columns' sums.
+template <class T, int SHAPE>
+__global__ __launch_bounds__((Form<T, SHAPE>::kThreads), 2) void k_tiles(Product<T> w, Product<T> x,
+                                                                      Columns<T> c) {
+  extern __shared__ __align__(1024) char lds[];
+  const uint32_t nw = w.tiles * w.slices, nx = x.tiles * x.slices, b = blockIdx.x;
+  if (b < nw) Form<T, SHAPE>::template run<true, true>(w, b, lds);
+  else if (b < nw + nx) Form<T, SHAPE>::template run<false, true>(x, b - nw, lds);
+  else add_columns(c, (int)(b - nw - nx), reinterpret_cast<float*>(lds));
+}
+
+// A kernel's LDS limit, set once per device.
+template <class K>
+void allow_lds(K k, int bytes, bool* set) {
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  if (set[dev & 15]) return;
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  set[dev & 15] = true;
+}
+
+template <class T, int SHAPE>
+void one(const Product<T>& a, hipStream_t st) {
+  typedef Form<T, SHAPE> Fm;
+  static bool set[16];
+  allow_lds(k_tile<T, SHAPE>, Fm::kLds, set);
+  k_tile<T, SHAPE><<<(unsigned)(a.tiles * a.slices), Fm::kThreads, Fm::kLds, st>>>(a);
+}
+
+template <class T, int SHAPE>
+void both(const Product<T>& w, const Product<T>& x, const Columns<T>& c, unsigned grid, hipStream_t st) {
+  typedef Form<T, SHAPE> Fm;
+  static bool set[16];
+  allow_lds(k_tiles<T, SHAPE>, Fm::kLds, set);
+  k_tiles<T, SHAPE><<<grid, Fm::kThreads, Fm::kLds, st>>>(w, x, c);
 }
 
 }  // namespace
@@ -370,12 +408,23 @@ TileShape tile_shape(int type, int shape) {
 }
 
 template <class T>
-void run_tiles(const Product<T>& a, int shape, bool xa, bool xb, hipStream_t st) {
-  if (shape == 0) run_shape<T, 0>(a, xa, xb, st);
-  else if (shape == 1) run_shape<T, 1>(a, xa, xb, st);
-  else if constexpr (sizeof(T) == 2) run_shape<T, 2>(a, xa, xb, st);
+void run_tile(const Product<T>& a, int shape, hipStream_t st) {
+  if (shape == 0) one<T, 0>(a, st);
+  else if (shape == 1) one<T, 1>(a, st);
+  else if constexpr (sizeof(T) == 2) one<T, 2>(a, st);
 }
-template void run_tiles<float>(const Product<float>&, int, bool, bool, hipStream_t);
-template void run_tiles<uint16_t>(const Product<uint16_t>&, int, bool, bool, hipStream_t);
+template <class T>
+void run_tiles(const Product<T>& w, const Product<T>& x, const Columns<T>& c, int shape,
+               unsigned grid, hipStream_t st) {
+  if (shape == 0) both<T, 0>(w, x, c, grid, st);
+  else if (shape == 1) both<T, 1>(w, x, c, grid, st);
+  else if constexpr (sizeof(T) == 2) both<T, 2>(w, x, c, grid, st);
+}
+template void run_tile<float>(const Product<float>&, int, hipStream_t);
+template void run_tile<uint16_t>(const Product<uint16_t>&, int, hipStream_t);
+template void run_tiles<float>(const Product<float>&, const Product<float>&, const Columns<float>&,
+                               int, unsigned, hipStream_t);
+template void run_tiles<uint16_t>(const Product<uint16_t>&, const Product<uint16_t>&,
+                                  const Columns<uint16_t>&, int, unsigned, hipStream_t);
 
 }  // namespace vcl

@@ -9,6 +9,7 @@ ValueError.
 """
 import ctypes
 import math
+import operator
 
 import torch
 
@@ -282,15 +283,20 @@ def adamw_moments(params, state):
     return out
 
 
+_numel, _data_ptr = torch.Tensor.numel, torch.Tensor.data_ptr
+_device_of, _contiguous = torch.Tensor.get_device, torch.Tensor.is_contiguous
+_dtype_of = operator.attrgetter('dtype')
+
+
 def _one_type(tensors, sizes, what):
     """Type number and pointers of a list of contiguous GPU tensors of one type."""
-    k, kind, dev = _type(tensors[0], what), tensors[0].dtype, tensors[0].get_device()
-    for t, n in zip(tensors, sizes):
-        if t.dtype is not kind or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
-            raise ValueError(f'vibecheck_amd: {what} are contiguous, of one type, on one device '
-                             f'and of their parameters\' sizes; got {t.dtype} {tuple(t.shape)} '
-                             f'on {t.device}')
-    return k, [t.data_ptr() for t in tensors]
+    k = _type(tensors[0], what)
+    if len(set(map(_dtype_of, tensors))) > 1 or len(set(map(_device_of, tensors))) > 1 or \
+            list(map(_numel, tensors)) != sizes or not all(map(_contiguous, tensors)):
+        raise ValueError(f'vibecheck_amd: {what} are contiguous, of one type, on one device and '
+                         f'of their parameters\' sizes {sizes}; got '
+                         f'{[(t.dtype, str(t.device), tuple(t.shape)) for t in tensors]}')
+    return k, list(map(_data_ptr, tensors))
 
 
 def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
@@ -307,7 +313,7 @@ def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8
     params, grads = list(params), list(grads)
     if not params:
         return
-    sizes = [p.numel() for p in params]
+    sizes = list(map(_numel, params))
     if len(grads) != len(params) or (copies is not None and len(copies) != len(params)):
         raise ValueError('vibecheck_amd: one gradient (and copy) for each parameter')
     kp, pp = _one_type(params, sizes, 'params')
