@@ -117,8 +117,8 @@ struct Product {
   int64_t lda, ldb, planeA, planeB;
 };
 
-// The tiled products of vc_linear_tile.hip, shape 0 the largest (bf16 256 x 256,
-// 128 x 128, 64 x 64; fp32 128 x 128, 64 x 64).  Rows (across: k) lie lda, ldb
+// The tiled products of vc_linear_tile.hip, shapes 0, 1, 2: 256 x 256 (fp32 256 x
+// 128), 128 x 128, 64 x 64.  Rows (across: k) lie lda, ldb
 // values apart.  The caller has seen to it that every operand's base and ld are
 // multiples of 16 bytes, that K is a multiple of eight (an operand whose k is
 // contiguous) or its lines are padded to one (read across), and that 256 of them

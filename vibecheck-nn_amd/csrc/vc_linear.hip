@@ -29,20 +29,39 @@ struct Raw {
 };
 
 // Values k .. k + 7 of a row of K; past the end zero.  whole (the same in all
-// lanes): none is.  A branch that lanes do not share would have each load waited
-// for before the next.
+// lanes): none is.  Every lane loads, and moves and masks what it has afterwards: a
+// branch that lanes do not share would have each load waited for before the next.
 template <class T>
 __device__ __forceinline__ void load_k8(const T* p, int k, int K, bool whole, uint32_t* d) {
   constexpr bool F = sizeof(T) == 4;
-  if (whole) {
-    const u4 a = load16(p + k);
+  constexpr int D = F ? 8 : 4;
+  if (whole || K >= 8) {
+    const int at = whole ? k : min(k, K - 8);
+    const u4 a = load16(p + at);
 #pragma unroll
     for (int j = 0; j < 4; ++j) d[j] = a[j];
     if (F) {
-      const u4 b = load16(p + k + 4);
+      const u4 b = load16(p + at + 4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) d[(4 + j) % (F ? 8 : 4)] = b[j];
+      for (int j = 0; j < 4; ++j) d[(4 + j) % D] = b[j];
     }
+    if (whole) return;
+    const int over = min(k - at, 8);  // values to drop from the front, zeros behind
+#pragma unroll
+    for (int step = 4; step >= 1; step /= 2) {
+      const bool on = over & step;
+      if (F || step > 1) {
+        const int n = F ? step : step / 2;
+#pragma unroll
+        for (int j = 0; j < D; ++j) d[j] = on ? (j + n < D ? d[(j + n) % D] : 0) : d[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < D; ++j)
+          d[j] = on ? d[j] >> 16 | (j + 1 < D ? d[(j + 1) % D] << 16 : 0) : d[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < D; ++j) d[j] = over >= 8 ? 0 : d[j];
     return;
   }
   uint32_t w[8];
@@ -54,7 +73,7 @@ __device__ __forceinline__ void load_k8(const T* p, int k, int K, bool whole, ui
     w[j] = k + j < K ? w[j] : 0;
   }
 #pragma unroll
-  for (int j = 0; j < (F ? 8 : 4); ++j) d[j] = F ? w[j] : w[2 * j % 8] | w[(2 * j + 1) % 8] << 16;
+  for (int j = 0; j < D; ++j) d[j] = F ? w[j] : w[2 * j % 8] | w[(2 * j + 1) % 8] << 16;
 }
 
 template <class T, bool ACROSS>
@@ -69,10 +88,10 @@ __device__ __forceinline__ void load_unit(const Operand<T>& o, int row, int k, i
   }
   // past the last row the last two (mend_unit)
   const int r0 = max(min(row, o.rows - 2), 0);
-  if (whole && o.rows > 1) {  // loads alone: nothing here waits for them
+  if (o.rows > 1) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const T* const p = o.p + (int64_t)(k + j) * o.ld + r0;
+      const T* const p = o.p + (int64_t)(whole ? k + j : min(k + j, K - 1)) * o.ld + r0;
       if constexpr (F) {
         const u2 w = *reinterpret_cast<const u2at4*>(p);
         v.d[2 * j] = w.x;
@@ -81,18 +100,23 @@ __device__ __forceinline__ void load_unit(const Operand<T>& o, int row, int k, i
         v.d[j] = *reinterpret_cast<const u1at2*>(p);
       }
     }
-    return;
+    if (whole) return;  // loads alone: nothing here waits for them
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const T w = o.p[(int64_t)min(k + j, K - 1) * o.ld];
+      if constexpr (F) v.d[2 * j] = v.d[2 * j + 1] = __builtin_bit_cast(uint32_t, w);
+      else v.d[j] = (uint32_t)w | (uint32_t)w << 16;
+    }
   }
-  const int r1 = min(r0 + 1, o.rows - 1);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const T* const p = o.p + (int64_t)min(k + j, K - 1) * o.ld;
     const bool in = k + j < K;
     if constexpr (F) {
-      v.d[2 * j] = in ? __builtin_bit_cast(uint32_t, p[r0]) : 0;
-      v.d[2 * j + 1] = in ? __builtin_bit_cast(uint32_t, p[r1]) : 0;
+      v.d[2 * j] = in ? v.d[2 * j] : 0;
+      v.d[2 * j + 1] = in ? v.d[2 * j + 1] : 0;
     } else {
-      v.d[j] = in ? (uint32_t)p[r0] | (uint32_t)p[r1] << 16 : 0;
+      v.d[j] = in ? v.d[j] : 0;
     }
   }
 }
@@ -357,10 +381,11 @@ __global__ __launch_bounds__(64 * kDirectWaves, 2) void k_direct(Product<T> a) {
     }
   // slices: workgroups, then waves, take every 64-deep piece in turn
   const int each = NW * gridDim.y;
-  const auto pieces = [&](int c, auto whole) {
-    uint32_t da[UN][2][MB][D], db[UN][2][NB][D];
+  const auto pieces = [&](int c, bool whole, auto count) {
+    constexpr int N = decltype(count)::value;
+    uint32_t da[N][2][MB][D], db[N][2][NB][D];
 #pragma unroll
-    for (int u = 0; u < UN; ++u)
+    for (int u = 0; u < N; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int k = (c + u * each) * 64 + 32 * h + 8 * g;
@@ -370,7 +395,7 @@ __global__ __launch_bounds__(64 * kDirectWaves, 2) void k_direct(Product<T> a) {
         for (int i = 0; i < MB; ++i) load_k8(pa[i], k, a.K, whole, da[u][h][i]);
       }
 #pragma unroll
-    for (int u = 0; u < UN; ++u)
+    for (int u = 0; u < N; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         u4 fb[NB][NP];
@@ -394,10 +419,10 @@ __global__ __launch_bounds__(64 * kDirectWaves, 2) void k_direct(Product<T> a) {
         }
       }
   };
-  for (int c = blockIdx.y * NW + wv; c * 64 < a.K; c += UN * each) {
-    if ((c + (UN - 1) * each) * 64 + 64 <= a.K) pieces(c, std::true_type{});
-    else pieces(c, std::false_type{});
-  }
+  int c = blockIdx.y * NW + wv;
+  for (; (c + (UN - 1) * each) * 64 + 64 <= a.K; c += UN * each)
+    pieces(c, true, std::integral_constant<int, UN>{});
+  for (; c * 64 < a.K; c += each) pieces(c, c * 64 + 64 <= a.K, std::integral_constant<int, 1>{});
 #pragma unroll
   for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -688,14 +713,13 @@ constexpr int kGroups32 = 3, kGroups16 = 4;
 // several that share one (measured on 264 x 328 and 512 x 512 outputs, and on 8192
 // x 16384 and 4096 x 4096).
 Cost tile_cost(int type, int shape) {
-  constexpr float alone[2][3] = {{1.15f, 0.50f, 0.f}, {1.45f, 1.0f, 0.45f}};
-  constexpr float shared[2][3] = {{1.39f, 0.46f, 0.f}, {1.95f, 0.55f, 0.21f}};
-  constexpr int share[2][3] = {{1, 3, 1}, {1, 2, 4}};
+  constexpr float alone[2][3] = {{2.0f, 1.1f, 0.8f}, {1.45f, 1.1f, 0.5f}};
+  constexpr float shared[2][3] = {{2.13f, 1.1f, 0.4f}, {1.9f, 0.58f, 0.21f}};
+  constexpr int share[2][3] = {{1, 1, 3}, {1, 2, 4}};
   const TileShape t = tile_shape(type, shape);
   const int b = type == VC_FP32 ? 0 : 1;
   return {t.bi, t.bj, t.bk, share[b][shape], alone[b][shape], shared[b][shape]};
 }
-constexpr int tile_shapes(int type) { return type == VC_FP32 ? 2 : 3; }
 
 // Up to two products by the kernel and shape expected to be fastest.  extra: what
 // the tiles' parts cost before.
@@ -713,7 +737,7 @@ float choose(int type, const Job* job, int n, bool tiles, float extra, Cut* out)
   };
   for (int shape = 0; shape < 2; ++shape) take(kProduct, shape, product_cost(type, shape), 0.f);
   if (tiles)
-    for (int shape = 0; shape < tile_shapes(type); ++shape) take(kTile, shape, tile_cost(type, shape), extra);
+    for (int shape = 0; shape < 3; ++shape) take(kTile, shape, tile_cost(type, shape), extra);
   return least;
 }
 

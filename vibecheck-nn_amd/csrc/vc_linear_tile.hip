@@ -1,4 +1,4 @@
-// The fc layer's large products: tiles of 64 x 64 to 256 x 256 (fp32 128 x 128), both operands as bf16
+// The fc layer's large products: tiles of 64 x 64 to 256 x 256 (fp32 256 x 128), both operands as bf16
 // (an fp32 value as three parts, vc_linear.hip) brought into LDS by loads that
 // pass no register.
 //
@@ -132,6 +132,24 @@ __device__ __forceinline__ void turn() {
   asm volatile("" ::: "memory");
 }
 
+// A value put together from its three parts; an infinity or NaN stands in the first.
+__device__ __forceinline__ float whole_value(const uint16_t* p, int64_t plane) {
+  const float h = bf_lo(p[0]);
+  return finite(h) ? (bf_lo(p[2 * plane]) + bf_lo(p[plane])) + h : h;
+}
+
+// The plain sum of the products k0 .. k1, where an infinity or NaN among the values
+// (or a sum past the largest) has made what the parts' products cannot say.
+template <bool XA, bool XB, class T>
+__device__ float plain_sum(const Product<T>& a, int64_t i, int64_t j, int64_t k0, int64_t k1) {
+  float s = 0.f;
+#pragma unroll 1
+  for (int64_t k = k0; k < k1 && s == s; ++k)  // NaN stays
+    s += whole_value(a.pa + (XA ? k * a.lda + i : i * a.lda + k), a.planeA) *
+         whole_value(a.pb + (XB ? k * a.ldb + j : j * a.ldb + k), a.planeB);
+  return s;
+}
+
 // NBUF: LDS buffers.  TURNS: the waves take turns, one for each 32 of k.
 template <class T, int NP, bool XA, bool XB, int BI, int BJ, int WI, int WJ, int BK, int NBUF,
           bool TURNS>
@@ -161,14 +179,11 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
   sa.init(a.pa, a.lda, XA ? (a.I + 7) & ~7 : a.I, i0, k0, wv, lane);
   sb.init(a.pb, a.ldb, XB ? (a.J + 7) & ~7 : a.J, j0, k0, wv, lane);
 
-  v4f acc[MI][MJ], small[NP == 3 ? MI : 1][NP == 3 ? MJ : 1];
+  v4f acc[MI][MJ];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < MJ; ++j) {
-      acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-      if (NP == 3) small[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int j = 0; j < MJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 
   // A step of an operand whose k is contiguous is 64 or 128 bytes of each of its
   // rows, and rows a power of two apart lie in one channel of the L2: with two such
@@ -206,16 +221,18 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
 #pragma unroll
         for (int j = 0; j < MJ; ++j) acc[i][j] = mfma_bf16(fb[j][0], fa[i][0], acc[i][j]);
       } else {
-        v4f z[MJ];  // the largest products, from zero
-#pragma unroll
-        for (int j = 0; j < MJ; ++j) z[j] = mfma_bf16(fb[j][0], fa[i][0], v4f{0.f, 0.f, 0.f, 0.f});
+        // from zero each step, the largest products apart; added in fp32
+        const v4f zero = v4f{0.f, 0.f, 0.f, 0.f};
+        v4f z[MJ], t[MJ];
 #pragma unroll
         for (int p = 0; p < 5; ++p)
 #pragma unroll
           for (int j = 0; j < MJ; ++j)
-            small[i][j] = mfma_bf16(fb[j][kPartA[p]], fa[i][kPartB[p]], small[i][j]);
+            t[j] = mfma_bf16(fb[j][kPartA[p]], fa[i][kPartB[p]], p ? t[j] : zero);
 #pragma unroll
-        for (int j = 0; j < MJ; ++j) acc[i][j] += z[j];
+        for (int j = 0; j < MJ; ++j) z[j] = mfma_bf16(fb[j][0], fa[i][0], zero);
+#pragma unroll
+        for (int j = 0; j < MJ; ++j) acc[i][j] += z[j] + t[j];
       }
     }
   };
@@ -311,16 +328,8 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < MJ; ++j) {
-          v4f v = acc[i][j];
-          if constexpr (NP == 3) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float t = v[q] + small[i][j][q];
-              v[q] = finite(t) ? t : v[q];
-            }
-          }
           const int row = ((ROWS == BI ? wi * MI : 0) + i) * 16 + r;
-          sums[row * Q + (((wj * MJ + j) * 4 + g) ^ (row & 15))] = v;
+          sums[row * Q + (((wj * MJ + j) * 4 + g) ^ (row & 15))] = acc[i][j];
         }
     }
     __syncthreads();
@@ -331,7 +340,13 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
       const int j = j0 + 4 * q;
       if (i >= a.I || j >= a.J) continue;
       const v4f w = sums[row * Q + (q ^ (row & 15))];
-      const float v[4] = {w[0], w[1], w[2], w[3]};
+      float v[4] = {w[0], w[1], w[2], w[3]};
+      if constexpr (NP == 3) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (!finite(v[k]) && j + k < a.J)
+            v[k] = plain_sum<XA, XB>(a, i, j + k, k0, k0 + left);
+      }
       deliver(a, slice, i, j, v);
     }
   }
@@ -341,15 +356,17 @@ template <class T, int SHAPE>
 struct Form {
   static constexpr bool F = sizeof(T) == 4;
   static constexpr int NP = F ? 3 : 1;
-  static constexpr int BI = (SHAPE == 0 ? 256 : SHAPE == 1 ? 128 : 64) / (F && SHAPE < 2 ? 2 : 1);
-  static constexpr int WI = 2, WJ = SHAPE == 0 ? 4 : 2;
+  static constexpr int BI = SHAPE == 0 ? 256 : SHAPE == 1 ? 128 : 64;
+  static constexpr int BJ = F && SHAPE == 0 ? 128 : BI;
+  static constexpr bool TURNS = SHAPE == 0 || (F && SHAPE == 1);
+  static constexpr int WI = F && SHAPE == 0 ? 4 : 2, WJ = (TURNS ? 8 : 4) / WI;
   static constexpr int BK = F ? 32 : 64;
-  static constexpr int NBUF = F && SHAPE == 0 ? 3 : 2;
+  static constexpr int NBUF = F && SHAPE == 1 ? 3 : 2;
   static constexpr int kThreads = 64 * WI * WJ;
-  static constexpr int kLds = NBUF * NP * 2 * BI * BK * 2;
+  static constexpr int kLds = NBUF * NP * (BI + BJ) * BK * 2;
   template <bool XA, bool XB>
   static __device__ __forceinline__ void run(const Product<T>& a, uint32_t block, char* lds) {
-    tile<T, NP, XA, XB, BI, BI, WI, WJ, BK, NBUF, SHAPE == 0>(a, block, lds);
+    tile<T, NP, XA, XB, BI, BJ, WI, WJ, BK, NBUF, TURNS>(a, block, lds);
   }
 };
 
@@ -402,23 +419,23 @@ void both(const Product<T>& w, const Product<T>& x, const Columns<T>& c, unsigne
 namespace vcl {
 
 TileShape tile_shape(int type, int shape) {
-  if (type == VC_FP32) return shape == 0 ? TileShape{128, 128, 32} : TileShape{64, 64, 32};
-  return shape == 0 ? TileShape{256, 256, 64}
-                    : shape == 1 ? TileShape{128, 128, 64} : TileShape{64, 64, 64};
+  const int bk = type == VC_FP32 ? 32 : 64;
+  if (shape == 0) return {256, type == VC_FP32 ? 128 : 256, bk};
+  return shape == 1 ? TileShape{128, 128, bk} : TileShape{64, 64, bk};
 }
 
 template <class T>
 void run_tile(const Product<T>& a, int shape, hipStream_t st) {
   if (shape == 0) one<T, 0>(a, st);
   else if (shape == 1) one<T, 1>(a, st);
-  else if constexpr (sizeof(T) == 2) one<T, 2>(a, st);
+  else one<T, 2>(a, st);
 }
 template <class T>
 void run_tiles(const Product<T>& w, const Product<T>& x, const Columns<T>& c, int shape,
                unsigned grid, hipStream_t st) {
   if (shape == 0) both<T, 0>(w, x, c, grid, st);
   else if (shape == 1) both<T, 1>(w, x, c, grid, st);
-  else if constexpr (sizeof(T) == 2) both<T, 2>(w, x, c, grid, st);
+  else both<T, 2>(w, x, c, grid, st);
 }
 template void run_tile<float>(const Product<float>&, int, hipStream_t);
 template void run_tile<uint16_t>(const Product<uint16_t>&, int, hipStream_t);

@@ -10,6 +10,7 @@
 // m)) + (m - z_t): nothing cancels where the target's probability is near one,
 // or where the logits are large beside their differences.
 #include <type_traits>
+#include <utility>
 
 #include "vc_common.h"
 
@@ -47,6 +48,7 @@ typedef uint32_t u4at2 __attribute__((ext_vector_type(4), aligned(2)));
 template <class T>
 struct Chunk {
   static constexpr int kN = 16 / sizeof(T);
+  static constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80u;  // -inf
   typedef std::conditional_t<sizeof(T) == 4, u4at4, u4at2> Any;
   static __device__ __forceinline__ u4 load(const T* p) { return *reinterpret_cast<const Any*>(p); }
   static __device__ __forceinline__ void store(T* p, u4 v) { *reinterpret_cast<Any*>(p) = v; }
@@ -68,16 +70,38 @@ struct Chunk {
     }
     return w;
   }
-  static __device__ __forceinline__ void set(u4& w, int i, uint32_t bits) {  // bits of a T
-#pragma unroll
-    for (int k = 0; k < kN; ++k) {
-      if (k != i) continue;
-      if constexpr (sizeof(T) == 4) w[k] = bits;
-      else w[k / 2] = k & 1 ? (w[k / 2] & 0xffffu) | bits << 16 : (w[k / 2] & 0xffff0000u) | bits;
+  static __device__ __forceinline__ u4 none_at(u4 w, int i) {  // -inf in place i
+    if constexpr (sizeof(T) == 4) {
+      return u4{i == 0 ? kNone : w[0], i == 1 ? kNone : w[1], i == 2 ? kNone : w[2],
+                i == 3 ? kNone : w[3]};
+    } else {
+      const uint32_t m = i & 1 ? 0xffffu : 0xffff0000u, v = i & 1 ? kNone << 16 : kNone;
+      return u4{i / 2 == 0 ? (w[0] & m) | v : w[0], i / 2 == 1 ? (w[1] & m) | v : w[1],
+                i / 2 == 2 ? (w[2] & m) | v : w[2], i / 2 == 3 ? (w[3] & m) | v : w[3]};
     }
   }
-  static constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80u;  // -inf
+  // The first n values dropped, -inf behind the others.
+  static __device__ __forceinline__ u4 drop(u4 w, int n) {
+    constexpr uint32_t f = sizeof(T) == 4 ? kNone : kNone | kNone << 16;
+    if constexpr (sizeof(T) == 4) {
+      w = n & 2 ? u4{w[2], w[3], f, f} : w;
+      w = n & 1 ? u4{w[1], w[2], w[3], f} : w;
+    } else {
+      w = n & 4 ? u4{w[2], w[3], f, f} : w;
+      w = n & 2 ? u4{w[1], w[2], w[3], f} : w;
+      w = n & 1 ? u4{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16,
+                     w[3] >> 16 | f << 16} : w;
+    }
+    return n >= kN ? u4{f, f, f, f} : w;
+  }
 };
+
+// f(0), f(1), .., each with a constant: an array indexed by them is in registers
+// from the start.
+template <class F, int... K>
+__device__ __forceinline__ void each(std::integer_sequence<int, K...>, F f) {
+  (f(std::integral_constant<int, K>{}), ...);
+}
 
 constexpr float kLog2e = 1.44269504088896341f;
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
@@ -174,8 +198,9 @@ __device__ void plain_row(const Rows& a, const T* z, T* dz, int64_t t, float zt,
   }
 }
 
-// A row is read once: its chunks stay in the team's registers, NV a thread, or
-// (NV 0, rows that do not fit) are read again for the gradient.
+// A row is read once: its chunks stay in the team's registers, NV a thread (the row
+// ends within the last ENDS of them), or (NV 0, rows that do not fit) are read again
+// for the gradient.
 //
 // While chunks arrive a thread keeps r, a whole number not below its largest
 // logit times log2 e, and the sum of 2^(z log2 e - r): one fma and one
@@ -185,7 +210,7 @@ __device__ void plain_row(const Rows& a, const T* z, T* dz, int64_t t, float zt,
 // apart (its place holds -inf meanwhile).
 //
 // 8,192 x 131,072 bf16: see the measured times at the entry point below.
-template <class T, int W, int NV, bool SMOOTH>
+template <class T, int W, int NV, int ENDS, bool SMOOTH>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
   typedef Chunk<T> C;
   typedef std::conditional_t<NV != 0, int, int64_t> Index;  // held rows: 32 bits beside the row's base
@@ -217,29 +242,36 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
     if constexpr (NV != 0) return p + (uint32_t)c * (uint32_t)N;
     else return (P*)p + c * N;
   };
+  // Every lane loads a whole chunk, one that would pass the row's end the row's
+  // last: a branch that lanes do not share would have each load waited for before
+  // the next.  What is not the chunk's own is masked when it is taken.
+  const Index last = (Index)(a.V - N);
   const auto fetch = [&](Index c) {
-    if (c < whole) return C::load(at(z, c));
-    u4 w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = sizeof(T) == 4 ? C::kNone : C::kNone | C::kNone << 16;
-    if (c == whole)
-      for (int64_t j = (int64_t)c * N; j < a.V; ++j) {
-        if constexpr (sizeof(T) == 4) C::set(w, (int)(j - (int64_t)c * N), __builtin_bit_cast(uint32_t, z[j]));
-        else C::set(w, (int)(j - (int64_t)c * N), z[j]);
-      }
-    return w;
+    const Index e = c < whole ? c * N : last;
+    if constexpr (NV != 0) return C::load(z + (uint32_t)e);
+    else return C::load(z + e);
+  };
+  // Of chunks first .. first + TH - 1, that of this lane: a part of one is moved to
+  // its front, the rest is -inf.
+  const auto mask = [&](u4 w, Index c, Index first) {
+    if (first + TH <= whole) return w;  // the same in all lanes
+    return C::drop(w, c < whole ? 0 : c == whole ? (int)((int64_t)c * N - last) : N);
   };
   float m = -INFINITY, r = -1e37f, s = 0.f, half = 0.f;
-  const auto take = [&](u4& w, Index c) {
+  const auto take = [&](u4 w, Index c, Index first, bool end) {
+    if (end) w = mask(w, c, first);
+    asm volatile("" : "+v"(w));  // one chunk's values at a time
     if (SMOOTH) {
-      if (c < whole) {
+      if (!end || first + TH <= whole) {
 #pragma unroll
         for (int i = 0; i < N; ++i) half += C::value(w, i) * iv;
-      } else if (c == whole) {
-        for (int64_t j = (int64_t)c * N; j < a.V; ++j) half += load1(z + j) * iv;
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) half += (int64_t)c * N + i < a.V ? C::value(w, i) * iv : 0.f;
       }
+      asm volatile("" : "+v"(half));
     }
-    if (c == ct) C::set(w, (int)(t - (int64_t)ct * N), C::kNone);
+    if (c == ct) w = C::none_at(w, (int)(t - (int64_t)ct * N));
     float top = C::value(w, 0);
 #pragma unroll
     for (int i = 1; i < N; ++i) top = fmaxf(top, C::value(w, i));
@@ -252,22 +284,20 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
       s += __builtin_amdgcn_exp2f(__builtin_fmaf(C::value(w, i), kLog2e, -r));
+    return w;
   };
   u4 v[NB];
+  constexpr std::make_integer_sequence<int, NB> held{};
   if (NV) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) v[k] = fetch(tid + k * TH);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      take(v[k], tid + k * TH);
+    each(held, [&](auto k) { v[k] = fetch(tid + k * TH); });
+    each(held, [&](auto k) {
+      v[k] = take(v[k], tid + k * TH, k * TH, k >= NV - ENDS);
       __builtin_amdgcn_sched_barrier(0);  // one chunk's floats at a time
-    }
+    });
   } else {
-    for (Index c = tid; c < chunks; c += NB * TH) {
-#pragma unroll
-      for (int k = 0; k < NB; ++k) v[k] = fetch(c + k * TH);
-#pragma unroll
-      for (int k = 0; k < NB; ++k) take(v[k], c + k * TH);
+    for (Index c = 0; c < chunks; c += NB * TH) {
+      each(held, [&](auto k) { v[k] = fetch(c + tid + k * TH); });
+      each(held, [&](auto k) { take(v[k], c + tid + k * TH, c + k * TH, true); });
     }
   }
   const float w = scale_of(a, lane);
@@ -286,7 +316,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
   if (!dz) return;
   const float inv = valid ? w / (s + et) : NAN, ev = a.smooth / (float)a.V * w;
   const float at_t = a.smooth * w - s * inv - ev;
-  const auto give = [&](u4 x, Index c) {
+  const auto give = [&](u4 x, Index c, bool end) {
     asm volatile("" : "+v"(x));  // unpacked again here, not kept from before: twice the registers
     float g[N];
 #pragma unroll
@@ -294,7 +324,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
       const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(C::value(x, i), kLog2e, -r));
       g[i] = SMOOTH ? __builtin_fmaf(p, inv, -ev) : p * inv;
     }
-    if (c < whole) {
+    if (!end || c < whole) {
       C::store(at(dz, c), C::pack(g));
     } else if (c == whole) {
 #pragma unroll
@@ -304,17 +334,18 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
     if (c == ct) store1(dz + t, at_t);
   };
   if (NV) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      give(v[k], tid + k * TH);
+    each(held, [&](auto k) {
+      give(v[k], tid + k * TH, k >= NV - ENDS);
       __builtin_amdgcn_sched_barrier(0);
-    }
+    });
   } else {
-    for (Index c = tid; c < chunks; c += NB * TH) {
-#pragma unroll
-      for (int k = 0; k < NB; ++k) v[k] = fetch(c + k * TH);
-#pragma unroll
-      for (int k = 0; k < NB; ++k) give(v[k], c + k * TH);
+    // dz may be z: a lane reads its chunk's own values before it writes them (what
+    // else a chunk at the row's end brings is masked)
+    for (Index c = 0; c < chunks; c += NB * TH) {
+      each(held, [&](auto k) { v[k] = fetch(c + tid + k * TH); });
+      each(held, [&](auto k) {
+        give(mask(v[k], c + tid + k * TH, c + k * TH), c + tid + k * TH, true);
+      });
     }
   }
 }
@@ -428,34 +459,41 @@ __global__ __launch_bounds__(1024) void k_loss_sum(const float* loss, int64_t R,
   }
 }
 
-template <class T, int W, int NV>
+template <class T, int W, int NV, int ENDS>
 void run_rows(const Rows& a, hipStream_t st) {
   const unsigned grid = (unsigned)(W == 1 ? (a.R + 3) / 4 : a.R);
   const int threads = W == 1 ? 256 : 64 * W;
-  if (a.smooth != 0.f) k_loss_rows<T, W, NV, true><<<grid, threads, 0, st>>>(a);
-  else k_loss_rows<T, W, NV, false><<<grid, threads, 0, st>>>(a);
+  if (a.smooth != 0.f) k_loss_rows<T, W, NV, ENDS, true><<<grid, threads, 0, st>>>(a);
+  else k_loss_rows<T, W, NV, ENDS, false><<<grid, threads, 0, st>>>(a);
 }
 
 constexpr int64_t kOneRows = 1024;    // of k_loss_few by one workgroup
 constexpr int64_t kCountRows = 1024;  // that every wave counts by itself
 
-// The team of a row: as many waves as hold it in at most 16 chunks a thread.
+// The team of a row: as many waves as hold it in at most 16 chunks a thread; the
+// row's end lies in the last chunks of a thread, those past the limit before.
 template <class T>
 void run_loss(const Rows& a, hipStream_t st) {
   const int64_t c = (a.V + Chunk<T>::kN - 1) / Chunk<T>::kN;
   if (a.V <= kFew) {
     if (a.R <= kOneRows) k_loss_few<T, kOneRows, true><<<1, kOneRows, 0, st>>>(a);
     else k_loss_few<T, 256, false><<<(unsigned)((a.R + 255) / 256), 256, 0, st>>>(a);
-  } else if (c <= 64) run_rows<T, 1, 1>(a, st);
-  else if (c <= 128) run_rows<T, 1, 2>(a, st);
-  else if (c <= 256) run_rows<T, 1, 4>(a, st);
-  else if (c <= 1024) run_rows<T, 4, 4>(a, st);
-  else if (c <= 2048) run_rows<T, 4, 8>(a, st);
-  else if (c <= 4096) run_rows<T, 8, 8>(a, st);
-  else if (c <= 8192) run_rows<T, 16, 8>(a, st);
-  else if (c <= 13312) run_rows<T, 16, 13>(a, st);
-  else if (c <= 16384) run_rows<T, 16, 16>(a, st);
-  else run_rows<T, 16, 0>(a, st);
+  } else if (c <= 64) run_rows<T, 1, 1, 1>(a, st);
+  else if (c <= 128) run_rows<T, 1, 2, 1>(a, st);
+  else if (c <= 256) run_rows<T, 1, 4, 2>(a, st);
+  else if (c <= 512) run_rows<T, 4, 2, 1>(a, st);
+  else if (c <= 768) run_rows<T, 4, 3, 1>(a, st);
+  else if (c <= 1024) run_rows<T, 4, 4, 1>(a, st);
+  else if (c <= 1536) run_rows<T, 4, 6, 2>(a, st);
+  else if (c <= 2048) run_rows<T, 4, 8, 2>(a, st);
+  else if (c <= 3072) run_rows<T, 16, 3, 1>(a, st);
+  else if (c <= 4096) run_rows<T, 16, 4, 1>(a, st);
+  else if (c <= 6144) run_rows<T, 16, 6, 2>(a, st);
+  else if (c <= 8192) run_rows<T, 16, 8, 2>(a, st);
+  else if (c <= 10240) run_rows<T, 16, 10, 2>(a, st);
+  else if (c <= 13312) run_rows<T, 16, 13, 3>(a, st);
+  else if (c <= 16384) run_rows<T, 16, 16, 3>(a, st);
+  else run_rows<T, 16, 0, 0>(a, st);
 }
 
 }  // namespace
