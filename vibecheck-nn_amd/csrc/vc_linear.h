@@ -136,6 +136,9 @@ struct Columns {
   T* db;
 };
 
+// The forward's product of fp32 rows as they are: bases, lds and K multiples of 16
+// bytes, 64 rows within 2^31.
+void run_raw(const Product<float>& a, hipStream_t st);
 // The forward's product.
 template <class T>
 void run_tile(const Product<T>& a, int shape, hipStream_t st);

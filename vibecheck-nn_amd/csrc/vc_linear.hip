@@ -619,7 +619,7 @@ constexpr int64_t kCus = 256;
 
 // How a product is cut: the kernel, its shape, and the slices of k, by the time
 // that they are expected to take (us).
-enum Kernel { kProduct, kDirect, kTile };
+enum Kernel { kProduct, kDirect, kTile, kRaw };
 struct Cut {
   Kernel kernel;
   int shape, slices, steps;
@@ -825,13 +825,22 @@ struct ForwardPlan {
   int64_t x, W, part, bytes;  // offsets in the workspace, and its size
 };
 
-ForwardPlan plan_forward(int type, int64_t M, int K, int N) {
+// raw: fp32 rows that the loads into LDS can take as they are.
+ForwardPlan plan_forward(int type, int64_t M, int K, int N, bool raw) {
   ForwardPlan p;
   const Job job = {M, N, K};
   const float pack = type == VC_FP32 || K % 8 ? pack_us(type, (M + N) * K) : 0.f;
   choose(type, &job, 1, tile_lines(K), pack, &p.c);
   const Cut d = cut_direct(type, M, N, K);
   if (d.us < p.c.us) p.c = d;
+  if (raw) {
+    // two steps of 32 alone on a CU, and of each of two that share one (512 x 784 x
+    // 1024)
+    const Cost c = {64, 32, 64, 2, 0.55f, 0.5f};
+    Grid g;
+    const float us = best_slices(type, c, &job, 1, &g);
+    if (us < p.c.us) p.c = {kRaw, 0, (int)g.slices, (int)g.steps * 2, g.tiles, g.nj, us};
+  }
   const bool tiles = p.c.kernel == kTile;
   p.x = 0;
   p.W = tiles ? parts_bytes(type, M, K) : 0;
@@ -845,7 +854,9 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
             int act, const void* res, int64_t ldr, void* y, void* z, void* work,
             int64_t work_bytes, hipStream_t st) {
   constexpr int type = sizeof(T) == 4 ? VC_FP32 : VC_BF16;
-  const ForwardPlan p = plan_forward(type, M, K, N);
+  const bool raw = type == VC_FP32 && K % 4 == 0 && K > 0 && ldx % 4 == 0 && aligned16(x) &&
+                   aligned16(W) && K < (1 << 21) && ldx < (1 << 21);
+  const ForwardPlan p = plan_forward(type, M, K, N, raw);
   if (p.bytes > work_bytes || (p.bytes && !work)) return VC_ERR_OOM;
   char* const base = (char*)work;
   Product<T> a = {};
@@ -880,8 +891,11 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
   const dim3 grid((unsigned)p.c.tiles, (unsigned)p.c.slices);
   const unsigned flat = (unsigned)(p.c.tiles * p.c.slices);
   constexpr int G = F ? kGroups32 : kGroups16, threads = 64 * kDirectWaves;
-  if (p.c.kernel == kTile) run_tile<T>(a, p.c.shape, st);
-  else if (p.c.kernel == kProduct && p.c.shape == 0) k_product<T, 1><<<flat, LNT, 0, st>>>(a);
+  if (p.c.kernel == kTile) {
+    run_tile<T>(a, p.c.shape, st);
+  } else if (p.c.kernel == kRaw) {
+    if constexpr (F) run_raw(a, st);
+  } else if (p.c.kernel == kProduct && p.c.shape == 0) k_product<T, 1><<<flat, LNT, 0, st>>>(a);
   else if (p.c.kernel == kProduct) k_product<T, G><<<flat, LNT * G, 0, st>>>(a);
   else if (p.c.shape == 0) k_direct<T, 1, 1, F ? 2 : 8><<<grid, threads, 0, st>>>(a);
   else if (p.c.shape == 1) k_direct<T, 1, 2, F ? 2 : 4><<<grid, threads, 0, st>>>(a);
@@ -1035,7 +1049,9 @@ bool known(int type, int act) {
 extern "C" int64_t vc_linear_workspace(int type, int64_t M, int K, int N) {
   if (!known(type, kNone) || !sizes_ok(M, K, N)) return -1;
   if (M == 0 || N == 0) return 0;
-  return plan_forward(type, M, K, N).bytes;
+  const int64_t a = plan_forward(type, M, K, N, false).bytes;
+  const int64_t b = plan_forward(type, M, K, N, type == VC_FP32).bytes;
+  return a > b ? a : b;
 }
 
 extern "C" int vc_linear(int type, const void* x, int64_t M, int K, int64_t ldx, const void* W,

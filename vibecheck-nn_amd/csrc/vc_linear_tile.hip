@@ -387,6 +387,103 @@ __global__ __launch_bounds__((Form<T, SHAPE>::kThreads), 2) void k_tiles(Product
   else add_columns(c, (int)(b - nw - nx), reinterpret_cast<float*>(lds));
 }
 
+// fp32 forward products too small for the parts' pass: 64 x 32 tiles straight from
+// x and W, on the fp32 matrix steps.  A row's 32 values of a step are 128 bytes, as
+// 64 of bf16 are: the same loads and order of LDS.  A lane's 16 bytes are four k;
+// matrix step q takes the q-th of every lane, the columns' operand alike.  Two
+// groups of four waves take the steps in turn, each with three buffers of its own,
+// and add their sums.
+constexpr int kRawI = 64, kRawJ = 32, kRawBuf = 3;
+
+__global__ __launch_bounds__(512, 2) void k_raw(Product<float> a) {
+  typedef Side<false, kRawI, 64, 4> SA;
+  typedef Side<false, kRawJ, 64, 4> SB;
+  constexpr int kStage = SA::kBytes + SB::kBytes, kLoads = SA::kOwn + SB::kOwn, AHEAD = kRawBuf - 1;
+  constexpr int Q = kRawJ / 4;
+  __shared__ __align__(1024) char all[2 * kRawBuf * kStage];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
+  const int grp = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int slice = __builtin_amdgcn_readfirstlane(blockIdx.x / (uint32_t)a.tiles);
+  const uint32_t w = (uint32_t)vcg::xcd_tile(blockIdx.x - slice * (uint32_t)a.tiles, a.tiles);
+  const int ti = __builtin_amdgcn_readfirstlane(a.f_nj.div(w));
+  const int i0 = ti * kRawI, j0 = ((int)w - ti * (int)a.f_nj.d) * kRawJ;
+  const int k0 = slice * a.steps * 32, left = min(a.steps * 32, a.K - k0);
+  const int steps = (left + 31) / 32, full = left / 32;
+  const int wi = wv >> 1, wj = wv & 1, g = lane >> 4, r = lane & 15;
+  char* const lds = all + grp * kRawBuf * kStage;
+  SA sa;
+  SB sb;
+  // lengths and strides in bf16's: two to a value
+  sa.init(reinterpret_cast<const uint16_t*>(a.A.p), 2 * a.A.ld, a.I, i0, 2 * (int64_t)k0, wv, lane);
+  sb.init(reinterpret_cast<const uint16_t*>(a.B.p), 2 * a.B.ld, a.J, j0, 2 * (int64_t)k0, wv, lane);
+  const auto load = [&](int s, int buf) {
+    char* const to = lds + buf * kStage;
+    if (s < full) {
+      sa.issue(sa.base + s * 64, to, wv);
+      sb.issue(sb.base + s * 64, to + SA::kBytes, wv);
+    } else {
+      sa.tail(sa.base + s * 64, to, wv, lane, 2 * (left - full * 32));
+      sb.tail(sb.base + s * 64, to + SA::kBytes, wv, lane, 2 * (left - full * 32));
+    }
+  };
+  v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+  // the group's own steps: grp, grp + 2, ..; both groups pass as many barriers
+  const int turns = (steps + 1) / 2;
+#pragma unroll
+  for (int t = 0; t < AHEAD; ++t)
+    if (2 * t + grp < steps) load(2 * t + grp, t);
+  int at = 0;
+#pragma unroll 1
+  for (int t = 0; t < turns; ++t) {
+    // in flight beyond this step: the next one, when it is a whole one
+    if (2 * (t + 1) + grp < full) wait_for<kLoads, true>();
+    else wait_for<0, true>();
+    turn();
+    const int before = at == 0 ? kRawBuf - 1 : at - 1;
+    if (2 * (t + AHEAD) + grp < steps) load(2 * (t + AHEAD) + grp, before);
+    if (2 * t + grp < steps) {
+      const char* const from = lds + at * kStage;
+      v4f fa[2][2], fb[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = ((4 * h + g) ^ (r & 7)) * 16;
+        fb[h] = *reinterpret_cast<const v4f*>(from + SA::kBytes + (wj * 16 + r) * 128 + c);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          fa[i][h] = *reinterpret_cast<const v4f*>(from + (wi * 32 + i * 16 + r) * 128 + c);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) acc[i] = mfma16x16x4(fb[h][q], fa[i][h][q], acc[i]);
+    }
+    at = at == kRawBuf - 1 ? 0 : at + 1;
+  }
+  // row, four columns c: at c ^ (row mod 8)
+  v4f* const sums = reinterpret_cast<v4f*>(all);
+  __syncthreads();
+#pragma unroll
+  for (int k = 1; k >= 0; --k) {
+    if (grp == k) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = wi * 32 + i * 16 + r;
+        v4f& s = sums[row * Q + ((wj * 4 + g) ^ (row & 7))];
+        s = k ? acc[i] : s + acc[i];
+      }
+    }
+    __syncthreads();
+  }
+  const int row = tid / Q, q = tid % Q, j = j0 + 4 * q;
+  if (i0 + row >= a.I || j >= a.J) return;
+  const v4f s = sums[row * Q + (q ^ (row & 7))];
+  const float v[4] = {s[0], s[1], s[2], s[3]};
+  deliver(a, slice, i0 + row, j, v);
+}
+
 // A kernel's LDS limit, set once per device.
 template <class K>
 void allow_lds(K k, int bytes, bool* set) {
@@ -422,6 +519,10 @@ TileShape tile_shape(int type, int shape) {
   const int bk = type == VC_FP32 ? 32 : 64;
   if (shape == 0) return {256, type == VC_FP32 ? 128 : 256, bk};
   return shape == 1 ? TileShape{128, 128, bk} : TileShape{64, 64, bk};
+}
+
+void run_raw(const Product<float>& a, hipStream_t st) {
+  k_raw<<<(unsigned)(a.tiles * a.slices), 512, 0, st>>>(a);
 }
 
 template <class T>
