@@ -215,24 +215,29 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
         fa[i][p] = SA::frag(from + p * SA::kBytes, (wi * MI + i) * 16, ks, lane);
   };
   const auto multiply = [&]() {
+    if constexpr (NP == 1) {
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      if constexpr (NP == 1) {
+      for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < MJ; ++j) acc[i][j] = mfma_bf16(fb[j][0], fa[i][0], acc[i][j]);
-      } else {
-        // from zero each step, the largest products apart; added in fp32
-        const v4f zero = v4f{0.f, 0.f, 0.f, 0.f};
-        v4f z[MJ], t[MJ];
+    } else {
+      // a step's six products from zero, smallest first, added in fp32 while the
+      // next rows' run
+      v4f t[2][MJ];
 #pragma unroll
-        for (int p = 0; p < 5; ++p)
+      for (int i = 0; i <= MI; ++i) {
+        if (i < MI) {
 #pragma unroll
-          for (int j = 0; j < MJ; ++j)
-            t[j] = mfma_bf16(fb[j][kPartA[p]], fa[i][kPartB[p]], p ? t[j] : zero);
+          for (int p = 0; p < 6; ++p)
 #pragma unroll
-        for (int j = 0; j < MJ; ++j) z[j] = mfma_bf16(fb[j][0], fa[i][0], zero);
+            for (int j = 0; j < MJ; ++j)
+              t[i & 1][j] = mfma_bf16(fb[j][kPartA[p]], fa[i][kPartB[p]],
+                                      p ? t[i & 1][j] : v4f{0.f, 0.f, 0.f, 0.f});
+        }
+        if (i > 0) {
 #pragma unroll
-        for (int j = 0; j < MJ; ++j) acc[i][j] += z[j] + t[j];
+          for (int j = 0; j < MJ; ++j) acc[i - 1][j] += t[(i - 1) & 1][j];
+        }
       }
     }
   };
