@@ -59,6 +59,15 @@ def _rows(t):
     return t, t.stride(0)
 
 
+def _lead(t, n):
+    """Rows of t's last axis, and t's shape with n in place of it."""
+    if t.dim() == 2:
+        M = t.shape[0]
+        return M, (M, n)
+    lead = tuple(t.shape[:-1])
+    return math.prod(lead), lead + (n,)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -96,7 +105,7 @@ def _linear(x, W, bias, act, residual, save):
         raise ValueError('vibecheck_amd: x has at least one axis, W two')
     N, K = W.shape
     _like(W, x, (N, x.shape[-1]), 'W')
-    shape = (*x.shape[:-1], N)
+    M, shape = _lead(x, N)
     if bias is not None:
         _like(bias, x, (N,), 'bias')
         bias = bias.contiguous()
@@ -104,7 +113,6 @@ def _linear(x, W, bias, act, residual, save):
         _like(residual, x, shape, 'residual')
     x, ldx = _rows(x)
     W = W.contiguous()
-    M = math.prod(shape[:-1])
     y = x.new_empty(shape)
     # the sign of relu's output is its input's; another activation's input is kept
     z = torch.empty_like(y) if save and act and (act != 1 or residual is not None) else None
@@ -143,14 +151,18 @@ def linear(x, W, bias=None, act=None, residual=None, save=False):
     for relu without a residual it is y itself).  Differentiable through autograd for inputs
     that require it; the saved tensors are then the node's own."""
     a = _act(act)
-    if not save and torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, W, bias, residual)):
+    if not save and torch.is_grad_enabled() and (
+            x.requires_grad or W.requires_grad or bias is not None and bias.requires_grad or
+            residual is not None and residual.requires_grad):
         return _Linear.apply(x, W, bias, a, residual)
     y, z = _linear(x, W, bias, a, residual, save)
     return (y, z) if save else y
 
 
-def linear_backward(dy, x, W, z=None, act=None, need=('x', 'W', 'bias')):
+_ALL = ('x', 'W', 'bias')
+
+
+def linear_backward(dy, x, W, z=None, act=None, need=_ALL):
     """(dx, dW, db) of y = act(x W^T + bias) from dy (..., N): dz = dy act'(z), dx = dz W,
     dW = dz^T x, db the sum of dz over rows; None for what ``need`` does not name.  ``z`` is
     what linear(save=True) returned.  The residual's gradient is dy."""
@@ -158,12 +170,12 @@ def linear_backward(dy, x, W, z=None, act=None, need=('x', 'W', 'bias')):
     k = _type(dy, 'dy')
     if W.dim() != 2 or dy.dim() < 1:
         raise ValueError('vibecheck_amd: dy has at least one axis, W two')
-    if not set(need) <= {'x', 'W', 'bias'}:
+    if need is not _ALL and not set(need) <= set(_ALL):
         raise ValueError(f"vibecheck_amd: need names {need!r}; 'x', 'W' and 'bias' are taken")
     N, K = W.shape
     _like(W, dy, (dy.shape[-1], K), 'W')
-    lead = tuple(dy.shape[:-1])
-    _like(x, dy, lead + (K,), 'x')
+    M, of_x = _lead(dy, K)
+    _like(x, dy, of_x, 'x')
     if a:
         if z is None:
             raise ValueError('vibecheck_amd: an activation needs z')
@@ -171,8 +183,7 @@ def linear_backward(dy, x, W, z=None, act=None, need=('x', 'W', 'bias')):
         z, ldz = _rows(z)
     else:
         z, ldz = None, 0
-    M = math.prod(lead)
-    dx = dy.new_empty(lead + (K,)) if 'x' in need else None
+    dx = dy.new_empty(of_x) if 'x' in need else None
     dW = dy.new_empty((N, K)) if 'W' in need else None
     # no row adds to it, no launch writes it
     db = (dy.new_empty if M else dy.new_zeros)(N) if 'bias' in need else None
@@ -215,7 +226,7 @@ def _cross_entropy(logits, target, reduction, ignore_index, smoothing, grad, out
         raise ValueError(f'vibecheck_amd: target is {target.dtype} {tuple(target.shape)} on '
                          f'{target.device}, expected int64 {tuple(lead)} on {logits.device}')
     R, kind = lead.numel(), REDUCTIONS[reduction]
-    loss = torch.empty(lead if kind == 0 else (), dtype=torch.float32, device=logits.device)
+    loss = logits.new_empty(lead if kind == 0 else (), dtype=torch.float32)
     if out is not None:
         _like(out, logits, logits.shape, 'out')
         if not out.is_contiguous():
@@ -290,8 +301,9 @@ _dtype_of = operator.attrgetter('dtype')
 
 def _one_type(tensors, sizes, what):
     """Type number and pointers of a list of contiguous GPU tensors of one type."""
-    k = _type(tensors[0], what)
-    if len(set(map(_dtype_of, tensors))) > 1 or len(set(map(_device_of, tensors))) > 1 or \
+    k, n = _type(tensors[0], what), len(tensors)
+    if list(map(_dtype_of, tensors)).count(tensors[0].dtype) != n or \
+            list(map(_device_of, tensors)).count(tensors[0].get_device()) != n or \
             list(map(_numel, tensors)) != sizes or not all(map(_contiguous, tensors)):
         raise ValueError(f'vibecheck_amd: {what} are contiguous, of one type, on one device and '
                          f'of their parameters\' sizes {sizes}; got '
@@ -319,7 +331,7 @@ def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8
     kp, pp = _one_type(params, sizes, 'params')
     kg, pg = _one_type(grads, sizes, 'grads')
     dev = params[0].get_device()  # the current one, as the gradients' and copies' is
-    n, cnt = sum((k + BLOCK - 1) // BLOCK for k in sizes), len(sizes)
+    n, cnt = sum([(k + BLOCK - 1) // BLOCK for k in sizes]), len(sizes)
     bits = state['bits']
     keys = ('m', 'v') if bits == 32 else ('m', 'v', 'm_scale', 'v_scale')
     for key in keys:
