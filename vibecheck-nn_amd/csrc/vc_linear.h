@@ -1,6 +1,8 @@
 // The fc layer's kernels share this: types, activations, what a product is and how
 // its sums are finished (bias, activation, residual, rounding, stores).
 #pragma once
+#include <type_traits>
+
 #include "vc_gemm_core.h"
 #include "vc_split.h"
 
@@ -14,6 +16,8 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4at4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u4at2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u2at4 __attribute__((ext_vector_type(2), aligned(4)));
+typedef uint32_t u2at2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef float v4fat4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u1at2 __attribute__((aligned(2)));
 
 // Sixteen bytes at any alignment of the type.
@@ -104,11 +108,11 @@ struct Product {
   Operand<T> A, B;
   int I, J, K;
   int slices, steps;  // steps of a slice
-  float* part;        // slices > 1: (slices, I, J)
+  float* part;        // slices > 1: (slices, I, part_line(J))
   const T *bias, *res;
   int64_t ldr;
   T *out, *z;
-  int act, wide;      // wide: four columns of out, z, res and bias by one access
+  int act;
   int64_t tiles;
   vcg::FastDiv f_nj;
   // as bf16 parts (an fp32 value is three): plane p of an operand starts p planes
@@ -147,87 +151,107 @@ template <class T>
 void run_tiles(const Product<T>& w, const Product<T>& x, const Columns<T>& c, int shape,
                unsigned grid, hipStream_t st);
 
-// Four columns j .. j + 3 of row i: bias, activation, residual, stores.
+// A line of a slice's sums.
+__host__ __device__ __forceinline__ int part_line(int J) { return (J + 3) & ~3; }
+
+// Four values at any alignment of the type.
+__device__ __forceinline__ v4f load4(const float* p) { return *reinterpret_cast<const v4fat4*>(p); }
+__device__ __forceinline__ v4f load4(const uint16_t* p) {
+  const u2 w = *reinterpret_cast<const u2at2*>(p);
+  return v4f{bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y)};
+}
+__device__ __forceinline__ void store4(float* p, const v4f& v) { *reinterpret_cast<v4fat4*>(p) = v; }
+__device__ __forceinline__ void store4(uint16_t* p, const v4f& v) {
+  *reinterpret_cast<u2at2*>(p) = u2{bf_pack(v[0], v[1]), bf_pack(v[2], v[3])};
+}
+
+// Columns j .. j + 3 (all within J) of rows i, i + step, .. as far as they go: bias,
+// activation, residual, stores.  Every row's loads come before the first that is
+// worked on, one branch chooses the activation of all.  bias: zeros where there is
+// none.
+template <class T, int U>
+__device__ __forceinline__ void finish_rows(const Product<T>& a, int i, int step, int j,
+                                            const v4f& bias, const v4f (&s)[U]) {
+  v4f z[U], v[U], r[U];
+  if (a.res) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) r[u] = load4(a.res + min(i + u * step, a.I - 1) * a.ldr + j);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) v[u] = z[u] = a.bias ? s[u] + bias : s[u];
+  const auto each = [&](auto act) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[u][q] = activate(z[u][q], act);
+  };
+  if (a.act == kRelu) each(std::integral_constant<int, kRelu>{});
+  else if (a.act == kGelu) each(std::integral_constant<int, kGelu>{});
+  else if (a.act == kSilu) each(std::integral_constant<int, kSilu>{});
+  if (a.res) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] += r[u];
+  }
+  const int64_t o = (int64_t)i * a.J + j;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (i + u * step >= a.I) continue;
+    store4(a.out + o + (int64_t)u * step * a.J, v[u]);
+    if (a.z) store4(a.z + o + (int64_t)u * step * a.J, z[u]);
+  }
+}
+
 template <class T>
-__device__ __forceinline__ void finish(const Product<T>& a, int64_t i, int j, const float* s) {
-  const int n = min(4, a.J - j);
-  float v[4], b[4] = {0.f, 0.f, 0.f, 0.f}, r[4] = {0.f, 0.f, 0.f, 0.f};
-  T* const o = a.out + i * a.J + j;
-  if (a.wide) {  // J a multiple of four
-    if (a.bias) {
+__device__ __forceinline__ v4f bias_of(const Product<T>& a, int j) {
+  v4f b = v4f{0.f, 0.f, 0.f, 0.f};
+  if (a.bias) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) b[q] = get(a.bias + j + q);
-    }
-    if (a.res) {
-      const T* const p = a.res + i * a.ldr + j;
-      if constexpr (sizeof(T) == 4) {
-        const v4f w = *reinterpret_cast<const v4f*>(p);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) r[q] = w[q];
-      } else {
-        const u2 w = *reinterpret_cast<const u2*>(p);
-        r[0] = bf_lo(w.x), r[1] = bf_hi(w.x), r[2] = bf_lo(w.y), r[3] = bf_hi(w.y);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (q >= n) continue;
-      if (a.bias) b[q] = get(a.bias + j + q);
-      if (a.res) r[q] = get(a.res + i * a.ldr + j + q);
-    }
+    for (int q = 0; q < 4; ++q) b[q] = get(a.bias + min(j + q, a.J - 1));
   }
-  float z[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    z[q] = a.bias ? s[q] + b[q] : s[q];
-    v[q] = activate(z[q], a.act);
-    if (a.res) v[q] += r[q];
-  }
-  if (a.wide) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<v4f*>(o) = v4f{v[0], v[1], v[2], v[3]};
-      if (a.z) *reinterpret_cast<v4f*>(a.z + i * a.J + j) = v4f{z[0], z[1], z[2], z[3]};
-    } else {
-      *reinterpret_cast<u2*>(o) = u2{bf_pack(v[0], v[1]), bf_pack(v[2], v[3])};
-      if (a.z)
-        *reinterpret_cast<u2*>(a.z + i * a.J + j) = u2{bf_pack(z[0], z[1]), bf_pack(z[2], z[3])};
-    }
+  return b;
+}
+
+// Four columns j .. j + 3 of row i, the last of them past J perhaps.
+template <class T>
+__device__ __forceinline__ void finish(const Product<T>& a, int i, int j, const v4f& s) {
+  if (j + 4 <= a.J) {
+    const v4f one[1] = {s};
+    finish_rows<T, 1>(a, i, 0, j, bias_of(a, j), one);
     return;
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    if (q >= n) continue;
-    put(o + q, v[q]);
-    if (a.z) put(a.z + i * a.J + j + q, z[q]);
+    if (j + q >= a.J) continue;
+    const int64_t o = (int64_t)i * a.J + j + q;
+    const float z = a.bias ? s[q] + get(a.bias + j + q) : s[q];
+    float v = activate(z, a.act);
+    if (a.res) v += get(a.res + i * a.ldr + j + q);
+    put(a.out + o, v);
+    if (a.z) put(a.z + o, z);
   }
 }
 
 // Four columns of row i of a slice: finished, or left for the join.
 template <class T>
-__device__ __forceinline__ void deliver(const Product<T>& a, int64_t slice, int64_t i, int j,
-                                        const float* v) {
-  if (a.slices == 1) {
-    finish(a, i, j, v);
-    return;
-  }
-  float* const o = a.part + (slice * a.I + i) * a.J + j;
-  if (a.J % 4 == 0) {
-    *reinterpret_cast<v4f*>(o) = v4f{v[0], v[1], v[2], v[3]};
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (j + q < a.J) o[q] = v[q];
-  }
+__device__ __forceinline__ void deliver(const Product<T>& a, int64_t slice, int i, int j,
+                                        const v4f& s) {
+  if (a.slices == 1) finish(a, i, j, s);
+  else *reinterpret_cast<v4f*>(a.part + (slice * a.I + i) * part_line(a.J) + j) = s;
 }
 
 // lds: 32 floats for every 32 threads.
 template <class T>
 __device__ __forceinline__ void add_columns(const Columns<T>& a, int block, float* lds) {
   const int c = threadIdx.x & 31, y = threadIdx.x >> 5, ny = blockDim.x >> 5, j = block * 32 + c;
+  const float* const p = a.sums + min(j, a.N - 1);
   float s = 0.f;
-  if (j < a.N)
-    for (int b = y; b < a.blocks; b += ny) s += a.sums[(int64_t)b * a.N + j];
+  for (int b = y; b < a.blocks; b += 8 * ny) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = p[(int64_t)min(b + u * ny, a.blocks - 1) * a.N];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += b + u * ny < a.blocks ? v[u] : 0.f;
+  }
   lds[y * 32 + c] = s;
   __syncthreads();
   if (y || j >= a.N) return;

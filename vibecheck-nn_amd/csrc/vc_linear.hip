@@ -312,8 +312,7 @@ __device__ __forceinline__ void product_tile(const Product<T>& a, uint32_t block
     for (int j = 0; j < M2; ++j) {
       const int col = j0 + (wj * M2 + j) * 16 + 4 * g;
       if (col >= a.J) continue;
-      const float v[4] = {sum[i][j][0], sum[i][j][1], sum[i][j][2], sum[i][j][3]};
-      deliver(a, slice, row, col, v);
+      deliver(a, slice, row, col, sum[i][j]);
     }
   }
 }
@@ -442,47 +441,42 @@ __global__ __launch_bounds__(64 * kDirectWaves, 2) void k_direct(Product<T> a) {
     v4f s = part[0][b][lane];
 #pragma unroll
     for (int k = 1; k < NW; ++k) s += part[k][b][lane];
-    const int64_t row = i0 + 16 * (b / NB) + r;
-    const int col = j0 + 16 * (b % NB) + 4 * g;
-    if (row >= a.I || col >= a.J) continue;
-    const float v[4] = {s[0], s[1], s[2], s[3]};
-    deliver(a, blockIdx.y, row, col, v);
+    const int row = i0 + 16 * (b / NB) + r, col = j0 + 16 * (b % NB) + 4 * g;
+    if (row < a.I && col < a.J) deliver(a, blockIdx.y, row, col, s);
   }
 }
 
-// The slices' sums joined in their order, of up to two products.
+// The slices' sums joined in their order, of up to two products; eight slices' (or
+// four, or two) loads before the first is added, the last again past the last.
 template <class T>
-__device__ __forceinline__ void join_quad(const Product<T>& a, int64_t t, int nq) {
-  const int64_t i = t / nq;
-  const int j = (int)(t - i * nq) * 4;
-  float v[4] = {-0.f, -0.f, -0.f, -0.f};  // adds nothing, not even a sign
-  const int64_t step = (int64_t)a.I * a.J;
-  const float* p = a.part + (int64_t)i * a.J + j;
-  if (a.J % 4 == 0) {
-#pragma unroll 8
-    for (int s = 0; s < a.slices; ++s, p += step) {
-      const v4f w = *reinterpret_cast<const v4f*>(p);
+__device__ __forceinline__ void join_quad(const Product<T>& a, uint32_t t, vcg::FastDiv line) {
+  const int i = (int)line.div(t), j = (int)(t - i * line.d) * 4;
+  const int64_t step = (int64_t)a.I * part_line(a.J);
+  const float* const p = a.part + (int64_t)t * 4;
+  v4f v = v4f{-0.f, -0.f, -0.f, -0.f};  // adds nothing, not even a sign
+  const auto some = [&](int s, auto count) {
+    constexpr int N = decltype(count)::value;
+    v4f w[N];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] += w[q];
-    }
-  } else {
-#pragma unroll 4
-    for (int s = 0; s < a.slices; ++s, p += step)
+    for (int u = 0; u < N; ++u)
+      w[u] = *reinterpret_cast<const v4f*>(p + min(s + u, a.slices - 1) * step);
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (j + q < a.J) v[q] += p[q];
-  }
+    for (int u = 0; u < N; ++u)
+      if (s + u < a.slices) v += w[u];
+  };
+  if (a.slices == 2) some(0, std::integral_constant<int, 2>{});
+  else if (a.slices <= 4) some(0, std::integral_constant<int, 4>{});
+  else
+    for (int s = 0; s < a.slices; s += 8) some(s, std::integral_constant<int, 8>{});
   finish(a, i, j, v);
 }
 
 template <class T>
-__global__ __launch_bounds__(LNT) void k_join(Product<T> a, Product<T> b) {
-  const int qa = (a.J + 3) / 4, qb = (b.J + 3) / 4;
-  const int64_t na = a.slices > 1 ? (int64_t)a.I * qa : 0, nb = b.slices > 1 ? (int64_t)b.I * qb : 0;
-  for (int64_t t = blockIdx.x * (int64_t)LNT + threadIdx.x; t < na + nb; t += (int64_t)gridDim.x * LNT) {
-    if (t < na) join_quad(a, t, qa);
-    else join_quad(b, t - na, qb);
-  }
+__global__ __launch_bounds__(LNT) void k_join(Product<T> a, uint32_t na, vcg::FastDiv la,
+                                              Product<T> b, uint32_t nb, vcg::FastDiv lb) {
+  const uint32_t t = blockIdx.x * LNT + threadIdx.x;
+  if (t < na) join_quad(a, t, la);
+  else if (t - na < nb) join_quad(b, t - na, lb);
 }
 
 // Eight values j .. j + 7 of a row of n, as floats; past the end zero.
@@ -563,31 +557,38 @@ __device__ __forceinline__ void slope_block(const Slope<T>& a, int bx, int by) {
   const int64_t m0 = (int64_t)by * a.rows;
   const int64_t m1 = m0 + a.rows < a.M ? m0 + a.rows : a.M;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  // R rows of this thread's: all their loads before the first is used
+  const auto take = [&](int64_t m, auto count) {
+    constexpr int R = decltype(count)::value;
+    float d[R][8], z[R][8];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const int64_t r = m + 8 * q < m1 ? m + 8 * q : m;
+      load8(a.dy + r * a.ldy, j, a.N, whole, d[q]);
+      if (a.act != kNone) load8(a.z + r * a.ldz, j, a.N, whole, z[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const int64_t r = m + 8 * q;
+      if (r >= m1) break;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (a.act != kNone) d[q][i] *= slope(z[q][i], a.act);
+        sum[i] += d[q][i];
+      }
+      if (a.parts) store_parts<T>(d[q], a.parts + r * a.np + j, a.M * a.np);
+      if (a.dz) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (j + i < a.N) put(a.dz + r * a.N + j + i, d[q][i]);
+      }
+    }
+  };
   if (j < a.N) {
-    for (int64_t m = m0 + y; m < m1; m += 32) {  // four rows' loads before the first is used
-      float d[4][8], z[4][8];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t r = m + 8 * q < m1 ? m + 8 * q : m;
-        load8(a.dy + r * a.ldy, j, a.N, whole, d[q]);
-        if (a.act != kNone) load8(a.z + r * a.ldz, j, a.N, whole, z[q]);
-      }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t r = m + 8 * q;
-        if (r >= m1) break;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (a.act != kNone) d[q][i] *= slope(z[q][i], a.act);
-          sum[i] += d[q][i];
-        }
-        if (a.parts) store_parts<T>(d[q], a.parts + r * a.np + j, a.M * a.np);
-        if (a.dz) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (j + i < a.N) put(a.dz + r * a.N + j + i, d[q][i]);
-        }
-      }
+    if (a.rows <= 8) {
+      if (m0 + y < m1) take(m0 + y, std::integral_constant<int, 1>{});
+    } else {
+      for (int64_t m = m0 + y; m < m1; m += 32) take(m, std::integral_constant<int, 4>{});
     }
   }
   if (!a.sums) return;
@@ -649,10 +650,10 @@ Grid grid_of(int64_t I, int64_t J, int64_t K, int bi, int bj, int bk, int64_t wa
 }
 
 // What a kernel's tiles cost: `alone` us a step for as many workgroups as share a
-// CU, `shared` us for each of them.
+// CU, `shared` us for each of them, `end` us for a tile's output.
 struct Cost {
   int bi, bj, bk, share;
-  float alone, shared;
+  float alone, shared, end;
 };
 
 // The expected time of up to two products in one launch, and of joining them.
@@ -673,7 +674,8 @@ float expect(int type, const Cost& c, const Job* job, const Grid* g, int n) {
   }
   const int64_t rounds = div_up(wgs, kCus * c.share), load = div_up(wgs, kCus);
   const float even = (float)(steps / kCus) * ((float)load * kCus / wgs);  // of a CU
-  const float a = c.alone * longest * rounds, s = c.shared * even, m = (float)(bytes / 4.5e6);
+  const float a = (c.alone * longest + c.end) * rounds, s = c.shared * even + c.end * load;
+  const float m = (float)(bytes / 4.5e6);
   const float work = a > s ? a : s;
   return 4.f + (work > m ? work : m) + join;
 }
@@ -687,7 +689,7 @@ float best_slices(int type, const Cost& c, const Job* job, int n, Grid* best) {
       bool sane = true;
       for (int i = 0; i < n; ++i) {
         const int64_t want = 1ll << (i ? q : p);
-        sane = sane && (want == 1 || 4 * want * c.bk <= job[i].K);
+        sane = sane && (want == 1 || (4 * want * c.bk <= job[i].K && job[i].I * job[i].J < (1ll << 31)));
         g[i] = grid_of(job[i].I, job[i].J, job[i].K, c.bi, c.bj, c.bk, want);
       }
       const float us = sane ? expect(type, c, job, g, n) : 1e30f;
@@ -704,21 +706,23 @@ float best_slices(int type, const Cost& c, const Job* job, int n, Grid* best) {
 // outputs).
 Cost product_cost(int type, int shape) {
   if (type == VC_FP32)
-    return shape ? Cost{64, 64, 96, 1, 2.0f, 1.75f} : Cost{64, 64, 32, 3, 1.05f, 0.54f};
-  return shape ? Cost{64, 64, 256, 1, 2.9f, 2.2f} : Cost{64, 64, 64, 4, 1.3f, 0.4f};
+    return shape ? Cost{64, 64, 96, 1, 2.0f, 1.75f, 1.f} : Cost{64, 64, 32, 3, 1.05f, 0.54f, 0.5f};
+  return shape ? Cost{64, 64, 256, 1, 2.9f, 2.2f, 1.f} : Cost{64, 64, 64, 4, 1.3f, 0.4f, 0.5f};
 }
 constexpr int kGroups32 = 3, kGroups16 = 4;
 
 // The tiles that go straight into LDS: a step of one alone on a CU, and of each of
 // several that share one (measured on 264 x 328 and 512 x 512 outputs, and on 8192
-// x 16384 and 4096 x 4096).
+// x 16384 and 4096 x 4096), and their outputs (8192 x 8192, fp32 4096 x 4096, of one
+// step: 41, 37 and 41 us, fp32 22, 24 and 19).
 Cost tile_cost(int type, int shape) {
   constexpr float alone[2][3] = {{2.0f, 1.1f, 0.8f}, {1.45f, 1.1f, 0.5f}};
   constexpr float shared[2][3] = {{2.13f, 1.1f, 0.4f}, {1.9f, 0.58f, 0.21f}};
   constexpr int share[2][3] = {{1, 1, 3}, {1, 2, 4}};
+  constexpr float end[2][3] = {{6.8f, 3.8f, 0.5f}, {7.5f, 1.5f, 0.4f}};
   const TileShape t = tile_shape(type, shape);
   const int b = type == VC_FP32 ? 0 : 1;
-  return {t.bi, t.bj, t.bk, share[b][shape], alone[b][shape], shared[b][shape]};
+  return {t.bi, t.bj, t.bk, share[b][shape], alone[b][shape], shared[b][shape], end[b][shape]};
 }
 
 // Up to two products by the kernel and shape expected to be fastest.  extra: what
@@ -750,12 +754,13 @@ Cut cut_direct(int type, int64_t I, int64_t J, int64_t K) {
   Cut c = {};
   c.us = 1e30f;
   const float e = type == VC_FP32 ? 4.f : 2.f;
-  for (int shape = 0; shape < 4; ++shape) {
+  // fp32 has no 64 by 32: its parts do not fit into the registers
+  for (int shape = 0; shape < (type == VC_FP32 ? 3 : 4); ++shape) {
     const int bi = kDirectRows[shape], bj = kDirectCols[shape];
     const int64_t nj = div_up(J, bj), tiles = div_up(I, bi) * nj;
     int64_t s = 1;
     while (tiles * s < kCus && 1024 * s < K && s < 16) s *= 2;
-    const float own = e * ((I < bi ? I : bi) + bj) * (float)K / s;
+    const float own = e * (bi + bj) * (float)K / s;  // rows past the last are read as the last
     const float l2 = div_up(tiles * s, kCus) * own / 25e3f;
     const float hbm = e * (I + J) * (float)K / 4.5e6f;
     const float us = 3.f + (l2 > hbm ? l2 : hbm) + join_us(s, I, J);
@@ -771,7 +776,7 @@ bool tile_lines(int64_t n) { return n > 0 && n < (1 << 21); }
 float pack_us(int type, int64_t n) { return 4.f + n * (type == VC_FP32 ? 10.f : 4.f) / 4e6f; }
 
 int64_t part_bytes(const Cut& c, int64_t I, int64_t J) {
-  return c.slices > 1 ? up256(4 * c.slices * I * J) : 0;
+  return c.slices > 1 ? up256(4 * c.slices * I * part_line((int)J)) : 0;
 }
 
 // A matrix of `rows` lines as parts, and whether it has to be made into them.
@@ -784,13 +789,7 @@ int64_t parts_bytes(int type, int64_t rows, int64_t n) {
 }
 
 template <class T>
-bool quads(const void* p, int64_t ld) {
-  return !p || (((uintptr_t)p & (4 * sizeof(T) - 1)) == 0 && ld % 4 == 0);
-}
-
-template <class T>
 void set_cut(Product<T>& a, const Cut& c, void* part) {
-  a.wide = a.J % 4 == 0 && quads<T>(a.out, a.J) && quads<T>(a.z, a.J) && quads<T>(a.res, a.ldr);
   a.slices = c.slices;
   a.steps = c.steps;
   a.part = (float*)part;
@@ -802,10 +801,15 @@ bool too_many(const Cut& c) { return c.tiles > (1 << 21) || c.tiles * c.slices >
 
 template <class T>
 void run_join(const Product<T>& a, const Product<T>& b, hipStream_t st) {
-  const int64_t n = (a.slices > 1 ? (int64_t)a.I * ((a.J + 3) / 4) : 0) +
-                    (b.slices > 1 ? (int64_t)b.I * ((b.J + 3) / 4) : 0);
-  const int64_t blocks = div_up(n, LNT);
-  if (n > 0) k_join<T><<<(unsigned)(blocks < 4096 ? blocks : 4096), LNT, 0, st>>>(a, b);
+  const auto quads = [](const Product<T>& p) {
+    return p.slices > 1 ? (uint32_t)p.I * (uint32_t)(part_line(p.J) / 4) : 0u;
+  };
+  const auto line = [](const Product<T>& p) {
+    return vcg::FastDiv::make((uint32_t)(p.slices > 1 ? part_line(p.J) / 4 : 1));
+  };
+  const uint32_t na = quads(a), nb = quads(b);
+  if (na + nb > 0)
+    k_join<T><<<(unsigned)div_up((int64_t)na + nb, LNT), LNT, 0, st>>>(a, na, line(a), b, nb, line(b));
 }
 
 template <class T>
@@ -836,7 +840,7 @@ ForwardPlan plan_forward(int type, int64_t M, int K, int N, bool raw) {
   if (raw) {
     // two steps of 32 alone on a CU, and of each of two that share one (512 x 784 x
     // 1024)
-    const Cost c = {64, 32, 64, 2, 0.55f, 0.5f};
+    const Cost c = {64, 32, 64, 2, 0.55f, 0.5f, 0.5f};
     Grid g;
     const float us = best_slices(type, c, &job, 1, &g);
     if (us < p.c.us) p.c = {kRaw, 0, (int)g.slices, (int)g.steps * 2, g.tiles, g.nj, us};
@@ -900,16 +904,17 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
   else if (p.c.shape == 0) k_direct<T, 1, 1, F ? 2 : 8><<<grid, threads, 0, st>>>(a);
   else if (p.c.shape == 1) k_direct<T, 1, 2, F ? 2 : 4><<<grid, threads, 0, st>>>(a);
   else if (p.c.shape == 2) k_direct<T, 1, 4, F ? 1 : 2><<<grid, threads, 0, st>>>(a);
-  else k_direct<T, 2, 4, F ? 1 : 2><<<grid, threads, 0, st>>>(a);
+  else if constexpr (!F) k_direct<T, 2, 4, 2><<<grid, threads, 0, st>>>(a);
   run_join<T>(a, {}, st);
   VC_LAUNCH_CHECK();
   return VC_OK;
 }
 
-// Rows of a block of dz: at most 256 blocks.
+// Rows of a block of dz: eight, one a thread, while 256 blocks hold M (265 x 461 with
+// silu: 32 rows 8.6 us, eight of them RRR), beyond that what 256 need.
 int slope_rows(int64_t M) {
   const int64_t r = (M + 255) / 256;
-  return (int)(r < 32 ? 32 : r);
+  return r <= 8 ? 8 : (int)(r < 32 ? 32 : r);
 }
 
 struct BackwardPlan {
@@ -929,8 +934,13 @@ BackwardPlan plan_backward(int type, int64_t M, int K, int N, int act, int need)
   job[1] = {M, K, N};
   if (need & 3) {
     const float pack = type == VC_FP32 || K % 8 ? pack_us(type, (M + N) * K) : 0.f;
-    choose(type, job, 2, tile_lines(K) && tile_lines(N), pack, c);
+    const bool can = tile_lines(K) && tile_lines(N);
+    const float one = choose(type, job, 2, can, pack, c);
     p.tiles = c[0].kernel == kTile;
+    // or a launch each, in a shape of its own
+    Cut w = {}, x = {};
+    const float two = choose(type, job, 1, can, pack, &w) + choose(type, job + 1, 1, can, 0.f, &x);
+    if (p.tiles && w.kernel == kTile && x.kernel == kTile && two < one) c[0] = w, c[1] = x;
   }
   if (need & 2) p.w = c[0];
   if (need & 1) p.x = c[1];
@@ -1026,12 +1036,14 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
   const unsigned grid = (unsigned)(p.w.tiles * p.w.slices + p.x.tiles * p.x.slices + (db ? div_up(N, 32) : 0));
   constexpr int G = sizeof(T) == 4 ? kGroups32 : kGroups16;
   const Cut& any = dW ? p.w : p.x;
-  // two that each fill the chip go one after the other: their tiles share what
-  // they read while they run in step (8192 x 4096 x 4096 bf16: 495 us, together 567)
-  if (p.tiles && dW && dx && p.w.tiles * p.w.slices >= kCus && p.x.tiles * p.x.slices >= kCus) {
-    run_tiles<T>(pw, {}, c, any.shape, (unsigned)(p.w.tiles * p.w.slices), st);
+  // two of different shapes, or that each fill the chip, go one after the other: their
+  // tiles share what they read while they run in step (8192 x 4096 x 4096 bf16: 495
+  // us, together 567)
+  const int64_t nw = p.w.tiles * p.w.slices, nx = p.x.tiles * p.x.slices;
+  if (p.tiles && dW && dx && (p.w.shape != p.x.shape || (nw >= kCus && nx >= kCus))) {
     Product<T> none = {};
-    run_tiles<T>(none, px, c, any.shape, grid - (unsigned)(p.w.tiles * p.w.slices), st);
+    run_tiles<T>(pw, none, c, p.w.shape, (unsigned)nw, st);
+    run_tiles<T>(none, px, c, p.x.shape, grid - (unsigned)nw, st);
   } else if (p.tiles) run_tiles<T>(pw, px, c, any.shape, grid, st);
   else if (any.shape == 0 || !(need & 3)) k_products<T, 1><<<grid, LNT, 0, st>>>(pw, px, c);
   else k_products<T, G><<<grid, LNT * G, 0, st>>>(pw, px, c);

@@ -96,9 +96,8 @@ struct Side {
       int line, chunk;
       at(i, wv, lane, line, chunk);
       const bool in = X ? line < left : chunk * 8 < left;
-      u4 v = u4{0, 0, 0, 0};
-      if (in) v = *reinterpret_cast<const u4*>(reinterpret_cast<const char*>(from) + off[i]);
-      *reinterpret_cast<u4*>(lds + (i * NW + wv) * 1024 + lane * 16) = v;
+      const u4 v = *reinterpret_cast<const u4*>(reinterpret_cast<const char*>(from) + (in ? off[i] : 0));
+      *reinterpret_cast<u4*>(lds + (i * NW + wv) * 1024 + lane * 16) = in ? v : u4{0, 0, 0, 0};
     }
   }
 
@@ -284,7 +283,7 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
             if (s + AHEAD < full) wait_for<(AHEAD - 1) * kLoads, true>();
             else wait_for<0, true>();
           } else {
-            __builtin_amdgcn_s_waitcnt(63 & 15 | 7 << 4 | 0 << 8 | 3 << 14);  // fragments only
+            __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 3 << 14);  // fragments only
           }
           turn();
           __builtin_amdgcn_s_setprio(1);
@@ -323,8 +322,12 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
   // c of row i at c ^ (i mod 16).
   constexpr int Q = BJ / 4, kFit = NBUF * kStage / (BJ * 4), ROWS = kFit < BI ? BI / WI : BI;
   static_assert(ROWS <= kFit && Q >= 16);
+  constexpr int STEP = 64 * NW / Q, U = ROWS < BI ? 4 : ROWS / STEP < 8 ? ROWS / STEP : 8;
+  static_assert(64 * NW % Q == 0 && ROWS % (STEP * U) == 0);
   v4f* const sums = reinterpret_cast<v4f*>(lds);
   const int g = lane >> 4, r = lane & 15;
+  const int q = tid % Q, row0 = tid / Q, j = j0 + 4 * q;
+  const v4f bias = bias_of(a, j);
 #pragma unroll 1
   for (int p = 0; p < BI / ROWS; ++p) {
     __syncthreads();
@@ -338,21 +341,44 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
         }
     }
     __syncthreads();
-#pragma unroll 4
-    for (int t = tid; t < ROWS * Q; t += 64 * NW) {
-      const int row = t / Q, q = t % Q;
-      const int64_t i = i0 + p * ROWS + row;
-      const int j = j0 + 4 * q;
-      if (i >= a.I || j >= a.J) continue;
-      const v4f w = sums[row * Q + (q ^ (row & 15))];
-      float v[4] = {w[0], w[1], w[2], w[3]};
+#pragma unroll 1
+    for (int t = row0; t < ROWS; t += U * STEP) {
+      const int i = i0 + p * ROWS + t;
+      if (i >= a.I || j >= a.J) break;
+      v4f w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = sums[(t + u * STEP) * Q + (q ^ ((t + u * STEP) & 15))];
+      bool apart = a.slices == 1 && j + 4 > a.J;
       if constexpr (NP == 3) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (!finite(v[k]) && j + k < a.J)
-            v[k] = plain_sum<XA, XB>(a, i, j + k, k0, k0 + left);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) apart |= !finite(w[u][k]);
       }
-      deliver(a, slice, i, j, v);
+      if (!apart && a.slices == 1) {
+        finish_rows<T, U>(a, i, STEP, j, bias, w);
+      } else if (!apart) {
+        const int line = part_line(a.J);
+        float* const o = a.part + (slice * (int64_t)a.I + i) * line + j;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (i + u * STEP < a.I) *reinterpret_cast<v4f*>(o + (int64_t)u * STEP * line) = w[u];
+      } else {
+#pragma unroll 1
+        for (int u = t; u < t + U * STEP && i0 + p * ROWS + u < a.I; u += STEP) {
+          const int iu = i0 + p * ROWS + u;
+          v4f x = sums[u * Q + (q ^ (u & 15))];
+          if constexpr (NP == 3) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float v = x[k];
+              if (!finite(v) && j + k < a.J)
+                x[k] = plain_sum<XA, XB>(a, iu, j + k, k0, k0 + left);
+            }
+          }
+          deliver(a, slice, iu, j, x);
+        }
+      }
     }
   }
 }
@@ -484,9 +510,7 @@ __global__ __launch_bounds__(512, 2) void k_raw(Product<float> a) {
   }
   const int row = tid / Q, q = tid % Q, j = j0 + 4 * q;
   if (i0 + row >= a.I || j >= a.J) return;
-  const v4f s = sums[row * Q + (q ^ (row & 7))];
-  const float v[4] = {s[0], s[1], s[2], s[3]};
-  deliver(a, slice, i0 + row, j, v);
+  deliver(a, slice, i0 + row, j, sums[row * Q + (q ^ (row & 7))]);
 }
 
 // A kernel's LDS limit, set once per device.
