@@ -682,13 +682,14 @@ float expect(int type, const Cost& c, const Job* job, const Grid* g, int n) {
 
 // The slices that are expected to be fastest, of up to two products.
 float best_slices(int type, const Cost& c, const Job* job, int n, Grid* best) {
+  constexpr int kWant[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32}, kN = 15;
   float least = 1e30f;
-  for (int p = 0; p < 6; ++p)
-    for (int q = 0; q < (n > 1 ? 6 : 1); ++q) {
+  for (int p = 0; p < kN; ++p)
+    for (int q = 0; q < (n > 1 ? kN : 1); ++q) {
       Grid g[2];
       bool sane = true;
       for (int i = 0; i < n; ++i) {
-        const int64_t want = 1ll << (i ? q : p);
+        const int64_t want = kWant[i ? q : p];
         sane = sane && (want == 1 || (4 * want * c.bk <= job[i].K && job[i].I * job[i].J < (1ll << 31)));
         g[i] = grid_of(job[i].I, job[i].J, job[i].K, c.bi, c.bj, c.bk, want);
       }
@@ -746,8 +747,9 @@ float choose(int type, const Job* job, int n, bool tiles, float extra, Cut* out)
 }
 
 // The direct kernel: 16 rows by 16 columns, 32 by 16, 64 by 16, 64 by 32.  A
-// workgroup's operands come at about 25 GB/s a CU (sixteen rows a load, 16 bytes a
-// lane), all of them together at no more than the memory's rate.
+// workgroup's operands come at about 40 GB/s a CU (sixteen rows a load, 16 bytes a
+// lane; 5 x 15872 x 788 fp32 18.7 us, the tiles of 64 x 32 30), all of them together
+// at no more than the memory's rate.
 constexpr int kDirectRows[4] = {16, 32, 64, 64}, kDirectCols[4] = {16, 16, 16, 32};
 
 Cut cut_direct(int type, int64_t I, int64_t J, int64_t K) {
@@ -761,7 +763,7 @@ Cut cut_direct(int type, int64_t I, int64_t J, int64_t K) {
     int64_t s = 1;
     while (tiles * s < kCus && 1024 * s < K && s < 16) s *= 2;
     const float own = e * (bi + bj) * (float)K / s;  // rows past the last are read as the last
-    const float l2 = div_up(tiles * s, kCus) * own / 25e3f;
+    const float l2 = div_up(tiles * s, kCus) * own / 40e3f;
     const float hbm = e * (I + J) * (float)K / 4.5e6f;
     const float us = 3.f + (l2 > hbm ? l2 : hbm) + join_us(s, I, J);
     if (us < c.us) c = {kDirect, shape, (int)s, 0, tiles, nj, us};
@@ -829,8 +831,32 @@ struct ForwardPlan {
   int64_t x, W, part, bytes;  // offsets in the workspace, and its size
 };
 
+// A thread's latest plans, by their sizes: the search takes up to 50 us.
+template <class Plan>
+struct Plans {
+  struct Entry {
+    int64_t key[6];
+    bool set;
+    Plan plan;
+  } all[64];
+  template <class Make>
+  const Plan& get(const int64_t (&key)[6], const Make& make) {
+    uint64_t h = 0;
+    for (const int64_t k : key) h = (h ^ (uint64_t)k) * 0x9e3779b97f4a7c15ull;
+    Entry& e = all[h >> 58];
+    bool same = e.set;
+    for (int i = 0; i < 6; ++i) same = same && e.key[i] == key[i];
+    if (!same) {
+      e.plan = make();
+      for (int i = 0; i < 6; ++i) e.key[i] = key[i];
+      e.set = true;
+    }
+    return e.plan;
+  }
+};
+
 // raw: fp32 rows that the loads into LDS can take as they are.
-ForwardPlan plan_forward(int type, int64_t M, int K, int N, bool raw) {
+ForwardPlan make_forward(int type, int64_t M, int K, int N, bool raw) {
   ForwardPlan p;
   const Job job = {M, N, K};
   const float pack = type == VC_FP32 || K % 8 ? pack_us(type, (M + N) * K) : 0.f;
@@ -851,6 +877,10 @@ ForwardPlan plan_forward(int type, int64_t M, int K, int N, bool raw) {
   p.part = p.W + (tiles ? parts_bytes(type, N, K) : 0);
   p.bytes = p.part + part_bytes(p.c, M, N);
   return p;
+}
+ForwardPlan plan_forward(int type, int64_t M, int K, int N, bool raw) {
+  static thread_local Plans<ForwardPlan> plans;
+  return plans.get({type, M, K, N, raw, 0}, [&] { return make_forward(type, M, K, N, raw); });
 }
 
 template <class T>
@@ -911,7 +941,7 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
 }
 
 // Rows of a block of dz: eight, one a thread, while 256 blocks hold M (265 x 461 with
-// silu: 32 rows 8.6 us, eight of them RRR), beyond that what 256 need.
+// silu: 32 rows 8.6 us, eight 3.8), beyond that what 256 need.
 int slope_rows(int64_t M) {
   const int64_t r = (M + 255) / 256;
   return r <= 8 ? 8 : (int)(r < 32 ? 32 : r);
@@ -924,7 +954,7 @@ struct BackwardPlan {
   int64_t dz, W, in, sums, px, pw, bytes;  // offsets in the workspace, and its size
 };
 
-BackwardPlan plan_backward(int type, int64_t M, int K, int N, int act, int need) {
+BackwardPlan make_backward(int type, int64_t M, int K, int N, int act, int need) {
   BackwardPlan p = {};
   const int64_t e = type == VC_FP32 ? 4 : 2;
   Job job[2];
@@ -960,6 +990,11 @@ BackwardPlan plan_backward(int type, int64_t M, int K, int N, int act, int need)
   if (need & 2) at += part_bytes(p.w, N, K);
   p.bytes = at;
   return p;
+}
+BackwardPlan plan_backward(int type, int64_t M, int K, int N, int act, int need) {
+  static thread_local Plans<BackwardPlan> plans;
+  return plans.get({type, M, K, N, act, need},
+                   [&] { return make_backward(type, M, K, N, act, need); });
 }
 
 template <class T>
