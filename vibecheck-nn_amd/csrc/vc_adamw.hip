@@ -152,7 +152,7 @@ __device__ __forceinline__ uint32_t dither_of(uint32_t i, uint32_t seed) {
 // those of the plain sequence of operations.
 __device__ __forceinline__ float update8(float p, float g, float& m, float& v, const Step& a) {
   m = a.b1 * m + a.c.w1 * g;
-  v = __fsqrt_rn(a.c.b2 * v + a.c.w2 * g * g);
+  v = __builtin_sqrtf(a.c.b2 * v + a.c.w2 * g * g);  // __fsqrt_rn can be off by one
   return p + __fdiv_rn(a.c.neg_step * m, __fdiv_rn(v, a.c.bc2) + a.c.eps);
 }
 
