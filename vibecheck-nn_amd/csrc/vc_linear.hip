@@ -471,10 +471,17 @@ __device__ __forceinline__ void join_quad(const Product<T>& a, uint32_t t, vcg::
   finish(a, i, j, v);
 }
 
+// Workgroups of the columns' sums first, where dz has any left to join.
 template <class T>
 __global__ __launch_bounds__(LNT) void k_join(Product<T> a, uint32_t na, vcg::FastDiv la,
-                                              Product<T> b, uint32_t nb, vcg::FastDiv lb) {
-  const uint32_t t = blockIdx.x * LNT + threadIdx.x;
+                                              Product<T> b, uint32_t nb, vcg::FastDiv lb,
+                                              Columns<T> c, uint32_t nc) {
+  __shared__ float lds[LNT];
+  if (blockIdx.x < nc) {
+    add_columns(c, (int)blockIdx.x, lds);
+    return;
+  }
+  const uint32_t t = (blockIdx.x - nc) * LNT + threadIdx.x;
   if (t < na) join_quad(a, t, la);
   else if (t - na < nb) join_quad(b, t - na, lb);
 }
@@ -717,8 +724,8 @@ constexpr int kGroups32 = 3, kGroups16 = 4;
 // x 16384 and 4096 x 4096), and their outputs (8192 x 8192, fp32 4096 x 4096, of one
 // step: 41, 37 and 41 us, fp32 22, 24 and 19).
 Cost tile_cost(int type, int shape) {
-  constexpr float alone[2][3] = {{2.0f, 1.1f, 0.8f}, {1.45f, 1.1f, 0.5f}};
-  constexpr float shared[2][3] = {{2.13f, 1.1f, 0.4f}, {1.9f, 0.58f, 0.21f}};
+  constexpr float alone[2][3] = {{2.0f, 0.98f, 0.8f}, {1.45f, 1.1f, 0.5f}};
+  constexpr float shared[2][3] = {{2.13f, 0.98f, 0.4f}, {1.9f, 0.58f, 0.21f}};
   constexpr int share[2][3] = {{1, 1, 3}, {1, 2, 4}};
   constexpr float end[2][3] = {{6.8f, 3.8f, 0.5f}, {7.5f, 1.5f, 0.4f}};
   const TileShape t = tile_shape(type, shape);
@@ -802,7 +809,7 @@ void set_cut(Product<T>& a, const Cut& c, void* part) {
 bool too_many(const Cut& c) { return c.tiles > (1 << 21) || c.tiles * c.slices > (1 << 21); }
 
 template <class T>
-void run_join(const Product<T>& a, const Product<T>& b, hipStream_t st) {
+void run_join(const Product<T>& a, const Product<T>& b, const Columns<T>& c, hipStream_t st) {
   const auto quads = [](const Product<T>& p) {
     return p.slices > 1 ? (uint32_t)p.I * (uint32_t)(part_line(p.J) / 4) : 0u;
   };
@@ -810,8 +817,9 @@ void run_join(const Product<T>& a, const Product<T>& b, hipStream_t st) {
     return vcg::FastDiv::make((uint32_t)(p.slices > 1 ? part_line(p.J) / 4 : 1));
   };
   const uint32_t na = quads(a), nb = quads(b);
-  if (na + nb > 0)
-    k_join<T><<<(unsigned)div_up((int64_t)na + nb, LNT), LNT, 0, st>>>(a, na, line(a), b, nb, line(b));
+  const uint32_t nc = c.db ? (uint32_t)div_up(c.N, 32) : 0u;
+  const unsigned grid = nc + (unsigned)div_up((int64_t)na + nb, LNT);
+  if (grid > 0) k_join<T><<<grid, LNT, 0, st>>>(a, na, line(a), b, nb, line(b), c, nc);
 }
 
 template <class T>
@@ -935,7 +943,7 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
   else if (p.c.shape == 1) k_direct<T, 1, 2, F ? 2 : 4><<<grid, threads, 0, st>>>(a);
   else if (p.c.shape == 2) k_direct<T, 1, 4, F ? 1 : 2><<<grid, threads, 0, st>>>(a);
   else if constexpr (!F) k_direct<T, 2, 4, 2><<<grid, threads, 0, st>>>(a);
-  run_join<T>(a, {}, st);
+  run_join<T>(a, {}, {}, st);
   VC_LAUNCH_CHECK();
   return VC_OK;
 }
@@ -1067,8 +1075,12 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
   px.pa = pw.pa = (const uint16_t*)dz;
   px.lda = pw.lda = ldd;
   px.planeA = pw.planeA = M * np;
-  const Columns<T> c = {(const float*)(base + p.sums), p.blocks, N, db ? (T*)db : nullptr};
-  const unsigned grid = (unsigned)(p.w.tiles * p.w.slices + p.x.tiles * p.x.slices + (db ? div_up(N, 32) : 0));
+  // the columns' sums: in the join's launch where there is one (beside the products they
+  // would wait for a CU's whole LDS), else in the products'
+  const Columns<T> sums = {(const float*)(base + p.sums), p.blocks, N, db ? (T*)db : nullptr};
+  const bool late = p.w.slices > 1 || p.x.slices > 1;
+  const Columns<T> c = late ? Columns<T>{} : sums;
+  const unsigned grid = (unsigned)(p.w.tiles * p.w.slices + p.x.tiles * p.x.slices + (c.db ? div_up(N, 32) : 0));
   constexpr int G = sizeof(T) == 4 ? kGroups32 : kGroups16;
   const Cut& any = dW ? p.w : p.x;
   // two of different shapes, or that each fill the chip, go one after the other: their
@@ -1079,10 +1091,11 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
     Product<T> none = {};
     run_tiles<T>(pw, none, c, p.w.shape, (unsigned)nw, st);
     run_tiles<T>(none, px, c, p.x.shape, grid - (unsigned)nw, st);
+  } else if (grid == 0) {
   } else if (p.tiles) run_tiles<T>(pw, px, c, any.shape, grid, st);
   else if (any.shape == 0 || !(need & 3)) k_products<T, 1><<<grid, LNT, 0, st>>>(pw, px, c);
   else k_products<T, G><<<grid, LNT * G, 0, st>>>(pw, px, c);
-  run_join<T>(pw, px, st);
+  run_join<T>(pw, px, late ? sums : Columns<T>{}, st);
   VC_LAUNCH_CHECK();
   return VC_OK;
 }
