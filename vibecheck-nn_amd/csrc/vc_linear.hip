@@ -680,7 +680,8 @@ float expect(int type, const Cost& c, const Job* job, const Grid* g, int n) {
     join = join > 0.f && j > 0.f ? join + j - 4.f : join + j;
   }
   const int64_t rounds = div_up(wgs, kCus * c.share), load = div_up(wgs, kCus);
-  const float even = (float)(steps / kCus) * ((float)load * kCus / wgs);  // of a CU
+  // of a CU: the busiest where several share one, else the mean
+  const float even = (float)(steps / kCus) * (c.share > 1 ? (float)load * kCus / wgs : 1.f);
   const float a = (c.alone * longest + c.end) * rounds, s = c.shared * even + c.end * load;
   const float m = (float)(bytes / 4.5e6);
   const float work = a > s ? a : s;
@@ -719,13 +720,15 @@ Cost product_cost(int type, int shape) {
 }
 constexpr int kGroups32 = 3, kGroups16 = 4;
 
-// The tiles that go straight into LDS: a step of one alone on a CU, and of each of
-// several that share one (measured on 264 x 328 and 512 x 512 outputs, and on 8192
-// x 16384 and 4096 x 4096), and their outputs (8192 x 8192, fp32 4096 x 4096, of one
-// step: 41, 37 and 41 us, fp32 22, 24 and 19).
+// The tiles that go straight into LDS: a step of as many as share a CU while others
+// stand idle, a step of each with all of them busy (random operands: the card's power
+// then sets the pace), and a tile's output (8192 x 8192, fp32 4096 x 4096, of one step:
+// 41, 37 and 41 us, fp32 22, 24 and 19).  8192 x 4096 x 4096 bf16 212, 255 and 383 us,
+// 1024 x 1024 x 1024 27, 13 and 7.5; fp32 8192 x 1024 x 4096 331, 348 and 485, 2048
+// x 2048 x 2048 134, 87 and 151, 1024 x 1024 x 1024 64, 36 and 24.
 Cost tile_cost(int type, int shape) {
-  constexpr float alone[2][3] = {{2.0f, 0.98f, 0.8f}, {1.45f, 1.1f, 0.5f}};
-  constexpr float shared[2][3] = {{2.13f, 0.98f, 0.4f}, {1.9f, 0.58f, 0.21f}};
+  constexpr float alone[2][3] = {{2.0f, 1.06f, 0.6f}, {1.15f, 0.6f, 0.25f}};
+  constexpr float shared[2][3] = {{2.3f, 1.19f, 0.48f}, {1.6f, 0.47f, 0.17f}};
   constexpr int share[2][3] = {{1, 1, 3}, {1, 2, 4}};
   constexpr float end[2][3] = {{6.8f, 3.8f, 0.5f}, {7.5f, 1.5f, 0.4f}};
   const TileShape t = tile_shape(type, shape);
@@ -735,7 +738,7 @@ Cost tile_cost(int type, int shape) {
 
 // Up to two products by the kernel and shape expected to be fastest.  extra: what
 // the tiles' parts cost before.
-float choose(int type, const Job* job, int n, bool tiles, float extra, Cut* out) {
+float choose(int type, const Job* job, int n, bool products, bool tiles, float extra, Cut* out) {
   float least = 1e30f;
   const auto take = [&](Kernel k, int shape, const Cost& c, float more) {
     Grid g[2];
@@ -747,7 +750,7 @@ float choose(int type, const Job* job, int n, bool tiles, float extra, Cut* out)
       out[i] = {k, shape, (int)g[i].slices, (int)g[i].steps * per, g[i].tiles, g[i].nj, us};
     }
   };
-  for (int shape = 0; shape < 2; ++shape) take(kProduct, shape, product_cost(type, shape), 0.f);
+  for (int shape = 0; shape < (products ? 2 : 0); ++shape) take(kProduct, shape, product_cost(type, shape), 0.f);
   if (tiles)
     for (int shape = 0; shape < 3; ++shape) take(kTile, shape, tile_cost(type, shape), extra);
   return least;
@@ -868,9 +871,11 @@ ForwardPlan make_forward(int type, int64_t M, int K, int N, bool raw) {
   ForwardPlan p;
   const Job job = {M, N, K};
   const float pack = type == VC_FP32 || K % 8 ? pack_us(type, (M + N) * K) : 0.f;
-  choose(type, &job, 1, tile_lines(K), pack, &p.c);
-  const Cut d = cut_direct(type, M, N, K);
-  if (d.us < p.c.us) p.c = d;
+  p.c = cut_direct(type, M, N, K);
+  Cut c = {};
+  // bf16 goes by the tiles or directly: between them the other products gain nothing
+  choose(type, &job, 1, type == VC_FP32, tile_lines(K), pack, &c);
+  if (c.us > 0.f && c.us < p.c.us) p.c = c;
   if (raw) {
     // two steps of 32 alone on a CU, and of each of two that share one (512 x 784 x
     // 1024)
@@ -932,13 +937,17 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
   constexpr bool F = sizeof(T) == 4;
   const dim3 grid((unsigned)p.c.tiles, (unsigned)p.c.slices);
   const unsigned flat = (unsigned)(p.c.tiles * p.c.slices);
-  constexpr int G = F ? kGroups32 : kGroups16, threads = 64 * kDirectWaves;
+  constexpr int threads = 64 * kDirectWaves;
   if (p.c.kernel == kTile) {
     run_tile<T>(a, p.c.shape, st);
   } else if (p.c.kernel == kRaw) {
     if constexpr (F) run_raw(a, st);
-  } else if (p.c.kernel == kProduct && p.c.shape == 0) k_product<T, 1><<<flat, LNT, 0, st>>>(a);
-  else if (p.c.kernel == kProduct) k_product<T, G><<<flat, LNT * G, 0, st>>>(a);
+  } else if (p.c.kernel == kProduct) {
+    if constexpr (F) {
+      if (p.c.shape == 0) k_product<T, 1><<<flat, LNT, 0, st>>>(a);
+      else k_product<T, kGroups32><<<flat, LNT * kGroups32, 0, st>>>(a);
+    }
+  }
   else if (p.c.shape == 0) k_direct<T, 1, 1, F ? 2 : 8><<<grid, threads, 0, st>>>(a);
   else if (p.c.shape == 1) k_direct<T, 1, 2, F ? 2 : 4><<<grid, threads, 0, st>>>(a);
   else if (p.c.shape == 2) k_direct<T, 1, 4, F ? 1 : 2><<<grid, threads, 0, st>>>(a);
@@ -973,11 +982,11 @@ BackwardPlan make_backward(int type, int64_t M, int K, int N, int act, int need)
   if (need & 3) {
     const float pack = type == VC_FP32 || K % 8 ? pack_us(type, (M + N) * K) : 0.f;
     const bool can = tile_lines(K) && tile_lines(N);
-    const float one = choose(type, job, 2, can, pack, c);
+    const float one = choose(type, job, 2, true, can, pack, c);
     p.tiles = c[0].kernel == kTile;
     // or a launch each, in a shape of its own
     Cut w = {}, x = {};
-    const float two = choose(type, job, 1, can, pack, &w) + choose(type, job + 1, 1, can, 0.f, &x);
+    const float two = choose(type, job, 1, false, can, pack, &w) + choose(type, job + 1, 1, false, can, 0.f, &x);
     if (p.tiles && w.kernel == kTile && x.kernel == kTile && two < one) c[0] = w, c[1] = x;
   }
   if (need & 2) p.w = c[0];
