@@ -106,6 +106,52 @@ def test_linear_backward(gpu, to, M, K, N, act):
     assert part[0] is None and part[2] is None and torch.equal(part[1], dW)
 
 
+# Long sums, many tiles, few of either: each way that a product can be cut, odd edges and tails.
+@pytest.mark.parametrize('to,M,K,N', [
+    (F32, 17, 1031, 1030), (F32, 520, 15872, 10), (F32, 8200, 5, 10), (F32, 4100, 784, 50),
+    (F32, 1, 15872, 513), (F32, 131, 203, 8200), (F32, 1, 15873, 2051), (F32, 131, 1031, 4096),
+    (F32, 17, 15873, 513), (F32, 1021, 333, 4096), (F32, 1021, 1031, 1030), (F32, 2050, 785, 2051),
+    (F32, 1021, 2049, 2051), (F32, 8200, 65, 8200), (F32, 513, 100, 33), (F32, 65, 2044, 97),
+    (BF16, 17, 1031, 1030), (BF16, 520, 15872, 10), (BF16, 8200, 5, 10), (BF16, 4100, 5, 50),
+    (BF16, 257, 15872, 50), (BF16, 1, 2048, 8200), (BF16, 1, 15872, 513), (BF16, 1021, 333, 4096),
+    (BF16, 2050, 15870, 256), (BF16, 1021, 781, 8200), (BF16, 131, 15872, 8198)])
+def test_linear_cuts(gpu, to, M, K, N):
+    test_linear(gpu, to, M, K, N, 'gelu', True)
+    test_linear(gpu, to, M, K, N, None, False)
+
+
+@pytest.mark.parametrize('to,M,K,N', [
+    (F32, 257, 5, 513), (F32, 8200, 5, 10), (F32, 1, 5, 8200), (F32, 1021, 64, 4096),
+    (F32, 1021, 2049, 1030), (F32, 1021, 4095, 2050), (F32, 8200, 333, 1030), (F32, 520, 783, 8200),
+    (F32, 1021, 333, 2051), (F32, 8200, 784, 513), (F32, 2050, 1031, 513), (F32, 257, 4096, 513),
+    (BF16, 4100, 333, 10), (BF16, 1021, 5, 8200), (BF16, 1, 5, 256), (BF16, 1021, 4096, 1030),
+    (BF16, 2050, 783, 8200), (BF16, 520, 4096, 4095), (BF16, 4100, 1031, 513), (BF16, 131, 4095, 8200),
+    (BF16, 8200, 784, 1030), (BF16, 2050, 5, 513), (BF16, 257, 15872, 117)])
+def test_linear_backward_cuts(gpu, to, M, K, N):
+    test_linear_backward(gpu, to, M, K, N, 'silu')
+    test_linear_backward(gpu, to, M, K, N, None)
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('M,K,N', [(520, 784, 1024), (1021, 333, 4096), (1021, 1031, 1030), (2050, 785, 2051)])
+def test_linear_infinities_and_nan_in_tiles(gpu, to, M, K, N):
+    test_linear_infinities_and_nan(gpu, to, M, K, N)
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+def test_linear_backward_infinities_and_nan(gpu, to):
+    """What is not finite in the gradient or the input reaches its own rows and columns."""
+    M, K, N = 1030, 520, 777
+    f = _randn(gpu, 12)
+    x, W, dy = f(M, K, to=to), f(N, K, to=to, std=0.05), f(M, N, to=to)
+    dy[5, 7], dy[700, 8], x[1000, 9] = math.inf, math.nan, -math.inf
+    got = train.linear_backward(dy, x, W)
+    d, xd = dy.double(), x.double()
+    for p, q in zip(got, (d @ W.double(), d.t() @ xd, d.sum(0))):
+        assert torch.equal(p.isnan(), q.isnan()) and torch.equal(p.isinf(), q.isinf())
+        assert torch.equal(p[p.isinf()].double(), q[q.isinf()])
+
+
 @pytest.mark.parametrize('to', [F32, BF16])
 def test_linear_strides_and_alignment(gpu, to):
     """Rows apart, bases off a 16-byte boundary, an expanded row, leading axes: the same results
@@ -298,6 +344,22 @@ def test_cross_entropy(gpu, to, R, V, e):
     t = torch.randint(0, V, (R,), device=gpu, generator=torch.Generator(device=gpu).manual_seed(V))
     t[1::5] = -100
     _check_loss(z, t, e)
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('held', [64, 128, 256, 512, 768, 1024, 1536, 2048, 3 * 1024, 4096, 6144, 8192,
+                                  10240, 13312, 16384])
+def test_cross_entropy_where_the_team_changes(gpu, to, held):
+    """Rows that just fill what a team holds, and that end just past it."""
+    V = held * (4 if to == F32 else 8)
+    for n in (V - 1, V + 3):
+        z = _randn(gpu, n)(5, n, to=to, std=3.0)
+        t = torch.tensor([0, n - 1, -100, n // 2, n - 4], device=gpu)
+        z[3, 1:] = -math.inf
+        z[3, t[3]] = 1.0
+        _check_loss(z, t, 0.0)
+        z[3] = 2.0
+        _check_loss(z, t, 0.1)
 
 
 @pytest.mark.parametrize('to', [F32, BF16])
@@ -500,6 +562,47 @@ def test_adamw_8(gpu, pt, gt, sizes, shift):
             at += nb
 
 
+def _single(x):
+    """Each operation in 64 bits and rounded to 32: what the operation in 32 bits gives."""
+    return x.float().double()
+
+
+def test_adamw_8_to_the_bit(gpu):
+    """What is stored is cut from m and u = sqrt(v), so their last bits count: state and scales
+    equal those of the plain sequence of 32-bit operations, bit for bit."""
+    n, (b1, b2) = 1 << 20, HYPER['betas']
+    f = _randn(gpu, 10)
+    p, state = f(n), train.adamw_state([f(n)], bits=8)
+    c = [float(torch.tensor(v, dtype=F32)) for v in (b1, 1 - b1, b2, 1 - b2, 1 / 448)]
+    i = torch.arange(n, device=gpu)
+    for k in range(1, 4):
+        g = f(n) * torch.exp(3 * f(n))
+        g[::5] = 0
+        m, u = (t.double() for t in (_single(state['m'].view(torch.float8_e4m3fn).double()
+                                             * state['m_scale'].double().repeat_interleave(256)),
+                                     _single(state['v'].view(torch.float8_e4m3fn).double()
+                                             * state['v_scale'].double().repeat_interleave(256))))
+        gd = g.double()
+        m = _single(_single(c[0] * m) + _single(c[1] * gd))
+        v = _single(_single(c[2] * _single(u * u)) + _single(_single(c[3] * gd) * gd))
+        u = _single(v.sqrt())
+        train.adamw_step([p], [g], state, k, **HYPER)
+        h = (i * 0x9E3779B9 + k * 0x6A09E667) & 0xffffffff
+        h = ((h ^ (h >> 15)) * 0xBB67AE85) & 0xffffffff
+        d = (h ^ (h >> 15)) >> 12
+        for x, key in ((m, 'm'), (u, 'v')):
+            top = x.abs().view(-1, 256).amax(1)
+            assert torch.equal(state[key + '_scale'].double(), _single(top * c[4])), key
+            t = _single(x.abs() * _single(_single(1 / top) * 448).repeat_interleave(256))
+            code = ((t.float().view(torch.int32).long() + d) >> 20) - 960
+            small = _single(t * 512 + d * 2.0 ** -20).long()
+            code = torch.where(t < 2.0 ** -6, small, code).clamp(max=126)
+            if key == 'v':
+                code = torch.where(t > 0, code.clamp(min=1), code)
+            code = torch.where((key == 'm') & x.signbit(), code + 128, code)
+            assert torch.equal(state[key].long(), code), key
+
+
 def test_adamw_8_moves_on_average(gpu):
     """A gradient of constant size takes v to its square though every step moves it by less than
     the grid's spacing, and the mean over many values comes within a few percent."""
@@ -600,3 +703,47 @@ def test_own_stream(gpu):
         got = step()
     s.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+def test_captured(gpu, to):
+    """A training step in a graph: every replay gives the eager step's bits, with other eager work
+    and new inputs between them."""
+    f = _randn(gpu, 13)
+    x, W, b = f(600, 300, to=to), f(264, 300, to=to, std=0.1), f(264, to=to)
+    t = torch.randint(0, 264, (600,), device=gpu)
+    w, c = W.clone(), b.clone()
+    state = train.adamw_state([w, c], 8)
+
+    def step():
+        y, z = train.linear(x, w, c, act='gelu', save=True)
+        loss, d = train.cross_entropy(y, t)
+        grads = train.linear_backward(d, x, w, z=z, act='gelu')
+        train.adamw_step([w, c], grads[1:], state, 1, lr=0.1)
+        return loss, grads[0]
+
+    def reset():
+        for p, q in ((w, W), (c, b)):
+            p.copy_(q)
+        for k in state:
+            if k != 'bits':
+                state[k].zero_()
+
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        step()
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(4):
+        x.copy_(f(600, 300, to=to))
+        t.copy_(torch.randint(0, 264, (600,), device=gpu))
+        reset()
+        want = [v.clone() for v in step()] + [w.clone(), c.clone()] + [
+            state[v].clone() for v in state if v != 'bits']
+        reset()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = list(out) + [w, c] + [state[v] for v in state if v != 'bits']
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), k

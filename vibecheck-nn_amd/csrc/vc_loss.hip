@@ -474,25 +474,25 @@ constexpr int64_t kCountRows = 1024;  // that every wave counts by itself
 // row's end lies in the last chunks of a thread, those past the limit before.
 template <class T>
 void run_loss(const Rows& a, hipStream_t st) {
-  const int64_t c = (a.V + Chunk<T>::kN - 1) / Chunk<T>::kN;
+  const auto fits = [&](int waves, int held) { return a.V <= 64ll * waves * held * Chunk<T>::kN; };
   if (a.V <= kFew) {
     if (a.R <= kOneRows) k_loss_few<T, kOneRows, true><<<1, kOneRows, 0, st>>>(a);
     else k_loss_few<T, 256, false><<<(unsigned)((a.R + 255) / 256), 256, 0, st>>>(a);
-  } else if (c <= 64) run_rows<T, 1, 1, 1>(a, st);
-  else if (c <= 128) run_rows<T, 1, 2, 1>(a, st);
-  else if (c <= 256) run_rows<T, 1, 4, 2>(a, st);
-  else if (c <= 512) run_rows<T, 4, 2, 1>(a, st);
-  else if (c <= 768) run_rows<T, 4, 3, 1>(a, st);
-  else if (c <= 1024) run_rows<T, 4, 4, 1>(a, st);
-  else if (c <= 1536) run_rows<T, 4, 6, 2>(a, st);
-  else if (c <= 2048) run_rows<T, 4, 8, 2>(a, st);
-  else if (c <= 3072) run_rows<T, 16, 3, 1>(a, st);
-  else if (c <= 4096) run_rows<T, 16, 4, 1>(a, st);
-  else if (c <= 6144) run_rows<T, 16, 6, 2>(a, st);
-  else if (c <= 8192) run_rows<T, 16, 8, 2>(a, st);
-  else if (c <= 10240) run_rows<T, 16, 10, 2>(a, st);
-  else if (c <= 13312) run_rows<T, 16, 13, 3>(a, st);
-  else if (c <= 16384) run_rows<T, 16, 16, 3>(a, st);
+  } else if (fits(1, 1)) run_rows<T, 1, 1, 1>(a, st);
+  else if (fits(1, 2)) run_rows<T, 1, 2, 1>(a, st);
+  else if (fits(1, 4)) run_rows<T, 1, 4, 2>(a, st);
+  else if (fits(4, 2)) run_rows<T, 4, 2, 1>(a, st);
+  else if (fits(4, 3)) run_rows<T, 4, 3, 1>(a, st);
+  else if (fits(4, 4)) run_rows<T, 4, 4, 1>(a, st);
+  else if (fits(4, 6)) run_rows<T, 4, 6, 2>(a, st);
+  else if (fits(4, 8)) run_rows<T, 4, 8, 2>(a, st);
+  else if (fits(16, 3)) run_rows<T, 16, 3, 1>(a, st);
+  else if (fits(16, 4)) run_rows<T, 16, 4, 1>(a, st);
+  else if (fits(16, 6)) run_rows<T, 16, 6, 2>(a, st);
+  else if (fits(16, 8)) run_rows<T, 16, 8, 2>(a, st);
+  else if (fits(16, 10)) run_rows<T, 16, 10, 2>(a, st);
+  else if (fits(16, 13)) run_rows<T, 16, 13, 3>(a, st);
+  else if (fits(16, 16)) run_rows<T, 16, 16, 3>(a, st);
   else run_rows<T, 16, 0, 0>(a, st);
 }
 
