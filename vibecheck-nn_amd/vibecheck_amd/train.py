@@ -7,12 +7,11 @@ allocates its outputs and workspace from torch and waits for nothing.  CPU tenso
 raise RuntimeError, other types NotImplementedError, sizes that do not fit
 ValueError.
 """
-import ctypes
 import math
 import operator
+from array import array
 
 import torch
-
 
 from ._lib import call, load, stream
 
@@ -308,7 +307,7 @@ def _one_type(tensors, sizes, what):
         raise ValueError(f'vibecheck_amd: {what} are contiguous, of one type, on one device and '
                          f'of their parameters\' sizes {sizes}; got '
                          f'{[(t.dtype, str(t.device), tuple(t.shape)) for t in tensors]}')
-    return k, list(map(_data_ptr, tensors))
+    return k, array('Q', map(_data_ptr, tensors))
 
 
 def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
@@ -340,20 +339,16 @@ def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8
         if t.dtype != want or t.numel() != (n if key[1:] else n * BLOCK) or \
                 t.get_device() != dev or not t.is_contiguous():
             raise ValueError(f'vibecheck_amd: state {key!r} does not fit these parameters')
-    array = ctypes.c_void_p * cnt
     if copies is not None:
         kc, pc = _one_type(copies, sizes, 'copies')
         if kc != 1:
             raise ValueError('vibecheck_amd: copies are bf16 tensors beside their parameters')
-        pc = array(*pc)
-    else:
-        pc = None
     if scale is not None and (scale.dtype != torch.float32 or scale.numel() != 1 or
                               scale.get_device() != dev):
         raise ValueError('vibecheck_amd: scale is one fp32 value on the parameters\' device')
-    pp, pg, pn = array(*pp), array(*pg), (ctypes.c_int64 * cnt)(*sizes)
-    call('vc_adamw_step', ctypes.addressof(pp), ctypes.addressof(pg),
-         ctypes.addressof(pc) if pc is not None else None, ctypes.addressof(pn), cnt, kp, kg, bits,
+    pn = array('q', sizes)
+    call('vc_adamw_step', pp.buffer_info()[0], pg.buffer_info()[0],
+         None if copies is None else pc.buffer_info()[0], pn.buffer_info()[0], cnt, kp, kg, bits,
          state['m'].data_ptr(), state['v'].data_ptr(), _ptr(state.get('m_scale')),
          _ptr(state.get('v_scale')), lr, betas[0], betas[1], eps, weight_decay, step, _ptr(scale),
          stream())
