@@ -560,17 +560,19 @@ struct Slope {
   uint16_t* parts; // or null
   float* sums;     // (blocks of rows, N), or null
   int64_t M;
-  int N, np, act, rows;
+  int N, np, act, rows, lanes;
 };
 
-constexpr int kSlopeCols = 256;  // of a workgroup: eight a thread, eight rows at a time
+// Lanes across a row, eight columns each; the workgroup's others take more rows.
+int slope_lanes(int N) { return N <= 64 ? 8 : N <= 128 ? 16 : 32; }
 
 template <class T>
 __device__ __forceinline__ void slope_block(const Slope<T>& a, int bx, int by) {
-  __shared__ float part[8][kSlopeCols + 8];
-  const int c = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const int j = bx * kSlopeCols + 8 * c;
-  const bool whole = (bx + 1) * kSlopeCols <= a.N;
+  __shared__ float part[LNT / 8 * 72];
+  const int cols = 8 * a.lanes, per = LNT / a.lanes, line = cols + 8;  // per: rows at a time
+  const int c = threadIdx.x & (a.lanes - 1), y = threadIdx.x / (unsigned)a.lanes;
+  const int j = bx * cols + 8 * c;
+  const bool whole = (bx + 1) * cols <= a.N;
   const int64_t m0 = (int64_t)by * a.rows;
   const int64_t m1 = m0 + a.rows < a.M ? m0 + a.rows : a.M;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -580,13 +582,13 @@ __device__ __forceinline__ void slope_block(const Slope<T>& a, int bx, int by) {
     float d[R][8], z[R][8];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      const int64_t r = m + 8 * q < m1 ? m + 8 * q : m;
+      const int64_t r = m + per * q < m1 ? m + per * q : m;
       load8(a.dy + r * a.ldy, j, a.N, whole, d[q]);
       if (a.act != kNone) load8(a.z + r * a.ldz, j, a.N, whole, z[q]);
     }
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      const int64_t r = m + 8 * q;
+      const int64_t r = m + per * q;
       if (r >= m1) break;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -602,21 +604,21 @@ __device__ __forceinline__ void slope_block(const Slope<T>& a, int bx, int by) {
     }
   };
   if (j < a.N) {
-    if (a.rows <= 8) {
+    if (a.rows <= per) {
       if (m0 + y < m1) take(m0 + y, std::integral_constant<int, 1>{});
     } else {
-      for (int64_t m = m0 + y; m < m1; m += 32) take(m, std::integral_constant<int, 4>{});
+      for (int64_t m = m0 + y; m < m1; m += 4 * per) take(m, std::integral_constant<int, 4>{});
     }
   }
   if (!a.sums) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) part[y][8 * c + i] = sum[i];
+  for (int i = 0; i < 8; ++i) part[y * line + 8 * c + i] = sum[i];
   __syncthreads();
-  const int k = bx * kSlopeCols + threadIdx.x;
-  if (k >= a.N) return;
+  const int k = bx * cols + threadIdx.x;
+  if ((int)threadIdx.x >= cols || k >= a.N) return;
   float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s += part[i][threadIdx.x];
+#pragma unroll 8
+  for (int i = 0; i < per; ++i) s += part[i * line + threadIdx.x];
   a.sums[(int64_t)by * a.N + k] = s;
 }
 
@@ -855,7 +857,7 @@ template <class T>
 void run_before(Slope<T> s, Pack<T> a, Pack<T> b, hipStream_t st) {
   const int64_t na = a.to ? div_up(a.rows * (a.np / 8), LNT) : 0;
   const int64_t nb = b.to ? div_up(b.rows * (b.np / 8), LNT) : 0;
-  const int cols = (int)div_up(s.N, kSlopeCols), ns = s.dy ? cols * (int)div_up(s.M, s.rows) : 0;
+  const int cols = s.dy ? (int)div_up(s.N, 8 * s.lanes) : 0, ns = s.dy ? cols * (int)div_up(s.M, s.rows) : 0;
   if (ns + na + nb > 0) k_before<T><<<(unsigned)(ns + na + nb), LNT, 0, st>>>(s, ns, cols, a, na, b);
 }
 
@@ -983,11 +985,12 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
   return VC_OK;
 }
 
-// Rows of a block of dz: eight, one a thread, while 256 blocks hold M (265 x 461 with
-// silu: 32 rows 8.6 us, eight 3.8), beyond that what 256 need.
-int slope_rows(int64_t M) {
-  const int64_t r = (M + 255) / 256;
-  return r <= 8 ? 8 : (int)(r < 32 ? 32 : r);
+// Rows of a block of dz: as many as its threads take at a time while 256 blocks hold M
+// (265 x 461 with silu: four a thread 8.6 us, one 3.8), beyond that what 256 need (4096
+// x 1024 by 512 blocks 18.5 us, by 256 15.9).
+int slope_rows(int64_t M, int N) {
+  const int64_t r = (M + 255) / 256, per = LNT / slope_lanes(N);
+  return (int)(r <= per ? per : r < 4 * per ? 4 * per : r);
 }
 
 struct BackwardPlan {
@@ -1020,7 +1023,7 @@ BackwardPlan make_backward(int type, int64_t M, int K, int N, int act, int need)
   }
   if (need & 2) p.w = c[0];
   if (need & 1) p.x = c[1];
-  p.rows = slope_rows(M);
+  p.rows = slope_rows(M, N);
   p.blocks = (int)div_up(M, p.rows);
   int64_t at = 0;
   if (need & 3) at += p.tiles ? parts_bytes(type, M, N) : act != kNone ? up256(e * M * N) : 0;
@@ -1076,6 +1079,7 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
   s.N = N;
   s.np = np;
   s.rows = p.rows;
+  s.lanes = slope_lanes(N);
   Pack<T> mw = {}, mx = {};
   if (p.tiles && dx && !as_it_is((const T*)W, K, K))
     mw = {(const T*)W, K, N, K, kp, (uint16_t*)(base + p.W)};
