@@ -745,21 +745,22 @@ constexpr int kGroups32 = 3, kGroups16 = 4;
 // (103 x 10768 x 12758 bf16, 277 MB: 64 x 64 in one slice 124 us, 128 x 128 in five 69;
 // fp32 64 x 8192 x 8192 in four slices 169, 104 and 103).
 Cost tile_cost(int type, int shape, bool far) {
-  constexpr float alone[2][2][3] = {{{2.0f, 1.06f, 0.8f}, {1.15f, 0.6f, 0.4f}},
-                                    {{2.0f, 1.06f, 0.88f}, {1.3f, 0.83f, 0.7f}}};
-  constexpr float shared[2][2][3] = {{{2.3f, 1.19f, 0.5f}, {1.6f, 0.47f, 0.17f}},
-                                     {{2.6f, 1.65f, 0.8f}, {2.0f, 0.95f, 0.38f}}};
-  constexpr int share[2][3] = {{1, 1, 3}, {1, 2, 4}};
-  constexpr float end[2][3] = {{6.8f, 3.8f, 0.5f}, {7.5f, 1.5f, 0.4f}};
+  constexpr float alone[2][2][4] = {{{2.0f, 1.06f, 0.8f}, {1.15f, 0.6f, 0.4f, 0.25f}},
+                                    {{2.0f, 1.06f, 0.88f}, {1.3f, 0.83f, 0.7f, 0.65f}}};
+  constexpr float shared[2][2][4] = {{{2.3f, 1.19f, 0.5f}, {1.6f, 0.47f, 0.17f, 0.3f}},
+                                     {{2.6f, 1.65f, 0.8f}, {2.0f, 0.95f, 0.38f, 0.38f}}};
+  constexpr int share[2][4] = {{1, 1, 2}, {1, 2, 4, 2}};
+  constexpr float end[2][4] = {{6.8f, 3.8f, 0.5f}, {7.5f, 1.5f, 0.4f, 0.4f}};
   const TileShape t = tile_shape(type, shape);
   const int b = type == VC_FP32 ? 0 : 1;
   return {t.bi, t.bj, t.bk, share[b][shape], alone[far][b][shape], shared[far][b][shape],
           end[b][shape]};
 }
 
-// Up to two products by the kernel and shape expected to be fastest.  extra: what
+// Up to two products by the kernel and shape expected to be fastest, of so many shapes
+// of tiles (0: tiles cannot be made).  extra: what
 // the tiles' parts cost before.
-float choose(int type, const Job* job, int n, bool products, bool tiles, float extra, Cut* out) {
+float choose(int type, const Job* job, int n, bool products, int tiles, float extra, Cut* out) {
   float least = 1e30f;
   const auto take = [&](Kernel k, int shape, const Cost& c, float more) {
     Grid g[2];
@@ -779,8 +780,7 @@ float choose(int type, const Job* job, int n, bool products, bool tiles, float e
   }
   far = far && bytes > (100 << 20);
   for (int shape = 0; shape < (products ? 2 : 0); ++shape) take(kProduct, shape, product_cost(type, shape), 0.f);
-  if (tiles)
-    for (int shape = 0; shape < 3; ++shape) take(kTile, shape, tile_cost(type, shape, far), extra);
+  for (int shape = 0; shape < tiles; ++shape) take(kTile, shape, tile_cost(type, shape, far), extra);
   return least;
 }
 
@@ -902,7 +902,7 @@ ForwardPlan make_forward(int type, int64_t M, int K, int N, bool raw) {
   p.c = cut_direct(type, M, N, K);
   Cut c = {};
   // bf16 goes by the tiles or directly: between them the other products gain nothing
-  choose(type, &job, 1, type == VC_FP32, tile_lines(K), pack, &c);
+  choose(type, &job, 1, type == VC_FP32, !tile_lines(K) ? 0 : type == VC_FP32 ? 3 : 4, pack, &c);
   if (c.us > 0.f && c.us < p.c.us) p.c = c;
   if (raw) {
     // two steps of 32 alone on a CU, and of each of two that share one (512 x 784 x
@@ -1013,7 +1013,7 @@ BackwardPlan make_backward(int type, int64_t M, int K, int N, int act, int need)
     const float pack = type == VC_FP32   ? pack_us(type, (M + N) * K + M * N / 5) - (act != kNone ? 4.f : 0.f)
                        : K % 8           ? pack_us(type, (M + N) * K) - (act != kNone ? 4.f : 0.f)
                                          : 0.f;
-    const bool can = tile_lines(K) && tile_lines(N);
+    const int can = tile_lines(K) && tile_lines(N) ? 3 : 0;
     const float one = choose(type, job, 2, true, can, pack, c);
     p.tiles = c[0].kernel == kTile;
     // or a launch each, in a shape of its own

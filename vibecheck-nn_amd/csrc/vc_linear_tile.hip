@@ -243,17 +243,23 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
   constexpr int kLoads = NP * (SA::kOwn + SB::kOwn), AHEAD = NBUF - 1;
   if (full > 0) {
     if constexpr (!TURNS) {
-      static_assert(NBUF == 2);
-      load(0, lds);
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s)
+        if (s < full) load(s, lds + s * kStage);
+      int at = 0;  // this step's buffer
 #pragma unroll 1
       for (int s = 0; s < full; ++s) {
-        __syncthreads();  // this step has arrived, the buffer of the one before is read
-        if (s + 1 < full) load(s + 1, lds + ((s + 1) & 1) * kStage);
+        // this step has arrived, the buffer of the one before is read
+        if (s + AHEAD <= full) wait_for<(AHEAD - 1) * kLoads, true>();
+        else wait_for<0, true>();
+        turn();
+        if (s + AHEAD < full) load(s + AHEAD, lds + (at == 0 ? NBUF - 1 : at - 1) * kStage);
 #pragma unroll
         for (int ks = 0; ks < BK / 32; ++ks) {
-          read(lds + (s & 1) * kStage, ks);
+          read(lds + at * kStage, ks);
           multiply();
         }
+        at = at == NBUF - 1 ? 0 : at + 1;
       }
     } else {
       // Waves wv and wv + 4 share a SIMD; the later ones run a turn behind.  A
@@ -392,7 +398,11 @@ struct Form {
   static constexpr bool TURNS = SHAPE == 0 || (F && SHAPE == 1);
   static constexpr int WI = F && SHAPE == 0 ? 4 : 2, WJ = (TURNS ? 8 : 4) / WI;
   static constexpr int BK = F ? 32 : 64;
-  static constexpr int NBUF = F && SHAPE == 1 ? 3 : 2;
+  // 64 x 64 in bf16 has two buffers, so that four workgroups share a CU (2048 cubed,
+  // backward's dW, 27 us; with four buffers and two workgroups 44), or as shape 3 four of
+  // them for few workgroups whose operands come from far (20 x 12480 x 2624 14 us; with two
+  // 20); fp32 has three (1024 cubed 22 us; with two 24)
+  static constexpr int NBUF = F && SHAPE > 0 ? 3 : SHAPE == 3 ? 4 : 2;
   static constexpr int kThreads = 64 * WI * WJ;
   static constexpr int kLds = NBUF * NP * (BI + BJ) * BK * 2;
   template <bool XA, bool XB>
@@ -558,7 +568,8 @@ template <class T>
 void run_tile(const Product<T>& a, int shape, hipStream_t st) {
   if (shape == 0) one<T, 0>(a, st);
   else if (shape == 1) one<T, 1>(a, st);
-  else one<T, 2>(a, st);
+  else if (sizeof(T) == 4 || shape == 2) one<T, 2>(a, st);
+  else if constexpr (sizeof(T) == 2) one<T, 3>(a, st);
 }
 template <class T>
 void run_tiles(const Product<T>& w, const Product<T>& x, const Columns<T>& c, int shape,
