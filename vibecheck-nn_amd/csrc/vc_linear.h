@@ -122,8 +122,8 @@ struct Product {
 };
 
 // The tiled products of vc_linear_tile.hip, shapes 0, 1, 2: 256 x 256 (fp32 256 x
-// 128), 128 x 128, 64 x 64; 3, bf16 forward alone: 64 x 64, loaded three steps ahead.  Rows (across: k) lie lda, ldb
-// values apart.  The caller has seen to it that every operand's base and ld are
+// 128), 128 x 128, 64 x 64; 3, bf16 forward alone: 64 x 64, loaded three steps ahead.
+// Rows (across: k) lie lda, ldb values apart.  The caller has seen to it that every operand's base and ld are
 // multiples of 16 bytes, that K is a multiple of eight (an operand whose k is
 // contiguous) or its lines are padded to one (read across), and that 256 of them
 // span less than 2^31 bytes.

@@ -171,7 +171,9 @@ __device__ __forceinline__ void unit_row(const Raw<T>& v, int r, u4* o) {
 // multiplied, then laid into the other of the group's two LDS buffers: [k
 // step][part][row][four 16-byte chunks], chunk c of row r at c ^ (r / 2 mod 4), so
 // that a fragment read meets every bank evenly.  The columns' fragment is the
-// matrix step's first operand: a lane holds four consecutive columns of one row.
+// matrix step's first operand: a lane holds four consecutive columns of one row.  fp32:
+// the five small part products run on in an accumulator of their own, the largest
+// starts from zero each step and is added in fp32.
 constexpr int kTileSide = 64;
 template <class T>
 constexpr int product_lds(int groups) {  // bytes
@@ -550,8 +552,11 @@ __device__ __forceinline__ void pack_block(const Pack<T>& m, int64_t block) {
   store_parts<T>(v, m.to + row * m.np + j, m.rows * m.np);
 }
 
-// dz = dy act'(z), and the columns' sums of each block of rows.  dz as values, or
-// as parts for the tiled products (lines of np values, zeros past N).
+// dz = dy act'(z), and the columns' sums of each block of rows, from dz in fp32.  dz as
+// values, or as parts for the tiled products (lines of np values, zeros past N).  In
+// bf16 it is rounded here: the matrix cores multiply bf16 with nothing wider, and parts
+// of dz would cost two or three times the products (dx, dW 2.3e-3 of their norm off,
+// 1.7e-3 of it the rounding of the result).
 template <class T>
 struct Slope {
   const T *dy, *z;

@@ -1,8 +1,8 @@
-// The fc layer's large products: tiles of 64 x 64 to 256 x 256 (fp32 256 x 128), both operands as bf16
-// (an fp32 value as three parts, vc_linear.hip) brought into LDS by loads that
-// pass no register.
+// The fc layer's large products: tiles of 64 x 64 to 256 x 256 (fp32 256 x 128), both
+// operands as bf16 (an fp32 value as three parts, vc_linear.hip) brought into LDS by
+// loads that pass no register.
 //
-// A step of BK goes into one of two or three LDS buffers while another is
+// A step of BK goes into one of two to four LDS buffers while another is
 // multiplied.  A load instruction writes 1 KB of LDS in lane order, so the order
 // that spreads a fragment's reads over the banks is made by which address each
 // lane reads from:
@@ -15,7 +15,10 @@
 // each SIMD, read their next fragments; a barrier ends each turn.  256 x 256 by
 // waves of 128 x 64: a turn of 32 products deep is 512 cycles of matrix
 // instructions on each SIMD beside 48 KB of fragment reads and 16 KB of loads into
-// LDS, at 128 bytes a cycle 512 as well.
+// LDS, at 128 bytes a cycle 512 as well.  8192 x 4096 x 16384 bf16 with gelu: 900 us,
+// 1222 TFLOP/s, the matrix units busy in 58% of the cycles at the 2.0 GHz that the
+// card's power leaves of 2.4; constant operands, which switch less, 770 us.  fp32
+// 4096 x 4096 x 4096 572 to 659 us (random operands), 209 to 240 TFLOP/s.
 #include "vc_linear.h"
 
 namespace {
@@ -324,8 +327,10 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
   }
 
   // The sums go through LDS, as many rows as fit: what follows them (bias,
-  // activation, residual, stores of whole lines) is one short loop.  Four columns
-  // c of row i at c ^ (i mod 16).
+  // activation, residual, stores of whole lines) is one short loop, eight rows of a
+  // thread's four columns at a time (four where half of the sums stay in registers
+  // meanwhile).  One after another, each waiting for its own loads, took 14 us of a 256
+  // x 256 tile, this takes 5.  Four columns c of row i at c ^ (i mod 16).
   constexpr int Q = BJ / 4, kFit = NBUF * kStage / (BJ * 4), ROWS = kFit < BI ? BI / WI : BI;
   static_assert(ROWS <= kFit && Q >= 16);
   constexpr int STEP = 64 * NW / Q, U = ROWS < BI ? 4 : ROWS / STEP < 8 ? ROWS / STEP : 8;
