@@ -209,9 +209,9 @@ __device__ void plain_row(const Rows& a, const T* z, T* dz, int64_t t, float zt,
 // every term, the largest's own (em) too, and cancels.  The target's term is kept
 // apart (its place holds -inf meanwhile).
 //
-// Memory bounds it: 8,192 x 131,072 bf16, logits read and gradient written, 877 us
-// (4.9 TB/s; read twice, as the first kernel did, 2,726); 999 x 50,021 fp32 rows that
-// no 16 bytes divide, 100 us (4.0).  A team is as small as holds its row in at most 16
+// Memory bounds it: 8,192 x 131,072 bf16, logits read and gradient written, 804 us
+// (5.3 TB/s), smoothed 853; read twice, as the first kernel did, 2,726.  1000 x 50,021
+// fp32 rows that no 16 bytes divide, 91 us (4.4).  A team is as small as holds its row in at most 16
 // chunks a thread: what a smaller one saves is the joins across waves, what a larger
 // one saves is registers, of which 16 chunks leave a CU two teams.
 template <class T, int W, int NV, int ENDS, bool SMOOTH>
@@ -273,7 +273,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
 #pragma unroll
         for (int i = 0; i < N; ++i) half += (int64_t)c * N + i < a.V ? C::value(w, i) * iv : 0.f;
       }
+      // the values are unpacked again for the sum below, not kept beside these: with three
+      // times the registers chunks would spill
       asm volatile("" : "+v"(half));
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" : "+v"(w));
     }
     if (c == ct) w = C::none_at(w, (int)(t - (int64_t)ct * N));
     float top = C::value(w, 0);
@@ -335,7 +339,6 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
       for (int i = 0; i < N; ++i)
         if ((int64_t)c * N + i < a.V) store1(dz + (int64_t)c * N + i, g[i]);
     }
-    if (c == ct) store1(dz + t, at_t);
   };
   if (NV) {
     each(held, [&](auto k) {
@@ -352,6 +355,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
       });
     }
   }
+  // its own place, over what the chunk left there, by the same thread
+  if (valid && tid == (int)(ct % TH)) store1(dz + t, at_t);
 }
 
 // Few classes: a thread a row, its values from the caches for each of its passes.
