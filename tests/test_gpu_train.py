@@ -363,6 +363,24 @@ def test_cross_entropy_where_the_team_changes(gpu, to, held):
 
 
 @pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('V', [33, 333, 4097, 50021, 140001])
+def test_cross_entropy_first_value(gpu, to, V):
+    """Rows that begin at odd places, whose first value is the target, the largest, masked, NaN."""
+    z = _randn(gpu, V)(8, V, to=to, std=3.0)
+    t = torch.tensor([0, 0, 1, 0, 5, V - 1, -100, 2], device=gpu)
+    _check_loss(z, t)
+    _check_loss(z, t, 0.1)
+    z[3, 0], z[5, 0] = 300.0, 300.0   # the target, another
+    _check_loss(z, t)
+    _check_loss(z, t, 0.1)
+    z[1, 0], z[7, 0] = -math.inf, -math.inf
+    _check_loss(z, t)
+    z[3], z[5, 1:] = -math.inf, -math.inf
+    z[7, 0] = math.nan
+    _check_loss(z, t)
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
 @pytest.mark.parametrize('V', [8, 300, 5000, 140000])
 def test_cross_entropy_masks(gpu, to, V):
     """Masked classes, rows that masks leave empty, the type's lowest value, infinities, NaN,

@@ -209,8 +209,8 @@ __device__ void plain_row(const Rows& a, const T* z, T* dz, int64_t t, float zt,
 // every term, the largest's own (em) too, and cancels.  The target's term is kept
 // apart (its place holds -inf meanwhile).
 //
-// Memory bounds it: 8,192 x 131,072 bf16, logits read and gradient written, 804 us
-// (5.3 TB/s), smoothed 853; read twice, as the first kernel did, 2,726.  1000 x 50,021
+// Memory bounds it: 8,192 x 131,072 bf16, logits read and gradient written, 760 us
+// (5.6 TB/s), x 50,021 343 (4.8); read twice, as the first kernel did, 2,726.  1000 x 50,021
 // fp32 rows that no 16 bytes divide, 91 us (4.4).  A team is as small as holds its row in at most 16
 // chunks a thread: what a smaller one saves is the joins across waves, what a larger
 // one saves is registers, of which 16 chunks leave a CU two teams.
@@ -228,19 +228,26 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
   const T* const z = (const T*)a.z + row * a.ld;
   T* const dz = a.dz ? (T*)a.dz + row * a.ldd : nullptr;
   const int64_t t = a.t[row];
+  // a bf16 row at an odd place: its first value goes by itself, the chunks start at a
+  // multiple of four bytes (8192 x 50021 498 us without, 343 with)
+  const int h = sizeof(T) == 2 && ((uintptr_t)z & 2) ? 1 : 0;
+  const T* const zh = z + h;
+  T* const dzh = dz + h;
+  const int64_t V = a.V - h;
   // chunks; what is left over belongs to chunk `whole`
-  const Index whole = (Index)(a.V / N), chunks = (Index)((a.V + N - 1) / N);
+  const Index whole = (Index)(V / N), chunks = (Index)((V + N - 1) / N);
   if (t == a.ignore) {
     if (tid == 0) a.loss[row] = 0.f;
     if (dz) {
-      for (int64_t c = tid; c < whole; c += TH) C::store(dz + c * N, u4{0, 0, 0, 0});
-      for (int64_t j = whole * N + tid; j < a.V; j += TH) store1(dz + j, 0.f);
+      for (int64_t c = tid; c < whole; c += TH) C::store(dzh + c * N, u4{0, 0, 0, 0});
+      for (int64_t j = whole * N + tid; j < V; j += TH) store1(dzh + j, 0.f);
+      if (h && tid == 0) store1(dz, 0.f);
     }
     return;
   }
   const bool valid = t >= 0 && t < a.V;
-  const float zt = load1(z + (valid ? t : 0)), iv = 0.5f / (float)a.V;
-  const Index ct = valid ? (Index)(t / N) : -1;
+  const float zt = load1(z + (valid ? t : 0)), z0 = load1(z), iv = 0.5f / (float)a.V;
+  const Index ct = valid && t >= h ? (Index)((t - h) / N) : -1;
   const auto at = [](auto* p, Index c) {
     typedef std::remove_pointer_t<decltype(p)> P;
     if constexpr (NV != 0) return p + (uint32_t)c * (uint32_t)N;
@@ -249,11 +256,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
   // Every lane loads a whole chunk, one that would pass the row's end the row's
   // last: a branch that lanes do not share would have each load waited for before
   // the next.  What is not the chunk's own is masked when it is taken.
-  const Index last = (Index)(a.V - N);
+  const Index last = (Index)(V - N);
   const auto fetch = [&](Index c) {
     const Index e = c < whole ? c * N : last;
-    if constexpr (NV != 0) return C::load(z + (uint32_t)e);
-    else return C::load(z + e);
+    if constexpr (NV != 0) return C::load(zh + (uint32_t)e);
+    else return C::load(zh + e);
   };
   // Of chunks first .. first + TH - 1, that of this lane: a part of one is moved to
   // its front, the rest is -inf.
@@ -271,7 +278,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
         for (int i = 0; i < N; ++i) half += C::value(w, i) * iv;
       } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) half += (int64_t)c * N + i < a.V ? C::value(w, i) * iv : 0.f;
+        for (int i = 0; i < N; ++i) half += (int64_t)c * N + i < V ? C::value(w, i) * iv : 0.f;
       }
       // the values are unpacked again for the sum below, not kept beside these: with three
       // times the registers chunks would spill
@@ -279,7 +286,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
       __builtin_amdgcn_sched_barrier(0);
       asm volatile("" : "+v"(w));
     }
-    if (c == ct) w = C::none_at(w, (int)(t - (int64_t)ct * N));
+    if (c == ct) w = C::none_at(w, (int)(t - h - (int64_t)ct * N));
     float top = C::value(w, 0);
 #pragma unroll
     for (int i = 1; i < N; ++i) top = fmaxf(top, C::value(w, i));
@@ -308,6 +315,18 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
       each(held, [&](auto k) { take(v[k], c + tid + k * TH, c + k * TH, true); });
     }
   }
+  if (h && tid == 0) {
+    if (SMOOTH) half += z0 * iv;
+    if (t != 0) {
+      if (z0 > m) {
+        m = z0;
+        const float to = fmaxf(ceilf(m * kLog2e), r);
+        s *= __builtin_amdgcn_exp2f(r - to);
+        r = to;
+      }
+      s += __builtin_amdgcn_exp2f(__builtin_fmaf(z0, kLog2e, -r));
+    }
+  }
   const float w = scale_of(a, lane);
   const float top = team.max_of(fmaxf(m, zt));
   if (!(fabsf(top) < 1e38f)) {  // the same in every thread of the row
@@ -324,20 +343,21 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
   if (!dz) return;
   const float inv = valid ? w / (s + et) : NAN, ev = a.smooth / (float)a.V * w;
   const float at_t = a.smooth * w - s * inv - ev;
+  const auto grad = [&](float x) {
+    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, -r));
+    return SMOOTH ? __builtin_fmaf(p, inv, -ev) : p * inv;
+  };
   const auto give = [&](u4 x, Index c, bool end) {
     asm volatile("" : "+v"(x));  // unpacked again here, not kept from before: twice the registers
     float g[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(C::value(x, i), kLog2e, -r));
-      g[i] = SMOOTH ? __builtin_fmaf(p, inv, -ev) : p * inv;
-    }
+    for (int i = 0; i < N; ++i) g[i] = grad(C::value(x, i));
     if (!end || c < whole) {
-      C::store(at(dz, c), C::pack(g));
+      C::store(at(dzh, c), C::pack(g));
     } else if (c == whole) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if ((int64_t)c * N + i < a.V) store1(dz + (int64_t)c * N + i, g[i]);
+        if ((int64_t)c * N + i < V) store1(dzh + (int64_t)c * N + i, g[i]);
     }
   };
   if (NV) {
@@ -355,8 +375,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
       });
     }
   }
+  if (h && tid == 0) store1(dz, valid && t == 0 ? at_t : grad(z0));
   // its own place, over what the chunk left there, by the same thread
-  if (valid && tid == (int)(ct % TH)) store1(dz + t, at_t);
+  if (ct >= 0 && tid == (int)(ct % TH)) store1(dz + t, at_t);
 }
 
 // Few classes: a thread a row, its values from the caches for each of its passes.
