@@ -54,11 +54,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2bf));
 }
 
-// Values i .. i + 3 of n; past the end zero.
-template <bool VEC>
+// At any alignment of the type.
+typedef float v4fat4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u2at2 __attribute__((ext_vector_type(2), aligned(2)));
+
+// Values i .. i + 3 of n; past the end zero (WHOLE: none is).
+template <bool WHOLE>
 __device__ __forceinline__ void load4(const float* p, int64_t i, int64_t n, float* o) {
-  if (VEC) {
-    const v4f w = *reinterpret_cast<const v4f*>(p + i);
+  if (WHOLE) {
+    const v4fat4 w = *reinterpret_cast<const v4fat4*>(p + i);
 #pragma unroll
     for (int q = 0; q < 4; ++q) o[q] = w[q];
   } else {
@@ -66,10 +70,10 @@ __device__ __forceinline__ void load4(const float* p, int64_t i, int64_t n, floa
     for (int q = 0; q < 4; ++q) o[q] = i + q < n ? p[i + q] : 0.f;
   }
 }
-template <bool VEC>
+template <bool WHOLE>
 __device__ __forceinline__ void load4(const uint16_t* p, int64_t i, int64_t n, float* o) {
-  if (VEC) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p + i);
+  if (WHOLE) {
+    const u2at2 w = *reinterpret_cast<const u2at2*>(p + i);
     o[0] = up((uint16_t)w.x);
     o[1] = __builtin_bit_cast(float, w.x & 0xffff0000u);
     o[2] = up((uint16_t)w.y);
@@ -79,20 +83,20 @@ __device__ __forceinline__ void load4(const uint16_t* p, int64_t i, int64_t n, f
     for (int q = 0; q < 4; ++q) o[q] = i + q < n ? up(p[i + q]) : 0.f;
   }
 }
-template <bool VEC>
+template <bool WHOLE>
 __device__ __forceinline__ void store4(float* p, int64_t i, int64_t n, const float* v) {
-  if (VEC) {
-    *reinterpret_cast<v4f*>(p + i) = v4f{v[0], v[1], v[2], v[3]};
+  if (WHOLE) {
+    *reinterpret_cast<v4fat4*>(p + i) = v4fat4{v[0], v[1], v[2], v[3]};
   } else {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       if (i + q < n) p[i + q] = v[q];
   }
 }
-template <bool VEC>
+template <bool WHOLE>
 __device__ __forceinline__ void store4(uint16_t* p, int64_t i, int64_t n, const float* v) {
-  if (VEC) {
-    *reinterpret_cast<uint2*>(p + i) = uint2{pack2(v[0], v[1]), pack2(v[2], v[3])};
+  if (WHOLE) {
+    *reinterpret_cast<u2at2*>(p + i) = u2at2{pack2(v[0], v[1]), pack2(v[2], v[3])};
   } else {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -162,13 +166,13 @@ __device__ __forceinline__ float update8(float p, float g, float& m, float& v, c
                         __builtin_amdgcn_rcpf(__builtin_fmaf(v, a.inv_bc2, a.c.eps)), p);
 }
 
-template <class P, class G, int BITS, bool VEC>
+template <class P, class G, int BITS, bool WHOLE>
 __device__ __forceinline__ void step_block(const Step& a, const Tensor& t, int64_t blk, int lane,
                                            float gs) {
   const int64_t i = blk * kBlock + 4 * lane, at = (t.b0 + blk) * kBlock + 4 * lane;
   float p[4], g[4], m[4], v[4];
-  load4<VEC>((const P*)t.p, i, t.n, p);
-  load4<VEC>((const G*)t.g, i, t.n, g);
+  load4<WHOLE>((const P*)t.p, i, t.n, p);
+  load4<WHOLE>((const G*)t.g, i, t.n, g);
   if (BITS == 32) {
     load4<true>((const float*)a.m, at, 0, m);
     load4<true>((const float*)a.v, at, 0, v);
@@ -184,8 +188,8 @@ __device__ __forceinline__ void step_block(const Step& a, const Tensor& t, int64
     if (BITS == 32) p[q] = adam_update(p[q] * a.decay, g[q], m[q], v[q], a.c);
     else p[q] = update8(p[q] * a.decay, g[q], m[q], v[q], a);
   }
-  store4<VEC>((P*)t.p, i, t.n, p);
-  if (t.c) store4<VEC>(t.c, i, t.n, p);
+  store4<WHOLE>((P*)t.p, i, t.n, p);
+  if (t.c) store4<WHOLE>(t.c, i, t.n, p);
   if (BITS == 32) {
     store4<true>((float*)a.m, at, 0, m);
     store4<true>((float*)a.v, at, 0, v);
@@ -221,13 +225,11 @@ __global__ __launch_bounds__(ANT) void k_adamw(Step a) {
   }
   const Tensor t = a.t[lo];
   const int64_t blocks = (t.n + kBlock - 1) / kBlock;
-  const bool vec = ((uintptr_t)t.p & (4 * sizeof(P) - 1)) == 0 &&
-                   ((uintptr_t)t.g & (4 * sizeof(G) - 1)) == 0 && ((uintptr_t)t.c & 7) == 0;
   const int64_t b = (int64_t)(w - a.w0[lo]) * kBlocksPerWg;
   for (int k = wv; k < kBlocksPerWg; k += ANT / 64) {
     const int64_t blk = b + k;
     if (blk >= blocks) break;
-    if (vec && (blk + 1) * kBlock <= t.n) step_block<P, G, BITS, true>(a, t, blk, lane, gs);
+    if ((blk + 1) * kBlock <= t.n) step_block<P, G, BITS, true>(a, t, blk, lane, gs);
     else step_block<P, G, BITS, false>(a, t, blk, lane, gs);
   }
 }
