@@ -1131,6 +1131,7 @@ int vc_mlp_bab_round(const int32_t *dims, int n_relu, const float *frag,
 #define VC_ACT_RELU 1
 #define VC_ACT_GELU 2 /* z (1 + erf(z / sqrt 2)) / 2 */
 #define VC_ACT_SILU 3 /* z / (1 + exp(-z)) */
+#define VC_DZ_ROUNDED 16 /* of the backward, or'ed to its act: see there */
 #define VC_REDUCE_NONE 0
 #define VC_REDUCE_SUM 1
 #define VC_REDUCE_MEAN 2
@@ -1146,8 +1147,10 @@ int vc_linear(int type, const void *x, int64_t M, int K, int64_t ldx,
 
 /* Its gradients: dz = dy act'(z) (z is not read without an activation),
  * dx = dz W (M, K), dW = dz^T x (N, K), db = column sums of dz (N), each
- * unless NULL (need: 1 dx, 2 dW, 4 db).  In bf16 dz is rounded before the
- * products, not before its sums. */
+ * unless NULL (need: 1 dx, 2 dW, 4 db).  dz keeps 16 bits or more in the
+ * products (in bf16 with GELU or SiLU at twice their work) unless act has
+ * VC_DZ_ROUNDED, with which a bf16 dz is rounded before them; db is the sum
+ * of what is not rounded. */
 int64_t vc_linear_backward_workspace(int type, int64_t M, int K, int N,
                                      int act, int need);
 int vc_linear_backward(int type, const void *dy, int64_t ldy, const void *x,

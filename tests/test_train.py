@@ -90,3 +90,18 @@ def test_workspaces():
     # a workspace too small is refused, not overrun
     with pytest.raises(torch.cuda.OutOfMemoryError):
         _lib.call('vc_cross_entropy', 0, P, 4, 10, 10, P, -100, 0.0, 2, P, None, 0, P, 8, None)
+
+
+def test_backward_of_a_rounded_dz():
+    """The flag belongs to the backward's activation; a dz in two parts needs the more room."""
+    lib = _lib.load()
+    for act in (2, 3):
+        assert lib.vc_linear_backward_workspace(1, 64, 64, 64, act | 16, 7) < \
+            lib.vc_linear_backward_workspace(1, 64, 64, 64, act, 7)
+    for act in (0, 1):
+        assert lib.vc_linear_backward_workspace(1, 64, 64, 64, act | 16, 7) == \
+            lib.vc_linear_backward_workspace(1, 64, 64, 64, act, 7)
+    assert lib.vc_linear_backward_workspace(1, 64, 64, 64, 32, 7) < 0
+    assert lib.vc_linear_backward_workspace(1, 64, 64, 64, 4 | 16, 7) < 0
+    with pytest.raises(ValueError):
+        _lib.call('vc_linear', 0, P, 4, 4, 4, P, 5, None, 1 | 16, None, 0, P, None, None, 0, None)

@@ -530,42 +530,79 @@ __device__ __forceinline__ void store_parts(const float* v, uint16_t* to, int64_
   }
 }
 
+// Eight fp32 values as 16 bytes of each of two bf16 parts, the first cut (store_parts
+// has three): 2^-16 of a value is lost.  An infinity or NaN stands in the first alone.
+__device__ __forceinline__ void store_two(const float* v, uint16_t* to, int64_t plane) {
+  u4 h, l;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t b0 = __builtin_bit_cast(uint32_t, v[2 * q]), b1 = __builtin_bit_cast(uint32_t, v[2 * q + 1]);
+    h[q] = __builtin_amdgcn_perm(b1, b0, 0x07060302);
+    l[q] = bf_pack(finite(v[2 * q]) ? v[2 * q] - bf_hi(b0) : 0.f,
+                   finite(v[2 * q + 1]) ? v[2 * q + 1] - bf_hi(b1) : 0.f);
+  }
+  *reinterpret_cast<u4*>(to) = h;
+  *reinterpret_cast<u4*>(to + plane) = l;
+}
+
 // Up to two matrices as parts for the tiled products, their lines padded with
 // zeros to a multiple of eight.
 template <class T>
 struct Pack {
   const T* p;
   int64_t ld, rows;
-  int n, np;  // values of a line, and with its padding
+  int n, np;      // values of a line, and with its padding
   uint16_t* to;
+  int64_t line;   // from one line written to the next
+  int64_t lines;  // with those of zeros behind the rows
+  int64_t again;  // bf16: from a line to its second copy, zeros for what is not finite, or 0
 };
+template <class T>
+Pack<T> pack_of(const void* p, int64_t ld, int64_t rows, int n, int np, void* to) {
+  return {(const T*)p, ld, rows, n, np, (uint16_t*)to, np, rows, 0};
+}
 
 template <class T>
 __device__ __forceinline__ void pack_block(const Pack<T>& m, int64_t block) {
   const int64_t t = block * LNT + threadIdx.x;
   const int c = m.np / 8;
   const int64_t row = t / c;
-  if (row >= m.rows) return;
+  if (row >= m.lines) return;
   const int j = (int)(t - row * c) * 8;
-  float v[8];
-  load8(m.p + row * m.ld, j, m.n, j + 8 <= m.n, v);
-  store_parts<T>(v, m.to + row * m.np + j, m.rows * m.np);
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (row < m.rows) load8(m.p + row * m.ld, j, m.n, j + 8 <= m.n, v);
+  uint16_t* const to = m.to + row * m.line + j;
+  store_parts<T>(v, to, m.rows * m.np);
+  if constexpr (sizeof(T) == 2) {
+    if (!m.again) return;
+    // dz's second parts meet this copy: they add nothing to an infinity or NaN
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = finite(v[q]) ? v[q] : 0.f;
+    store_parts<T>(v, to + m.again, 0);
+  }
 }
 
 // dz = dy act'(z), and the columns' sums of each block of rows, from dz in fp32.  dz as
-// values, or as parts for the tiled products (lines of np values, zeros past N).  In
-// bf16 it is rounded here: the matrix cores multiply bf16 with nothing wider, and parts
-// of dz would cost two or three times the products (dx, dW 2.3e-3 of their norm off,
-// 1.7e-3 of it the rounding of the result).
+// values, or as parts for the tiled products (lines of np values, zeros past N).
+//
+// The matrix cores multiply bf16 with nothing wider, and in bf16 the dz of GELU and SiLU
+// has more bits than that (ReLU's and none's are dy's own).  So it is two parts, and
+// the products are those of a sum twice as long: a row of dz is its h and then its l,
+//   dx[m] = [h_m l_m] [W; W],   dW = sum over lines h_0, l_0, h_1, .. times x_0, x_0, x_1, ..
+// with W and x copied so by the pass before.  Twice the products' work for dx and dW 1.7e-3 of
+// their norm off, which is the rounding of the result, instead of 2.3e-3 with dz rounded;
+// a caller who prefers the time asks for that (VC_DZ_ROUNDED).
 template <class T>
 struct Slope {
   const T *dy, *z;
   int64_t ldy, ldz;
   T* dz;           // lines of N, or null
   uint16_t* parts; // or null
+  int64_t line, plane;  // of the parts: from a row to the next, from a part to the next
   float* sums;     // (blocks of rows, N), or null
   int64_t M;
-  int N, np, act, rows, lanes;
+  int N, act, rows, lanes;
+  bool two;        // bf16 in two parts
 };
 
 // Lanes across a row, eight columns each; the workgroup's others take more rows.
@@ -600,7 +637,11 @@ __device__ __forceinline__ void slope_block(const Slope<T>& a, int bx, int by) {
         if (a.act != kNone) d[q][i] *= slope(z[q][i], a.act);
         sum[i] += d[q][i];
       }
-      if (a.parts) store_parts<T>(d[q], a.parts + r * a.np + j, a.M * a.np);
+      if (a.parts) {
+        uint16_t* const to = a.parts + r * a.line + j;
+        if (sizeof(T) == 2 && a.two) store_two(d[q], to, a.plane);
+        else store_parts<T>(d[q], to, a.plane);
+      }
       if (a.dz) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -860,8 +901,8 @@ void run_join(const Product<T>& a, const Product<T>& b, const Columns<T>& c, hip
 
 template <class T>
 void run_before(Slope<T> s, Pack<T> a, Pack<T> b, hipStream_t st) {
-  const int64_t na = a.to ? div_up(a.rows * (a.np / 8), LNT) : 0;
-  const int64_t nb = b.to ? div_up(b.rows * (b.np / 8), LNT) : 0;
+  const int64_t na = a.to ? div_up(a.lines * (a.np / 8), LNT) : 0;
+  const int64_t nb = b.to ? div_up(b.lines * (b.np / 8), LNT) : 0;
   const int cols = s.dy ? (int)div_up(s.N, 8 * s.lanes) : 0, ns = s.dy ? cols * (int)div_up(s.M, s.rows) : 0;
   if (ns + na + nb > 0) k_before<T><<<(unsigned)(ns + na + nb), LNT, 0, st>>>(s, ns, cols, a, na, b);
 }
@@ -954,8 +995,8 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
   if (p.c.kernel == kTile) {
     const int kp = (int)up8(K);
     Pack<T> px = {}, pw = {};
-    if (!as_it_is((const T*)x, ldx, K)) px = {(const T*)x, ldx, M, K, kp, (uint16_t*)(base + p.x)};
-    if (!as_it_is((const T*)W, K, K)) pw = {(const T*)W, K, N, K, kp, (uint16_t*)(base + p.W)};
+    if (!as_it_is((const T*)x, ldx, K)) px = pack_of<T>(x, ldx, M, K, kp, base + p.x);
+    if (!as_it_is((const T*)W, K, K)) pw = pack_of<T>(W, K, N, K, kp, base + p.W);
     run_before<T>({}, px, pw, st);
     a.pa = px.to ? px.to : (const uint16_t*)x;
     a.lda = px.to ? kp : ldx;
@@ -998,8 +1039,14 @@ int slope_rows(int64_t M, int N) {
   return (int)(r <= per ? per : r < 4 * per ? 4 * per : r);
 }
 
+// Whether the products take dz in two parts (slope_block), by act as the caller gave it.
+constexpr int kRounded = VC_DZ_ROUNDED;
+bool two_parts(int type, int act, int need) {
+  return type == VC_BF16 && (act == kGelu || act == kSilu) && (need & 3);
+}
+
 struct BackwardPlan {
-  bool tiles;
+  bool tiles, two;
   Cut x, w;
   int rows, blocks;
   int64_t dz, W, in, sums, px, pw, bytes;  // offsets in the workspace, and its size
@@ -1008,17 +1055,21 @@ struct BackwardPlan {
 BackwardPlan make_backward(int type, int64_t M, int K, int N, int act, int need) {
   BackwardPlan p = {};
   const int64_t e = type == VC_FP32 ? 4 : 2;
+  p.two = two_parts(type, act, need);
+  act &= ~kRounded;
+  const int64_t np = up8(N), times = p.two ? 2 : 1;
   Job job[2];
   Cut c[2] = {};
   // for both products, whichever are asked for: the same bits either way
-  job[0] = {N, K, M};
-  job[1] = {M, K, N};
+  job[0] = {N, K, times * M};
+  job[1] = {M, K, p.two ? 2 * np : N};
   if (need & 3) {
-    // the parts of W and x, and of dz beyond its values, in dz's own pass
+    // the parts of W and x, and of dz beyond its values, in dz's own pass; with dz in two
+    // parts both are copied for any kernel
     const float pack = type == VC_FP32   ? pack_us(type, (M + N) * K + M * N / 5) - (act != kNone ? 4.f : 0.f)
-                       : K % 8           ? pack_us(type, (M + N) * K) - (act != kNone ? 4.f : 0.f)
+                       : K % 8 && !p.two ? pack_us(type, (M + N) * K) - (act != kNone ? 4.f : 0.f)
                                          : 0.f;
-    const int can = tile_lines(K) && tile_lines(N) ? 3 : 0;
+    const int can = tile_lines(K) && tile_lines(times * np) ? 3 : 0;
     const float one = choose(type, job, 2, true, can, pack, c);
     p.tiles = c[0].kernel == kTile;
     // or a launch each, in a shape of its own
@@ -1031,11 +1082,12 @@ BackwardPlan make_backward(int type, int64_t M, int K, int N, int act, int need)
   p.rows = slope_rows(M, N);
   p.blocks = (int)div_up(M, p.rows);
   int64_t at = 0;
-  if (need & 3) at += p.tiles ? parts_bytes(type, M, N) : act != kNone ? up256(e * M * N) : 0;
+  const bool parts = p.tiles || p.two;
+  if (need & 3) at += parts ? parts_bytes(type, times * M, N) : act != kNone ? up256(e * M * N) : 0;
   p.W = at;
-  if ((need & 1) && p.tiles) at += parts_bytes(type, N, K);
+  if ((need & 1) && parts) at += parts_bytes(type, p.two ? 2 * np : N, K);
   p.in = at;
-  if ((need & 2) && p.tiles) at += parts_bytes(type, M, K);
+  if ((need & 2) && parts) at += parts_bytes(type, times * M, K);
   p.sums = at;
   if (need & 4) at += up256(4ll * p.blocks * N);
   p.px = at;
@@ -1063,45 +1115,55 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
   const int need = (dx ? 1 : 0) | (dW ? 2 : 0) | (db ? 4 : 0);
   if (!need) return VC_OK;
   const BackwardPlan p = plan_backward(type, M, K, N, act, need);
+  act &= ~kRounded;
   if (p.bytes > work_bytes || (p.bytes && !work)) return VC_ERR_OOM;
   if (too_many(p.x) || too_many(p.w)) return VC_ERR_UNSUPPORTED;
   char* const base = (char*)work;
   const int np = (int)up8(N), kp = (int)up8(K);
   // dy itself is dz where nothing is between them and the products can read it
   const bool made = (need & 3) && (act != kNone || (p.tiles && !as_it_is((const T*)dy, ldy, N)));
+  const bool parts = p.tiles || p.two;
   Slope<T> s = {};
   if (N > 0 && M > 0 && (made || db)) {
     s.dy = (const T*)dy;
     s.z = (const T*)z;
     s.ldy = ldy;
     s.ldz = ldz;
-    if (made && p.tiles) s.parts = (uint16_t*)(base + p.dz);
+    if (made && parts) s.parts = (uint16_t*)(base + p.dz);
     else if (made) s.dz = (T*)(base + p.dz);
     s.sums = db ? (float*)(base + p.sums) : nullptr;
     s.act = act;
   }
   s.M = M;
   s.N = N;
-  s.np = np;
+  s.two = p.two;
+  s.line = p.two ? 2 * np : np;
+  s.plane = p.two ? np : M * np;
   s.rows = p.rows;
   s.lanes = slope_lanes(N);
   Pack<T> mw = {}, mx = {};
-  if (p.tiles && dx && !as_it_is((const T*)W, K, K))
-    mw = {(const T*)W, K, N, K, kp, (uint16_t*)(base + p.W)};
-  if (p.tiles && dW && !as_it_is((const T*)x, ldx, K))
-    mx = {(const T*)x, ldx, M, K, kp, (uint16_t*)(base + p.in)};
+  if (dx && (p.two || (p.tiles && !as_it_is((const T*)W, K, K))))
+    mw = pack_of<T>(W, K, N, K, kp, base + p.W);
+  if (dW && (p.two || (p.tiles && !as_it_is((const T*)x, ldx, K))))
+    mx = pack_of<T>(x, ldx, M, K, kp, base + p.in);
+  if (p.two) {
+    mw.lines = np;
+    mw.again = (int64_t)np * kp;
+    mx.line = 2 * kp;
+    mx.again = kp;
+  }
   run_before<T>(s, mw, mx, st);
 
   Product<T> px = {}, pw = {};
   const T* const dz = made ? (const T*)(base + p.dz) : (const T*)dy;
-  const int64_t ldd = !made ? ldy : p.tiles ? np : N;
+  const int64_t ldd = !made ? ldy : parts ? np : N;
   if (dx) {
     px.I = (int)M;
     px.J = K;
-    px.K = N;
+    px.K = p.two ? 2 * np : N;
     px.out = (T*)dx;
-    px.A = {dz, ldd, (int)M};
-    px.B = {(const T*)W, K, K};
+    px.A = {dz, p.two ? 2 * np : ldd, (int)M};
+    px.B = {(const T*)(p.two ? (const void*)mw.to : W), p.two ? kp : K, K};
     px.pb = mw.to ? mw.to : (const uint16_t*)W;
     px.ldb = kp;
     px.planeB = (int64_t)N * kp;
@@ -1110,17 +1172,18 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
   if (dW) {
     pw.I = N;
     pw.J = K;
-    pw.K = (int)M;
+    pw.K = p.two ? 2 * (int)M : (int)M;
     pw.out = (T*)dW;
     pw.A = {dz, ldd, N};
-    pw.B = {(const T*)x, ldx, K};
+    pw.B = {(const T*)(p.two ? (const void*)mx.to : x), p.two ? kp : ldx, K};
     pw.pb = mx.to ? mx.to : (const uint16_t*)x;
     pw.ldb = mx.to ? kp : ldx;
     pw.planeB = M * kp;
     set_cut(pw, p.w, base + p.pw);
   }
   px.pa = pw.pa = (const uint16_t*)dz;
-  px.lda = pw.lda = ldd;
+  px.lda = px.A.ld;
+  pw.lda = pw.A.ld;
   px.planeA = pw.planeA = M * np;
   // the columns' sums: in the join's launch where there is one (beside the products they
   // would wait for a CU's whole LDS), else in the products'
@@ -1150,6 +1213,11 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
 bool known(int type, int act) {
   return (type == VC_FP32 || type == VC_BF16) && act >= kNone && act <= kSilu;
 }
+bool backward_ok(int type, int64_t M, int K, int N, int act) {
+  if (!known(type, act & ~kRounded) || !sizes_ok(M, K, N)) return false;
+  // sums twice as long are counted in 32 bits
+  return !two_parts(type, act, 3) || (M <= (1 << 30) - 8 && N <= (1 << 29));
+}
 
 }  // namespace
 
@@ -1176,7 +1244,7 @@ extern "C" int vc_linear(int type, const void* x, int64_t M, int K, int64_t ldx,
 
 extern "C" int64_t vc_linear_backward_workspace(int type, int64_t M, int K, int N, int act,
                                                 int need) {
-  if (!known(type, act) || !sizes_ok(M, K, N)) return -1;
+  if (!backward_ok(type, M, K, N, act)) return -1;
   return plan_backward(type, M, K, N, act, need).bytes;
 }
 
@@ -1184,9 +1252,9 @@ extern "C" int vc_linear_backward(int type, const void* dy, int64_t ldy, const v
                                   int64_t ldx, const void* W, const void* z, int64_t ldz, int act,
                                   int64_t M, int K, int N, void* dx, void* dW, void* db,
                                   void* work, int64_t work_bytes, vc_stream_t stream) {
-  if (!known(type, act) || !sizes_ok(M, K, N)) return VC_ERR_ARG;
-  const bool some = M > 0 && N > 0;
-  if (some && (!dy || ldy < N || (act != kNone && (!z || ldz < N)))) return VC_ERR_ARG;
+  if (!backward_ok(type, M, K, N, act)) return VC_ERR_ARG;
+  const bool some = M > 0 && N > 0, slopes = (act & ~kRounded) != kNone;
+  if (some && (!dy || ldy < N || (slopes && (!z || ldz < N)))) return VC_ERR_ARG;
   if (some && K > 0 && ((dx && !W) || (dW && (!x || ldx < K)))) return VC_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
   return type == VC_FP32 ? backward<float>(dy, ldy, x, ldx, W, z, ldz, act, M, K, N, dx, dW, db,
