@@ -1,4 +1,5 @@
-"""Where the training operators can go wrong: dz's bits in the bf16 backward.
+"""Where the training operators can go wrong: dz's bits in the bf16 backward, masks by large finite
+values and logits far from zero in the loss.
 
 Tolerances are those of test_gpu_train, whose helpers these tests use.
 """
@@ -90,3 +91,113 @@ def test_bf16_backward_infinities_and_nan_behind_an_activation(gpu, M, K, N, rou
     for p, q in zip(got, (d @ W.double(), d.t() @ xd, d.sum(0))):
         assert torch.equal(p.isnan(), q.isnan()) and torch.equal(p.isinf(), q.isinf())
         assert torch.equal(p[p.isinf()].double(), q[q.isinf()])
+
+
+# ----------------------------------------------------------------------- loss
+
+FILLS = [-1e9, -1e10, -1e20, -1e30, -1e35, 'lowest']
+VS = [300, 5003, 140001]  # a wave, a workgroup, a row that registers do not hold
+
+
+def _fill(fill, to):
+    return torch.finfo(to).min if fill == 'lowest' else fill
+
+
+def _loss_and_grad(z, t, **kw):
+    return train.cross_entropy(z, torch.tensor(t, device=z.device), reduction='none', **kw)
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('V', VS)
+@pytest.mark.parametrize('fill', FILLS)
+def test_cross_entropy_masked_by_large_values(gpu, to, V, fill):
+    """Classes masked by a large finite value in front, behind, in whole chunks, at odd places, all
+    but one: the loss and the gradient of what is left, whose values are within 30 of each other.
+    2^-18 of the loss: (32 + V / 64 + 4 * 30) units of 2^-24 at V 5003, 2^-12 at V 140001."""
+    live = torch.ones(6, V, dtype=torch.bool, device=gpu)
+    live[0, :V // 2] = False
+    live[1, V // 2:] = False
+    live[2, 8:64] = False
+    live[2, V - 70:] = False
+    live[3, ::2] = False
+    live[4] = False
+    live[4, V // 3] = True
+    live[5, 1:] = False
+    z = tt._randn(gpu, V)(6, V, to=to, std=3.0)
+    t = [int(r.nonzero()[len(r.nonzero()) // 2]) for r in live]
+    masked = torch.where(live, z, torch.full_like(z, _fill(fill, to)))
+    want = torch.where(live, z.double(), -math.inf)
+    want_l = torch.logsumexp(want, 1) - want[range(6), t]
+    want_d = torch.softmax(want, 1)
+    want_d[range(6), t] -= 1
+    for h in (0, 1):  # rows at even and odd places
+        buf = torch.zeros(6, V + 3, dtype=to, device=gpu)
+        buf[:, h:h + V] = masked
+        loss, d = _loss_and_grad(buf[:, h:h + V], t)
+        rel = (32 + V / 64 + 120) * 2.0 ** -24
+        tt._within(loss, want_l, rel * (1 + want_l.abs()), 'loss')
+        half = 2.0 ** -8 if to == BF16 else 0.0
+        tt._within(d, want_d, (rel + half) * want_d.abs() + rel * 2.0 ** -24 + 1e-37, 'gradient')
+        assert not d[~live].any()
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('V', VS)
+@pytest.mark.parametrize('at', [3e6, 1e7, 1e10, 1e20, 1e30, -3e6, -1e7, -1e10, -1e20, -1e30, -2e37])
+def test_cross_entropy_uniform_rows_far_from_zero(gpu, to, V, at):
+    """log V and 1 / V, whatever the value; of the two halves' values the larger alone counts."""
+    z = torch.full((3, V), at, dtype=to, device=gpu)
+    z[1, :V // 2] -= abs(at) / 2
+    z[2, V // 2:] -= abs(at) / 2
+    t = [V - 1, V - 1, 1]
+    n = torch.tensor([V, V - V // 2, V // 2], dtype=F64, device=gpu)
+    loss, d = _loss_and_grad(z, t)
+    rel = (32 + V / 64) * 2.0 ** -24
+    tt._within(loss, n.log(), rel * (1 + n.log()), 'loss')
+    want = torch.where(z == z.amax(1, keepdim=True), 1 / n.unsqueeze(1), 0.0)
+    want[range(3), t] -= 1
+    half = 2.0 ** -8 if to == BF16 else 0.0
+    tt._within(d, want, (rel + half) * want.abs() + 1e-37, 'gradient')
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('V', VS)
+@pytest.mark.parametrize('e', [0.0, 0.1])
+@pytest.mark.parametrize('by', [1e6, 1e9, 1e13, 1e20, 1e30])
+def test_cross_entropy_large_logits(gpu, to, V, e, by):
+    """Logits so large that the softmax is one class: the loss is a difference of logits, to a few
+    units of the largest; the gradient the chosen class's less the target's."""
+    z = tt._randn(gpu, V + 1)(5, V, std=by).to(to)
+    z[0, 7] = 6 * by
+    t = [7, 8, V - 1, 0, V // 2]
+    tgt = torch.tensor(t, device=gpu)
+    lw, dw = tt._loss64(z, tgt, e, -100)
+    loss, d = _loss_and_grad(z, t, smoothing=e)
+    tt._within(loss, lw, 2.0 ** -18 * z.double().abs().amax(1), 'loss')
+    # where two classes are within some 100 of each other the exponentials show it
+    top = z.double().topk(2, dim=1).values
+    clear = (top[:, 0] - top[:, 1]) > 200
+    half = 2.0 ** -8 if to == BF16 else 2.0 ** -18
+    tt._within(d[clear], dw[clear], half * dw[clear].abs() + 2.0 ** -40, 'gradient')
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('V', [20] + VS)
+@pytest.mark.parametrize('at', [0, 1, 299, -1])
+def test_cross_entropy_nan_beside_large_values(gpu, to, V, at):
+    """A NaN anywhere makes its row's loss NaN, in front of, behind or among large values; the
+    target's own counts, and one masked by a large value costs that value."""
+    at = min(at, V - 1)
+    for v in (1e10, -1e10, 2e38, -math.inf):
+        z = torch.full((2, V), v, dtype=to, device=gpu)
+        z[0, at] = math.nan
+        z[1] = 1.0
+        z[1, 2] = v
+        loss, _ = _loss_and_grad(z, [3, 2])
+        assert loss[0].isnan()
+        want = z[1].double()
+        want = torch.logsumexp(want, 0) - want[2]
+        if v > 0:
+            assert abs(float(loss[1])) < 1e-6
+        else:
+            assert float(loss[1]) == pytest.approx(float(want), rel=1e-6)

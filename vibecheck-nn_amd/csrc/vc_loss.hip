@@ -169,8 +169,16 @@ __device__ __forceinline__ float scale_of(const Rows& a, int lane) {
   return 1.f / (float)n;
 }
 
+// A row's largest logit within kFar of zero: its product with log2 e is off by at most
+// a quarter, and the whole number above it is exact.  Further out (half a last place of the
+// product is 128 from 3e9 on) the difference has to come before the product: plain_row.
+// A thread's reference starts at kLowest, below any that such a row can end with, so that
+// logits far below (masks such as -1e10 or -1e30) add zeros, alone in a thread too.
+constexpr float kFar = 0x1p22f, kLowest = -0x1p23f;
+static_assert(-kLowest > kFar * kLog2e + 1.f, "what a thread starts with lies below");
+
 // A row of any values, two passes over memory: rows without a finite largest
-// logit, or one so large that its exponent's product would not be.
+// logit, or one too far from zero.
 template <class T, int W>
 __device__ void plain_row(const Rows& a, const T* z, T* dz, int64_t t, float zt, int tid, float w,
                           float* loss, Team<W> team) {
@@ -179,7 +187,8 @@ __device__ void plain_row(const Rows& a, const T* z, T* dz, int64_t t, float zt,
   float m = -INFINITY, s = 0.f, half = 0.f;
   for (int64_t j = tid; j < a.V; j += 64 * W) {
     const float v = load1(z + j);
-    join(m, s, v, v == -INFINITY || j == t ? 0.f : 1.f);
+    // a NaN is no maximum: it is kept in the sum, before there is a maximum too
+    join(m, s, v, v != v ? v : v == -INFINITY || j == t ? 0.f : 1.f);
     half += v * iv;
   }
   if (W > 1) __syncthreads();
@@ -206,7 +215,8 @@ __device__ void plain_row(const Rows& a, const T* z, T* dz, int64_t t, float zt,
 // logit times log2 e, and the sum of 2^(z log2 e - r): one fma and one
 // exponential a value, and moving to another r multiplies by a power of two,
 // which rounds nothing.  What the rounding of log2 e does to large logits is in
-// every term, the largest's own (em) too, and cancels.  The target's term is kept
+// every term, the largest's own (em) too, and cancels; a thread that meets one beyond
+// kFar may end with any sum, its row goes to plain_row.  The target's term is kept
 // apart (its place holds -inf meanwhile).
 //
 // Memory bounds it: 8,192 x 131,072 bf16, logits read and gradient written, 760 us
@@ -268,7 +278,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
     if (first + TH <= whole) return w;  // the same in all lanes
     return C::drop(w, c < whole ? 0 : c == whole ? (int)((int64_t)c * N - last) : N);
   };
-  float m = -INFINITY, r = -1e37f, s = 0.f, half = 0.f;
+  float m = -INFINITY, r = kLowest, s = 0.f, half = 0.f;
   const auto take = [&](u4 w, Index c, Index first, bool end) {
     if (end) w = mask(w, c, first);
     asm volatile("" : "+v"(w));  // one chunk's values at a time
@@ -329,7 +339,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
   }
   const float w = scale_of(a, lane);
   const float top = team.max_of(fmaxf(m, zt));
-  if (!(fabsf(top) < 1e38f)) {  // the same in every thread of the row
+  if (!(fabsf(top) < kFar)) {  // the same in every thread of the row
     plain_row<T, W>(a, z, dz, t, zt, tid, w, a.loss + row, team);
     return;
   }
