@@ -201,3 +201,61 @@ def test_cross_entropy_nan_beside_large_values(gpu, to, V, at):
             assert abs(float(loss[1])) < 1e-6
         else:
             assert float(loss[1]) == pytest.approx(float(want), rel=1e-6)
+
+
+# ------------------------------------------------------------------- autograd
+
+def test_second_derivatives_raise(gpu):
+    """What create_graph=True returns has the first derivative's values, and a penalty on it does
+    not lose its gradient without a word: alone, beside another loss, through either operator."""
+    f = tt._randn(gpu, 21)
+    x, W, b = (t.requires_grad_() for t in (f(8, 20), f(40, 20), f(40)))
+    t = torch.arange(8, device=gpu)
+    for make in (lambda: train.linear(x, W, b, act='gelu').square().sum(),
+                 lambda: train.linear(x, W, b).sum(),
+                 lambda: train.cross_entropy(x, t)[0],
+                 lambda: train.cross_entropy(x, t, reduction='none')[0].sum(),
+                 lambda: train.cross_entropy(train.linear(x, W, b, act='silu'), t)[0]):
+        want, = torch.autograd.grad(make(), x)
+        for also in (0.0, 1.0):
+            g, = torch.autograd.grad(make(), x, create_graph=True)
+            assert torch.equal(g, want) and g.requires_grad
+            with pytest.raises(NotImplementedError, match='second derivative'):
+                (g.square().sum() + also * x.square().sum()).backward()
+    # the gradients of a bias and a weight alike; what the upstream gradient itself carries passes
+    gW, gb = torch.autograd.grad(train.linear(x, W, b, act='gelu').square().sum(), (W, b), create_graph=True)
+    for g in (gW, gb):
+        for of in (x, W, b):
+            with pytest.raises(NotImplementedError, match='second derivative'):
+                torch.autograd.grad(g.sum(), of, retain_graph=True, allow_unused=True)
+    # one that requires none of the others' gradients
+    for i in range(3):
+        ts = [u if j == i else u.detach() for j, u in enumerate((x, W, b))]
+        g, = torch.autograd.grad(train.linear(*ts, act='silu').sum(), ts[i], create_graph=True)
+        with pytest.raises(NotImplementedError, match='second derivative'):
+            torch.autograd.grad(g.sum(), ts[i], allow_unused=True)
+    with pytest.raises(NotImplementedError, match='second derivative'):
+        torch.autograd.functional.hessian(lambda u: train.cross_entropy(u, t)[0], x.detach())
+    r, up = f(8, 40).requires_grad_(), f(8, 40).requires_grad_()
+    g, = torch.autograd.grad(train.linear(x, W, b, residual=r), r, up, create_graph=True)
+    assert torch.equal(torch.autograd.grad(g.sum(), up)[0], torch.ones_like(up))
+    g, = torch.autograd.grad(train.cross_entropy(x, t, reduction='none')[0], x, f(8).requires_grad_(),
+                             create_graph=True)
+    assert g.requires_grad
+
+
+def test_forward_mode_raises(gpu):
+    f = tt._randn(gpu, 22)
+    x, W, t = f(8, 20), f(40, 20), torch.arange(8, device=gpu)
+    y, z = train.linear(x, W, act='gelu', save=True)
+    with torch.autograd.forward_ad.dual_level():
+        def dual(t):
+            return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: train.linear(dual(x), W), lambda: train.linear(x, dual(W), save=True),
+                     lambda: train.linear(x, W, residual=dual(y)),
+                     lambda: train.linear(dual(x), W.clone().requires_grad_()),
+                     lambda: train.linear_backward(dual(y), x, W, z=z, act='gelu'),
+                     lambda: train.cross_entropy(dual(x), t)):
+            with pytest.raises(NotImplementedError, match='forward-mode'):
+                call()
+        assert torch.equal(train.linear(x, W, act='gelu'), y)

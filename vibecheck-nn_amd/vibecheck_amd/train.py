@@ -6,12 +6,16 @@ Tensors are fp32 or bf16 on the GPU; every function runs on the current stream,
 allocates its outputs and workspace from torch and waits for nothing.  CPU tensors
 raise RuntimeError, other types NotImplementedError, sizes that do not fit
 ValueError.
+
+Gradients are first derivatives in reverse mode: a second derivative (through what
+create_graph=True returned) and forward mode (a dual tensor) raise NotImplementedError.
 """
 import math
 import operator
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import call, load, stream
 
@@ -34,6 +38,30 @@ def _type(t, what):
     if t.get_device() != torch._C._cuda_getDevice():
         raise ValueError(f'vibecheck_amd: {what} is on {t.device}, not on the current device')
     return k
+
+
+def _no_tangents(*tensors):
+    """Forward-mode derivatives would be lost without a word."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError('vibecheck_amd: the kernels have no forward-mode derivative')
+
+
+class _First(torch.autograd.Function):
+    """Passes on what follows n tensors that it depends on; a derivative of it raises."""
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tensors[n:]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError('vibecheck_amd: the kernels have no second derivative')
+
+
+def _first(grads, *on):
+    """What a backward gives: under create_graph=True no constant, but dependent on ``on``."""
+    return _First.apply(len(on), *on, *grads) if torch.is_grad_enabled() else grads
 
 
 def _like(t, ref, shape, what):
@@ -131,7 +159,7 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, W, bias, act, residual, round_dz):
         y, z = _linear(x, W, bias, act, residual, True)
         ctx.save_for_backward(x, W, z)
-        ctx.act, ctx.round_dz = act, round_dz
+        ctx.act, ctx.round_dz, ctx.bias = act, round_dz, bias
         return y
 
     @staticmethod
@@ -139,8 +167,10 @@ class _Linear(torch.autograd.Function):
         x, W, z = ctx.saved_tensors
         needs = ctx.needs_input_grad
         need = [n for n, on in zip(('x', 'W', 'bias'), needs) if on]
-        dx, dW, db = linear_backward(dy, x, W, z, ctx.act, need, ctx.round_dz) if need else \
-            (None, None, None)
+        dx = dW = db = None
+        if need:
+            dx, dW, db = _first(linear_backward(dy, x, W, z, ctx.act, need, ctx.round_dz),
+                                dy, x, W, ctx.bias)
         return dx, dW, db, None, dy if needs[4] else None, None
 
 
@@ -153,6 +183,7 @@ def linear(x, W, bias=None, act=None, residual=None, save=False, round_dz=False)
     that require it; the saved tensors are then the node's own, and ``round_dz`` is what
     linear_backward is given."""
     a = _act(act)
+    _no_tangents(x, W, bias, residual)
     if not save and torch.is_grad_enabled() and (
             x.requires_grad or W.requires_grad or bias is not None and bias.requires_grad or
             residual is not None and residual.requires_grad):
@@ -173,6 +204,7 @@ def linear_backward(dy, x, W, z=None, act=None, need=_ALL, round_dz=False):
     dx and dW are off by their own rounding alone (1.7e-3 of their norm).  ``round_dz`` rounds
     it to bf16 first (2.3e-3); it changes nothing for the other activations or in fp32."""
     a = act if isinstance(act, int) else _act(act)
+    _no_tangents(dy, x, W, z)
     k = _type(dy, 'dy')
     if W.dim() != 2 or dy.dim() < 1:
         raise ValueError('vibecheck_amd: dy has at least one axis, W two')
@@ -209,16 +241,17 @@ def linear_backward(dy, x, W, z=None, act=None, need=_ALL, round_dz=False):
 
 class _Loss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, target, reduction, ignore_index, smoothing):
+    def forward(ctx, logits, tie, target, reduction, ignore_index, smoothing):
         loss, d = _cross_entropy(logits, target, reduction, ignore_index, smoothing, True, None)
         ctx.save_for_backward(d)
+        ctx.tie = tie
         ctx.mark_non_differentiable(d)
         return loss, d
 
     @staticmethod
     def backward(ctx, g, _):
-        d, = ctx.saved_tensors
-        return (d * g.unsqueeze(-1) if g.dim() else d * g).to(d.dtype), None, None, None, None
+        d, = _first(ctx.saved_tensors, ctx.tie)
+        return (d * g.unsqueeze(-1) if g.dim() else d * g).to(d.dtype), None, None, None, None, None
 
 
 def _cross_entropy(logits, target, reduction, ignore_index, smoothing, grad, out):
@@ -260,8 +293,11 @@ def cross_entropy(logits, target, reduction='mean', ignore_index=-100, smoothing
     over the rows whose target is not ``ignore_index``; dlogits is its gradient (per row for
     'none').  A target that is no class gives NaN, a row without a logit above -inf an infinite
     loss and no gradient.  The loss is differentiable where the logits require it."""
+    _no_tangents(logits)
     if torch.is_grad_enabled() and logits.requires_grad and grad and out is None:
-        return _Loss.apply(logits, target, reduction, ignore_index, smoothing)
+        # no value of the logits, but their place in the graph: the node need not keep them
+        tie = logits[..., :0].clone()
+        return _Loss.apply(logits, tie, target, reduction, ignore_index, smoothing)
     return _cross_entropy(logits, target, reduction, ignore_index, smoothing, grad, out)
 
 
