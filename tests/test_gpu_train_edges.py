@@ -259,3 +259,35 @@ def test_forward_mode_raises(gpu):
             with pytest.raises(NotImplementedError, match='forward-mode'):
                 call()
         assert torch.equal(train.linear(x, W, act='gelu'), y)
+
+
+def test_written_tensors_count_as_written(gpu):
+    """A graph that saved a parameter, a working copy or an output that is written in place
+    raises, as it does behind torch's own in-place operations."""
+    f = tt._randn(gpu, 23)
+    x, up = f(8, 20), f(8, 40)
+    for bits in (32, 8):
+        W, c = f(40, 20).requires_grad_(), f(40, 20, to=BF16).requires_grad_()
+        state = train.adamw_state([W], bits)
+        before = {k: t._version for k, t in state.items() if k != 'bits'}
+        x.requires_grad_()
+        ys = [train.linear(x, W, act='gelu').sum(), train.linear(x.to(BF16), c).sum()]
+        train.adamw_step([W], [f(40, 20)], state, 1, copies=[c])
+        for y in ys:
+            with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+                y.backward()
+        assert all(state[k]._version > v for k, v in before.items())
+    # relu's output is what its backward needs; the gradient has taken its place
+    y = train.linear(x, f(40, 20), act='relu')
+    loss, d = train.cross_entropy(y.detach(), torch.arange(8, device=gpu), out=y.detach())
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.backward(d)
+    # where nothing that is needed was overwritten all goes on
+    y = train.linear(x, f(40, 20))
+    loss, d = train.cross_entropy(y.detach(), torch.arange(8, device=gpu), out=y.detach())
+    y.backward(d)
+    with torch.inference_mode():
+        W = f(40, 20)
+        train.adamw_step([W], [f(40, 20)], train.adamw_state([W]), 1)
+        z = f(8, 20)
+        train.cross_entropy(z, torch.arange(8, device=gpu), out=z)

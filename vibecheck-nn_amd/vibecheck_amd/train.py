@@ -9,6 +9,7 @@ ValueError.
 
 Gradients are first derivatives in reverse mode: a second derivative (through what
 create_graph=True returned) and forward mode (a dual tensor) raise NotImplementedError.
+What is written in place counts as written: a graph that saved it raises when it is used.
 """
 import math
 import operator
@@ -16,6 +17,7 @@ from array import array
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from ._lib import call, load, stream
 
@@ -280,6 +282,8 @@ def _cross_entropy(logits, target, reduction, ignore_index, smoothing, grad, out
     work, at, nbytes = _work(logits, 'vc_cross_entropy_workspace', R, kind)
     call('vc_cross_entropy', k, z.data_ptr(), R, V, ld, target.data_ptr(), ignore_index, smoothing,
          kind, loss.data_ptr(), _ptr(d), V, at, nbytes, stream())
+    if out is not None:
+        increment_version(out)
     return loss, d
 
 
@@ -397,3 +401,4 @@ def adamw_step(params, grads, state, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8
          state['m'].data_ptr(), state['v'].data_ptr(), _ptr(state.get('m_scale')),
          _ptr(state.get('v_scale')), lr, betas[0], betas[1], eps, weight_decay, step, _ptr(scale),
          stream())
+    increment_version(params + [state[k] for k in keys] + list(copies or ()))
