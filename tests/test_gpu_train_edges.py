@@ -291,3 +291,27 @@ def test_written_tensors_count_as_written(gpu):
         train.adamw_step([W], [f(40, 20)], train.adamw_state([W]), 1)
         z = f(8, 20)
         train.cross_entropy(z, torch.arange(8, device=gpu), out=z)
+
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('V', [10, 300])
+def test_loss_without_its_gradient_is_differentiable(gpu, to, V):
+    """grad=False leaves the gradient out of the answer, not out of the graph."""
+    f = tt._randn(gpu, 24)
+    z, t = f(4, 5, V, to=to).requires_grad_(), torch.arange(20, device=gpu).view(4, 5) % V
+    t[0, 1] = -100
+    for red, up in (('none', f(4, 5)), ('sum', f(1)[0]), ('mean', None)):
+        kw = dict(reduction=red, smoothing=0.1)
+        loss, d = train.cross_entropy(z, t, **kw)
+        only, none = train.cross_entropy(z, t, grad=False, **kw)
+        assert none is None and torch.equal(only, loss)
+        got, = torch.autograd.grad(only, z, up)
+        assert torch.equal(got, torch.autograd.grad(loss, z, up)[0])
+    g, = torch.autograd.grad(train.cross_entropy(z, t, grad=False)[0], z, create_graph=True)
+    with pytest.raises(NotImplementedError, match='second derivative'):
+        g.sum().backward()
+    with torch.no_grad():
+        assert not train.cross_entropy(z, t, grad=False)[0].requires_grad
+    # with out the caller passes the gradient on
+    loss, d = train.cross_entropy(z, t, out=torch.empty_like(z, requires_grad=False))
+    assert not loss.requires_grad and torch.equal(d, train.cross_entropy(z, t)[1])

@@ -180,10 +180,10 @@ def linear(x, W, bias=None, act=None, residual=None, save=False, round_dz=False)
     """act(x W^T + bias) + residual for x (..., K), W (N, K), bias (N), residual (..., N), all of
     one type.  ``act``: None, 'relu', 'gelu' (the erf form) or 'silu'.
 
-    With ``save`` returns (y, z), z what linear_backward needs (None without an activation;
-    for relu without a residual it is y itself).  Differentiable through autograd for inputs
-    that require it; the saved tensors are then the node's own, and ``round_dz`` is what
-    linear_backward is given."""
+    Differentiable through autograd for inputs that require it; ``round_dz`` is what
+    linear_backward is then given.  With ``save`` it returns (y, z) instead, outside of any
+    graph, z what the caller gives to linear_backward (None without an activation; for relu
+    without a residual it is y itself)."""
     a = _act(act)
     _no_tangents(x, W, bias, residual)
     if not save and torch.is_grad_enabled() and (
@@ -256,6 +256,21 @@ class _Loss(torch.autograd.Function):
         return (d * g.unsqueeze(-1) if g.dim() else d * g).to(d.dtype), None, None, None, None, None
 
 
+class _LossAlone(torch.autograd.Function):
+    """The gradient computed when it is asked for."""
+    @staticmethod
+    def forward(ctx, logits, target, *how):
+        ctx.save_for_backward(logits, target)
+        ctx.how = how
+        return _cross_entropy(logits, target, *how, False, None)[0]
+
+    @staticmethod
+    def backward(ctx, g):
+        logits, target = ctx.saved_tensors
+        d, = _first(_cross_entropy(logits, target, *ctx.how, True, None)[1:], logits)
+        return (d * g.unsqueeze(-1) if g.dim() else d * g).to(d.dtype), None, None, None, None
+
+
 def _cross_entropy(logits, target, reduction, ignore_index, smoothing, grad, out):
     k = _type(logits, 'logits')
     if reduction not in REDUCTIONS:
@@ -296,9 +311,12 @@ def cross_entropy(logits, target, reduction='mean', ignore_index=-100, smoothing
     loss = lse - (1 - smoothing) z_t - smoothing mean(z) per row ('none'), summed, or averaged
     over the rows whose target is not ``ignore_index``; dlogits is its gradient (per row for
     'none').  A target that is no class gives NaN, a row without a logit above -inf an infinite
-    loss and no gradient.  The loss is differentiable where the logits require it."""
+    loss and no gradient.  The loss is differentiable where the logits require it; with ``out``
+    it is not: the gradient is there to be passed on (logits.backward(out))."""
     _no_tangents(logits)
-    if torch.is_grad_enabled() and logits.requires_grad and grad and out is None:
+    if torch.is_grad_enabled() and logits.requires_grad and out is None:
+        if not grad:
+            return _LossAlone.apply(logits, target, reduction, ignore_index, smoothing), None
         # no value of the logits, but their place in the graph: the node need not keep them
         tie = logits[..., :0].clone()
         return _Loss.apply(logits, tie, target, reduction, ignore_index, smoothing)
