@@ -315,3 +315,20 @@ def test_loss_without_its_gradient_is_differentiable(gpu, to, V):
     # with out the caller passes the gradient on
     loss, d = train.cross_entropy(z, t, out=torch.empty_like(z, requires_grad=False))
     assert not loss.requires_grad and torch.equal(d, train.cross_entropy(z, t)[1])
+
+
+def test_cross_entropy_more_rows_than_a_launch_has_threads(gpu):
+    """2^26 rows and some by a wavefront each, 4.4 GB: every sixty-fourth row alike."""
+    V, n = 33, (1 << 20) + 3
+    f = tt._randn(gpu, 25)
+    z, t = f(64, V, to=BF16, std=3.0), torch.arange(64, device=gpu) % V
+    t[5] = -100
+    many = torch.empty(n, 64, V, dtype=BF16, device=gpu)
+    many[:] = z
+    want, dw = train.cross_entropy(z, t, reduction='none')
+    loss, d = train.cross_entropy(many, t.expand(n, 64), reduction='none')
+    assert torch.equal(loss, want.expand(n, 64)) and bool((d == dw).all())
+    loss, d = train.cross_entropy(many, t.expand(n, 64), out=d)
+    mean, dm = train.cross_entropy(z, t)
+    assert float(loss) == pytest.approx(float(mean), rel=1e-6)
+    tt._within(d[-1] * 1024.0, dm.double() * 1024.0 / n, 2.0 ** -7 * dm.double().abs() * 1024.0 / n + 1e-30, 'd')

@@ -159,7 +159,7 @@ struct Team {
   }
 };
 
-// One over the rows that count, by every wave for itself (few rows).
+// One over the rows that count, by every wave for itself (few rows, one launch).
 __device__ __forceinline__ float scale_of(const Rows& a, int lane) {
   if (!a.mean) return 1.f;
   if (a.scale) return *a.scale;
@@ -500,16 +500,28 @@ __global__ __launch_bounds__(1024) void k_loss_sum(const float* loss, int64_t R,
   }
 }
 
+// A launch has fewer than 2^32 threads: more rows than 2^31 threads take (33 million by a
+// wave each, 2 million by sixteen) go by several.
 template <class T, int W, int NV, int ENDS>
 void run_rows(const Rows& a, hipStream_t st) {
-  const unsigned grid = (unsigned)(W == 1 ? (a.R + 3) / 4 : a.R);
+  const int64_t most = (1ll << 31) / (64 * W);
   const int threads = W == 1 ? 256 : 64 * W;
-  if (a.smooth != 0.f) k_loss_rows<T, W, NV, ENDS, true><<<grid, threads, 0, st>>>(a);
-  else k_loss_rows<T, W, NV, ENDS, false><<<grid, threads, 0, st>>>(a);
+  for (int64_t at = 0; at < a.R; at += most) {
+    Rows b = a;
+    b.R = a.R - at < most ? a.R - at : most;
+    b.z = (const T*)a.z + at * a.ld;
+    b.t = a.t + at;
+    b.loss = a.loss + at;
+    if (a.dz) b.dz = (T*)a.dz + at * a.ldd;
+    const unsigned grid = (unsigned)(W == 1 ? (b.R + 3) / 4 : b.R);
+    if (a.smooth != 0.f) k_loss_rows<T, W, NV, ENDS, true><<<grid, threads, 0, st>>>(b);
+    else k_loss_rows<T, W, NV, ENDS, false><<<grid, threads, 0, st>>>(b);
+  }
 }
 
 constexpr int64_t kOneRows = 1024;    // of k_loss_few by one workgroup
 constexpr int64_t kCountRows = 1024;  // that every wave counts by itself
+static_assert(kCountRows <= (1ll << 31) / 1024, "one launch has them all");
 
 // The team of a row: as many waves as hold it in at most 16 chunks a thread; the
 // row's end lies in the last chunks of a thread, those past the limit before.
