@@ -1124,7 +1124,8 @@ int vc_mlp_bab_round(const int32_t *dims, int n_relu, const float *frag,
  * apart where an ld is given (contiguous where none is), at any alignment of
  * their type.  Sums are held in fp32, results rounded once.  Workspaces are
  * the caller's, of the bytes that the _workspace function gives for the same
- * sizes (-1: refused); their contents need not be kept between calls. */
+ * sizes (-1: refused, as more tiles than one launch has threads for); their
+ * contents need not be kept between calls. */
 #define VC_FP32 0
 #define VC_BF16 1
 #define VC_ACT_NONE 0

@@ -332,3 +332,49 @@ def test_cross_entropy_more_rows_than_a_launch_has_threads(gpu):
     mean, dm = train.cross_entropy(z, t)
     assert float(loss) == pytest.approx(float(mean), rel=1e-6)
     tt._within(d[-1] * 1024.0, dm.double() * 1024.0 / n, 2.0 ** -7 * dm.double().abs() * 1024.0 / n + 1e-30, 'd')
+
+
+# ------------------------------------------------- sizes near a launch's limit
+
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('M', [40_000_003, 140_000_003])
+def test_linear_many_rows(gpu, to, M):
+    """More rows than the kernel that would be the fastest has workgroups for in a launch: rows in
+    a period of 61, whole numbers, so that every sum is exact."""
+    K = N = 8
+    g = torch.Generator(device=gpu).manual_seed(3)
+    x = torch.randint(-1, 2, (61, K), generator=g, device=gpu).to(to)
+    dy = torch.randint(-1, 2, (61, N), generator=g, device=gpu).to(to)
+    x[60] = -x[:60].sum(0)  # a period adds nothing to dW or db: no sum grows
+    dy[:] = dy[0]
+    W = torch.randint(-2, 3, (N, K), generator=g, device=gpu).to(to)
+    times, rest = divmod(M, 61)
+
+    def rows(t):
+        out = torch.empty(M, 8, dtype=to, device=gpu)
+        out[:times * 61].view(times, 61, 8)[:] = t
+        out[times * 61:] = t[:rest]
+        return out
+
+    def whole(got, want):
+        return torch.equal(got[:61], want) and bool((got[:times * 61].view(times, 61, 8) == want).all()) \
+            and torch.equal(got[times * 61:], want[:rest])
+
+    big = rows(x)
+    assert whole(train.linear(big, W), (x.double() @ W.double().t()).to(to))
+    dx, dW, db = train.linear_backward(rows(dy), big, W)
+    assert whole(dx, (dy.double() @ W.double()).to(to))
+    want = times * (dy.double().t() @ x.double()) + dy[:rest].double().t() @ x[:rest].double()
+    assert torch.equal(dW.double(), want.to(to).double())
+    want = times * dy.double().sum(0) + dy[:rest].double().sum(0)
+    tt._within(db, want, 2.0 ** -7 * want.abs(), 'db')
+
+
+def test_backward_of_many_columns(gpu):
+    """The columns' sums where there are more of them than workgroups: 10 million."""
+    N = 10_000_019
+    dy = (torch.arange(3 * N, device=gpu).view(3, N) % 7).float()
+    x, W = torch.ones(3, 1, device=gpu), torch.ones(N, 1, device=gpu)
+    _, dW, db = train.linear_backward(dy, x, W, need=('W', 'bias'))
+    assert torch.equal(db, dy.sum(0)) and torch.equal(dW[:, 0], db)
+    assert torch.equal(train.linear_backward(dy, x, W, need=('bias',))[2], db)

@@ -105,3 +105,18 @@ def test_backward_of_a_rounded_dz():
     assert lib.vc_linear_backward_workspace(1, 64, 64, 64, 4 | 16, 7) < 0
     with pytest.raises(ValueError):
         _lib.call('vc_linear', 0, P, 4, 4, 4, P, 5, None, 1 | 16, None, 0, P, None, None, 0, None)
+
+
+def test_sizes_that_no_launch_holds():
+    """Refused by the workspace, before anything is launched; whatever some cut can hold is not."""
+    lib = _lib.load()
+    top = 0x7fffff00
+    for k in (0, 1):
+        assert lib.vc_linear_workspace(k, top, 64, 1 << 30) < 0
+        assert lib.vc_linear_backward_workspace(k, top, 64, 1 << 30, 0, 7) < 0
+        for M in (40_000_003, 140_000_003, 400_000_000):
+            assert lib.vc_linear_workspace(k, M, 8, 8) >= 0
+            assert lib.vc_linear_backward_workspace(k, M, 8, 8, 0, 7) >= 0
+    assert lib.vc_linear_backward_workspace(1, top, 8, 8, 2, 7) < 0  # sums over 2 M lines
+    with pytest.raises(NotImplementedError):
+        _lib.call('vc_linear', 1, P, top, 64, 64, P, 1 << 30, None, 0, None, 0, P, None, None, 0, None)

@@ -132,12 +132,13 @@ struct TileShape {
 };
 TileShape tile_shape(int type, int shape);
 
-// The blocks' sums of dz's columns, joined: 32 columns a workgroup.
+// The blocks' sums of dz's columns, joined: 32 columns a workgroup at a time.
 template <class T>
 struct Columns {
   const float* sums;  // (blocks, N)
   int blocks, N;
   T* db;
+  int groups;         // workgroups
 };
 
 // The forward's product of fp32 rows as they are: bases, lds and K multiples of 16
@@ -242,21 +243,26 @@ __device__ __forceinline__ void deliver(const Product<T>& a, int64_t slice, int 
 // lds: 32 floats for every 32 threads.
 template <class T>
 __device__ __forceinline__ void add_columns(const Columns<T>& a, int block, float* lds) {
-  const int c = threadIdx.x & 31, y = threadIdx.x >> 5, ny = blockDim.x >> 5, j = block * 32 + c;
-  const float* const p = a.sums + min(j, a.N - 1);
-  float s = 0.f;
-  for (int b = y; b < a.blocks; b += 8 * ny) {
-    float v[8];
+  const int c = threadIdx.x & 31, y = threadIdx.x >> 5, ny = blockDim.x >> 5;
+#pragma unroll 1
+  for (int at = block * 32; at < a.N; at += a.groups * 32) {
+    const int j = at + c;
+    const float* const p = a.sums + min(j, a.N - 1);
+    float s = 0.f;
+    for (int b = y; b < a.blocks; b += 8 * ny) {
+      float v[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = p[(int64_t)min(b + u * ny, a.blocks - 1) * a.N];
+      for (int u = 0; u < 8; ++u) v[u] = p[(int64_t)min(b + u * ny, a.blocks - 1) * a.N];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) s += b + u * ny < a.blocks ? v[u] : 0.f;
+      for (int u = 0; u < 8; ++u) s += b + u * ny < a.blocks ? v[u] : 0.f;
+    }
+    __syncthreads();  // the turn before has read
+    lds[y * 32 + c] = s;
+    __syncthreads();
+    if (y || j >= a.N) continue;
+    for (int i = 1; i < ny; ++i) s += lds[i * 32 + c];
+    put(a.db + j, s);
   }
-  lds[y * 32 + c] = s;
-  __syncthreads();
-  if (y || j >= a.N) return;
-  for (int i = 1; i < ny; ++i) s += lds[i * 32 + c];
-  put(a.db + j, s);
 }
 
 }  // namespace vcl

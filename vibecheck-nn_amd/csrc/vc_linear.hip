@@ -563,22 +563,23 @@ Pack<T> pack_of(const void* p, int64_t ld, int64_t rows, int n, int np, void* to
 }
 
 template <class T>
-__device__ __forceinline__ void pack_block(const Pack<T>& m, int64_t block) {
-  const int64_t t = block * LNT + threadIdx.x;
+__device__ __forceinline__ void pack_block(const Pack<T>& m, int64_t block, int64_t blocks) {
   const int c = m.np / 8;
-  const int64_t row = t / c;
-  if (row >= m.lines) return;
-  const int j = (int)(t - row * c) * 8;
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (row < m.rows) load8(m.p + row * m.ld, j, m.n, j + 8 <= m.n, v);
-  uint16_t* const to = m.to + row * m.line + j;
-  store_parts<T>(v, to, m.rows * m.np);
-  if constexpr (sizeof(T) == 2) {
-    if (!m.again) return;
-    // dz's second parts meet this copy: they add nothing to an infinity or NaN
+#pragma unroll 1
+  for (int64_t t = block * LNT + threadIdx.x; t < m.lines * c; t += blocks * LNT) {
+    const int64_t row = t / c;
+    const int j = (int)(t - row * c) * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (row < m.rows) load8(m.p + row * m.ld, j, m.n, j + 8 <= m.n, v);
+    uint16_t* const to = m.to + row * m.line + j;
+    store_parts<T>(v, to, m.rows * m.np);
+    if constexpr (sizeof(T) == 2) {
+      if (!m.again) continue;
+      // dz's second parts meet this copy: they add nothing to an infinity or NaN
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = finite(v[q]) ? v[q] : 0.f;
-    store_parts<T>(v, to + m.again, 0);
+      for (int q = 0; q < 8; ++q) v[q] = finite(v[q]) ? v[q] : 0.f;
+      store_parts<T>(v, to + m.again, 0);
+    }
   }
 }
 
@@ -675,8 +676,8 @@ __global__ __launch_bounds__(LNT) void k_before(Slope<T> s, int ns, int cols, Pa
                                                 Pack<T> b) {
   const int64_t w = blockIdx.x;
   if (w < ns) slope_block(s, (int)w % cols, (int)w / cols);
-  else if (w < ns + na) pack_block(a, w - ns);
-  else pack_block(b, w - ns - na);
+  else if (w < ns + na) pack_block(a, w - ns, na);
+  else pack_block(b, w - ns - na, gridDim.x - ns - na);
 }
 
 int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
@@ -694,6 +695,16 @@ struct Cut {
 };
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// A launch has fewer than 2^32 threads.  A product's workgroups, of so many threads at most, have
+// fewer than 2^30 of them: two of these go together, with the columns' sums (2^18
+// workgroups at most, that take more columns each beyond).
+bool fits(int64_t tiles, int64_t slices, int threads) {
+  return tiles < (1 << 30) && tiles * slices * threads < (1 << 30);
+}
+constexpr int64_t kMostGroups = 1 << 18;
+constexpr int64_t kMostPacks = 1 << 20;  // workgroups of a matrix's parts
+constexpr int64_t kMostSlopes = (1 << 24) - 2 * kMostPacks - 1;  // of dz, beside them
 
 // The slices' sums written, read again and joined by a launch.
 float join_us(int64_t slices, int64_t I, int64_t J) {
@@ -717,7 +728,7 @@ Grid grid_of(int64_t I, int64_t J, int64_t K, int bi, int bj, int bk, int64_t wa
 // What a kernel's tiles cost: `alone` us a step for as many workgroups as share a
 // CU, `shared` us for each of them, `end` us for a tile's output.
 struct Cost {
-  int bi, bj, bk, share;
+  int bi, bj, bk, threads, share;
   float alone, shared, end;
 };
 
@@ -758,6 +769,7 @@ float best_slices(int type, const Cost& c, const Job* job, int n, Grid* best) {
         const int64_t want = kWant[i ? q : p];
         sane = sane && (want == 1 || (4 * want * c.bk <= job[i].K && job[i].I * job[i].J < (1ll << 31)));
         g[i] = grid_of(job[i].I, job[i].J, job[i].K, c.bi, c.bj, c.bk, want);
+        sane = sane && fits(g[i].tiles, g[i].slices, c.threads);
       }
       const float us = sane ? expect(type, c, job, g, n) : 1e30f;
       if (us < least) {
@@ -774,12 +786,14 @@ float best_slices(int type, const Cost& c, const Job* job, int n, Grid* best) {
 // the best tiles: fp32 265 x 352 x 461 16.4, 16.9 and 18.6 us, 512 x 784 x 1024 36.9, 38.7
 // and 27.2, 5171 x 896 x 64 33, 42 and 31; bf16 1021 x 333 x 777 22.5, 18.1 and 19.1, 2050 x
 // 512 x 1030 47, 50 and 36, 17 x 256 x 64 7.2, 9.2 and 7.8.
+constexpr int kGroups32 = 3, kGroups16 = 4;
 Cost product_cost(int type, int shape) {
   if (type == VC_FP32)
-    return shape ? Cost{64, 64, 96, 1, 2.0f, 1.75f, 1.f} : Cost{64, 64, 32, 3, 1.12f, 0.6f, 0.5f};
-  return shape ? Cost{64, 64, 256, 1, 2.9f, 2.2f, 1.f} : Cost{64, 64, 64, 4, 1.3f, 0.4f, 0.5f};
+    return shape ? Cost{64, 64, 96, LNT * kGroups32, 1, 2.0f, 1.75f, 1.f}
+                 : Cost{64, 64, 32, LNT, 3, 1.12f, 0.6f, 0.5f};
+  return shape ? Cost{64, 64, 256, LNT * kGroups16, 1, 2.9f, 2.2f, 1.f}
+               : Cost{64, 64, 64, LNT, 4, 1.3f, 0.4f, 0.5f};
 }
-constexpr int kGroups32 = 3, kGroups16 = 4;
 
 // The tiles that go straight into LDS: a step of as many as share a CU while others
 // stand idle, a step of each with all of them busy (random operands: the card's power
@@ -799,7 +813,7 @@ Cost tile_cost(int type, int shape, bool far) {
   constexpr float end[2][4] = {{6.8f, 3.8f, 0.5f}, {7.5f, 1.5f, 0.4f, 0.4f}};
   const TileShape t = tile_shape(type, shape);
   const int b = type == VC_FP32 ? 0 : 1;
-  return {t.bi, t.bj, t.bk, share[b][shape], alone[far][b][shape], shared[far][b][shape],
+  return {t.bi, t.bj, t.bk, 512, share[b][shape], alone[far][b][shape], shared[far][b][shape],
           end[b][shape]};
 }
 
@@ -844,6 +858,7 @@ Cut cut_direct(int type, int64_t I, int64_t J, int64_t K) {
   for (int shape = 0; shape < (type == VC_FP32 ? 3 : 4); ++shape) {
     const int bi = kDirectRows[shape], bj = kDirectCols[shape];
     const int64_t nj = div_up(J, bj), tiles = div_up(I, bi) * nj;
+    if (!fits(tiles, 1, 64 * kDirectWaves)) continue;
     int64_t s = 1;
     while (tiles * s < kCus && 1024 * s < K && s < 16) s *= 2;
     const float own = e * (bi + bj) * (float)K / s;  // rows past the last are read as the last
@@ -882,9 +897,6 @@ void set_cut(Product<T>& a, const Cut& c, void* part) {
   a.tiles = c.tiles;
   a.f_nj = vcg::FastDiv::make((uint32_t)c.nj);
 }
-// Workgroups of a launch, of up to 1024 threads: below 2^32 of these.
-bool too_many(const Cut& c) { return c.tiles > (1 << 21) || c.tiles * c.slices > (1 << 21); }
-
 template <class T>
 void run_join(const Product<T>& a, const Product<T>& b, const Columns<T>& c, hipStream_t st) {
   const auto quads = [](const Product<T>& p) {
@@ -894,15 +906,18 @@ void run_join(const Product<T>& a, const Product<T>& b, const Columns<T>& c, hip
     return vcg::FastDiv::make((uint32_t)(p.slices > 1 ? part_line(p.J) / 4 : 1));
   };
   const uint32_t na = quads(a), nb = quads(b);
-  const uint32_t nc = c.db ? (uint32_t)div_up(c.N, 32) : 0u;
+  const uint32_t nc = c.db ? (uint32_t)c.groups : 0u;
   const unsigned grid = nc + (unsigned)div_up((int64_t)na + nb, LNT);
   if (grid > 0) k_join<T><<<grid, LNT, 0, st>>>(a, na, line(a), b, nb, line(b), c, nc);
 }
 
 template <class T>
 void run_before(Slope<T> s, Pack<T> a, Pack<T> b, hipStream_t st) {
-  const int64_t na = a.to ? div_up(a.lines * (a.np / 8), LNT) : 0;
-  const int64_t nb = b.to ? div_up(b.lines * (b.np / 8), LNT) : 0;
+  const auto packs = [](const Pack<T>& m) {
+    const int64_t all = m.to ? div_up(m.lines * (m.np / 8), LNT) : 0;
+    return all < kMostPacks ? all : kMostPacks;
+  };
+  const int64_t na = packs(a), nb = packs(b);
   const int cols = s.dy ? (int)div_up(s.N, 8 * s.lanes) : 0, ns = s.dy ? cols * (int)div_up(s.M, s.rows) : 0;
   if (ns + na + nb > 0) k_before<T><<<(unsigned)(ns + na + nb), LNT, 0, st>>>(s, ns, cols, a, na, b);
 }
@@ -913,7 +928,7 @@ bool sizes_ok(int64_t M, int K, int N) {
 
 struct ForwardPlan {
   Cut c;
-  int64_t x, W, part, bytes;  // offsets in the workspace, and its size
+  int64_t x, W, part, bytes;  // offsets in the workspace, and its size (-1: no cut fits a launch)
 };
 
 // A thread's latest plans, by their sizes: the search takes up to 50 us.
@@ -953,10 +968,14 @@ ForwardPlan make_forward(int type, int64_t M, int K, int N, bool raw) {
   if (raw) {
     // two steps of 32 alone on a CU, and of each of two that share one (512 x 784 x
     // 1024 12.2 us, 64 x 8192 x 1024 in eight slices 14.9, 1024 x 784 x 1024 23)
-    const Cost c = {64, 32, 64, 2, 0.68f, 0.68f, 0.5f};
+    const Cost c = {64, 32, 64, 512, 2, 0.68f, 0.68f, 0.5f};
     Grid g;
     const float us = best_slices(type, c, &job, 1, &g);
     if (us < p.c.us) p.c = {kRaw, 0, (int)g.slices, (int)g.steps * 2, g.tiles, g.nj, us};
+  }
+  if (p.c.us >= 1e30f) {
+    p.bytes = -1;
+    return p;
   }
   const bool tiles = p.c.kernel == kTile;
   p.x = 0;
@@ -978,6 +997,7 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
   const bool raw = type == VC_FP32 && K % 4 == 0 && K > 0 && ldx % 4 == 0 && aligned16(x) &&
                    aligned16(W) && K < (1 << 21) && ldx < (1 << 21);
   const ForwardPlan p = plan_forward(type, M, K, N, raw);
+  if (p.bytes < 0) return VC_ERR_UNSUPPORTED;
   if (p.bytes > work_bytes || (p.bytes && !work)) return VC_ERR_OOM;
   char* const base = (char*)work;
   Product<T> a = {};
@@ -1006,7 +1026,6 @@ int forward(const void* x, int64_t M, int K, int64_t ldx, const void* W, int N, 
     a.planeB = (int64_t)N * kp;
     a.K = kp;
   }
-  if (too_many(p.c)) return VC_ERR_UNSUPPORTED;
   set_cut(a, p.c, base + p.part);
   constexpr bool F = sizeof(T) == 4;
   const dim3 grid((unsigned)p.c.tiles, (unsigned)p.c.slices);
@@ -1049,7 +1068,7 @@ struct BackwardPlan {
   bool tiles, two;
   Cut x, w;
   int rows, blocks;
-  int64_t dz, W, in, sums, px, pw, bytes;  // offsets in the workspace, and its size
+  int64_t dz, W, in, sums, px, pw, bytes;  // offsets in the workspace, and its size (-1: as above)
 };
 
 BackwardPlan make_backward(int type, int64_t M, int K, int N, int act, int need) {
@@ -1071,6 +1090,10 @@ BackwardPlan make_backward(int type, int64_t M, int K, int N, int act, int need)
                                          : 0.f;
     const int can = tile_lines(K) && tile_lines(times * np) ? 3 : 0;
     const float one = choose(type, job, 2, true, can, pack, c);
+    if (one >= 1e30f) {
+      p.bytes = -1;
+      return p;
+    }
     p.tiles = c[0].kernel == kTile;
     // or a launch each, in a shape of its own
     Cut w = {}, x = {};
@@ -1081,6 +1104,10 @@ BackwardPlan make_backward(int type, int64_t M, int K, int N, int act, int need)
   if (need & 1) p.x = c[1];
   p.rows = slope_rows(M, N);
   p.blocks = (int)div_up(M, p.rows);
+  if (div_up(N, 8 * slope_lanes(N)) * p.blocks > kMostSlopes) {
+    p.bytes = -1;
+    return p;
+  }
   int64_t at = 0;
   const bool parts = p.tiles || p.two;
   if (need & 3) at += parts ? parts_bytes(type, times * M, N) : act != kNone ? up256(e * M * N) : 0;
@@ -1116,8 +1143,8 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
   if (!need) return VC_OK;
   const BackwardPlan p = plan_backward(type, M, K, N, act, need);
   act &= ~kRounded;
+  if (p.bytes < 0) return VC_ERR_UNSUPPORTED;
   if (p.bytes > work_bytes || (p.bytes && !work)) return VC_ERR_OOM;
-  if (too_many(p.x) || too_many(p.w)) return VC_ERR_UNSUPPORTED;
   char* const base = (char*)work;
   const int np = (int)up8(N), kp = (int)up8(K);
   // dy itself is dz where nothing is between them and the products can read it
@@ -1187,10 +1214,12 @@ int backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void
   px.planeA = pw.planeA = M * np;
   // the columns' sums: in the join's launch where there is one (beside the products they
   // would wait for a CU's whole LDS), else in the products'
-  const Columns<T> sums = {(const float*)(base + p.sums), p.blocks, N, db ? (T*)db : nullptr};
+  const int64_t each = div_up(N, 32);
+  const Columns<T> sums = {(const float*)(base + p.sums), p.blocks, N, db ? (T*)db : nullptr,
+                           (int)(each < kMostGroups ? each : kMostGroups)};
   const bool late = p.w.slices > 1 || p.x.slices > 1;
   const Columns<T> c = late ? Columns<T>{} : sums;
-  const unsigned grid = (unsigned)(p.w.tiles * p.w.slices + p.x.tiles * p.x.slices + (c.db ? div_up(N, 32) : 0));
+  const unsigned grid = (unsigned)(p.w.tiles * p.w.slices + p.x.tiles * p.x.slices + (c.db ? c.groups : 0));
   constexpr int G = sizeof(T) == 4 ? kGroups32 : kGroups16;
   const Cut& any = dW ? p.w : p.x;
   // two of different shapes, or that each fill the chip, go one after the other: their
@@ -1226,7 +1255,7 @@ extern "C" int64_t vc_linear_workspace(int type, int64_t M, int K, int N) {
   if (M == 0 || N == 0) return 0;
   const int64_t a = plan_forward(type, M, K, N, false).bytes;
   const int64_t b = plan_forward(type, M, K, N, type == VC_FP32).bytes;
-  return a > b ? a : b;
+  return a < 0 || b < 0 ? -1 : a > b ? a : b;
 }
 
 extern "C" int vc_linear(int type, const void* x, int64_t M, int K, int64_t ldx, const void* W,
