@@ -93,6 +93,25 @@ def test_bf16_backward_infinities_and_nan_behind_an_activation(gpu, M, K, N, rou
         assert torch.equal(p[p.isinf()].double(), q[q.isinf()])
 
 
+@pytest.mark.parametrize('to', [F32, BF16])
+@pytest.mark.parametrize('M,K,N', [(7, 20, 50), (300, 333, 203), (1030, 520, 776)])
+def test_relu_chooses(gpu, to, M, K, N):
+    """An infinite or NaN gradient where a ReLU is closed adds nothing, at zero too: the results
+    are those of zeros there, to the bit."""
+    f = tt._randn(gpu, 31)
+    x, W, dy, z = f(M, K, to=to), f(N, K, to=to), f(M, N, to=to), f(M, N, to=to)
+    z[2, 5], z[3, 6], z[4], z[5, 7] = -1.0, -0.0, 0.0, -math.inf
+    clean = dy.clone()
+    dy[2, 5], dy[3, 6], dy[4], dy[5, 7] = math.inf, math.nan, -math.inf, math.nan
+    clean[2, 5], clean[3, 6], clean[4], clean[5, 7] = 0, 0, 0, 0
+    got = train.linear_backward(dy, x, W, z=z, act='relu')
+    assert all(map(torch.equal, got, train.linear_backward(clean, x, W, z=z, act='relu')))
+    assert all(bool(t.isfinite().all()) for t in got)
+    z[2, 5] = 1.0  # open: it passes
+    dx, _, db = train.linear_backward(dy, x, W, z=z, act='relu')
+    assert db[5] == math.inf and not bool(dx[2].isfinite().any())
+
+
 # ----------------------------------------------------------------------- loss
 
 FILLS = [-1e9, -1e10, -1e20, -1e30, -1e35, 'lowest']

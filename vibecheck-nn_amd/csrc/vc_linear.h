@@ -83,15 +83,16 @@ __device__ __forceinline__ float activate(float z, int act) {
   return z;
 }
 
-__device__ __forceinline__ float slope(float z, int act) {
-  if (act == kRelu) return z > 0.f ? 1.f : 0.f;
+// dy act'(z).  ReLU's is a choice: an infinite or NaN dy where it is closed adds nothing.
+__device__ __forceinline__ float dz_of(float dy, float z, int act) {
+  if (act == kRelu) return z > 0.f ? dy : 0.f;
   if (act == kGelu) {
     float e;
     const float c = normal_cdf(z, e);
-    return __builtin_fmaf(z * e, 0.39894228040143268f, c);
+    return dy * __builtin_fmaf(z * e, 0.39894228040143268f, c);
   }
   const float s = __builtin_amdgcn_rcpf(1.f + exp_of(-z));
-  return s * (1.f + z * (1.f - s));
+  return dy * (s * (1.f + z * (1.f - s)));
 }
 
 // An operand: `rows` of its free axis; (row, k) at p[row ld + k], across at

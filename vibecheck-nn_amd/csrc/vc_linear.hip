@@ -635,7 +635,7 @@ __device__ __forceinline__ void slope_block(const Slope<T>& a, int bx, int by) {
       if (r >= m1) break;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (a.act != kNone) d[q][i] *= slope(z[q][i], a.act);
+        if (a.act != kNone) d[q][i] = dz_of(d[q][i], z[q][i], a.act);
         sum[i] += d[q][i];
       }
       if (a.parts) {
