@@ -112,6 +112,36 @@ def test_relu_chooses(gpu, to, M, K, N):
     assert db[5] == math.inf and not bool(dx[2].isfinite().any())
 
 
+@pytest.mark.parametrize('act', ['gelu', 'silu'])
+@pytest.mark.parametrize('M,K,N', [(1, 64, 4096), (300, 100, 51), (512, 784, 1024), (2050, 785, 2051)])
+def test_fp32_activations_to_a_few_units(gpu, act, M, K, N):
+    """fp32 results to a few units in the last place of each result, small ones beside negative
+    arguments among them.  gelu: (8 + 2 z^2) units of 2^-24 (the argument of erfc, of exp is rounded,
+    which 2 z^2 / 2 multiplies), silu eight units; slopes the same of their terms' magnitudes,
+    and 2^-22 for what the product of parts leaves out.  The oracle's normal integral is by erfc:
+    by 1 + erf it would lose what is measured here."""
+    def side(z):
+        return torch.special.erfc(-z / math.sqrt(2)) / 2 if act == 'gelu' else torch.sigmoid(z)
+
+    f = tt._randn(gpu, 41 + M)
+    x, W = f(M, K), f(N, K, std=3 * K ** -0.5)
+    y, z = train.linear(x, W, f(N), act=act, save=True)
+    zd = z.double()
+    assert float(zd.min()) < -4
+    unit = (8 + 2 * zd.square() if act == 'gelu' else 8) * 2.0 ** -24
+    tt._within(y, zd * side(zd), unit * (zd * side(zd)).abs() + 1e-37, act)
+    # one column: dx is dz itself
+    z = zd.flatten()[:100_000].float().unsqueeze(1)
+    dy, one = f(len(z), 1), torch.ones(1, 1, device=gpu)
+    dx, _, _ = train.linear_backward(dy, torch.zeros_like(z), one, z=z, act=act, need=('x',))
+    zd = z.double()
+    q = side(zd)
+    other = torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi) if act == 'gelu' else q * side(-zd)
+    unit = (8 + 2 * zd.square() if act == 'gelu' else 8) * 2.0 ** -24
+    tol = (unit * (q + zd.abs() * other) + 2.0 ** -22 * (q + zd * other).abs()) * dy.double().abs()
+    tt._within(dx, dy.double() * (q + zd * other), tol + 1e-37, 'slope')
+
+
 # ----------------------------------------------------------------------- loss
 
 FILLS = [-1e9, -1e10, -1e20, -1e30, -1e35, 'lowest']

@@ -59,7 +59,7 @@ __device__ __forceinline__ void put(T* p, float v) {
 constexpr float kLog2e = 1.44269504088896341f;
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// The normal distribution's integral up to z, and e = exp(-z^2 / 2) on the way
+// bf16: the normal distribution's integral up to z, and e = exp(-z^2 / 2) on the way
 // (Abramowitz and Stegun 7.1.26, off by at most 7.5e-8): twenty instructions,
 // where the library's erff takes twice as many and the 134 million values of an
 // 8192 x 16384 output showed it (150 us of 1140).
@@ -75,24 +75,44 @@ __device__ __forceinline__ float normal_cdf(float z, float& e) {
   return z < 0.f ? q : 1.f - q;
 }
 
+// In fp32 the forms that lose nothing: erfc keeps the small values of a negative z, and
+// exp(-|z|) both of a sigmoid's sides.
+template <class T>
 __device__ __forceinline__ float activate(float z, int act) {
-  float e;
   if (act == kRelu) return z > 0.f ? z : (z != z ? z : 0.f);
-  if (act == kGelu) return z * normal_cdf(z, e);
-  if (act == kSilu) return z * __builtin_amdgcn_rcpf(1.f + exp_of(-z));
+  if constexpr (sizeof(T) == 4) {
+    if (act == kGelu) return 0.5f * z * erfcf(z * -0.70710678118654752f);
+    if (act == kSilu) {
+      const float e = expf(-fabsf(z));
+      return (z < 0.f ? z * e : z) / (1.f + e);
+    }
+  } else {
+    float e;
+    if (act == kGelu) return z * normal_cdf(z, e);
+    if (act == kSilu) return z * __builtin_amdgcn_rcpf(1.f + exp_of(-z));
+  }
   return z;
 }
 
 // dy act'(z).  ReLU's is a choice: an infinite or NaN dy where it is closed adds nothing.
+template <class T>
 __device__ __forceinline__ float dz_of(float dy, float z, int act) {
   if (act == kRelu) return z > 0.f ? dy : 0.f;
-  if (act == kGelu) {
-    float e;
-    const float c = normal_cdf(z, e);
-    return dy * __builtin_fmaf(z * e, 0.39894228040143268f, c);
+  if constexpr (sizeof(T) == 4) {
+    if (act == kGelu)
+      return dy * __builtin_fmaf(z * expf(-0.5f * z * z), 0.39894228040143268f,
+                                 0.5f * erfcf(z * -0.70710678118654752f));
+    const float e = expf(-fabsf(z)), u = 1.f / (1.f + e), v = e * u;
+    return dy * __builtin_fmaf(z * u, v, z < 0.f ? v : u);
+  } else {
+    if (act == kGelu) {
+      float e;
+      const float c = normal_cdf(z, e);
+      return dy * __builtin_fmaf(z * e, 0.39894228040143268f, c);
+    }
+    const float s = __builtin_amdgcn_rcpf(1.f + exp_of(-z));
+    return dy * (s * (1.f + z * (1.f - s)));
   }
-  const float s = __builtin_amdgcn_rcpf(1.f + exp_of(-z));
-  return dy * (s * (1.f + z * (1.f - s)));
 }
 
 // An operand: `rows` of its free axis; (row, k) at p[row ld + k], across at
@@ -170,10 +190,17 @@ __device__ __forceinline__ void store4(uint16_t* p, const v4f& v) {
 // Columns j .. j + 3 (all within J) of rows i, i + step, .. as far as they go: bias,
 // activation, residual, stores.  Every row's loads come before the first that is
 // worked on, one branch chooses the activation of all.  bias: zeros where there is
-// none.
-template <class T, int U>
+// none.  BARE: a product with none of them, as the backward's are.
+template <class T, bool BARE, int U>
 __device__ __forceinline__ void finish_rows(const Product<T>& a, int i, int step, int j,
                                             const v4f& bias, const v4f (&s)[U]) {
+  const int64_t o = (int64_t)i * a.J + j;
+  if (BARE) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * step < a.I) store4(a.out + o + (int64_t)u * step * a.J, s[u]);
+    return;
+  }
   v4f z[U], v[U], r[U];
   if (a.res) {
 #pragma unroll
@@ -185,7 +212,7 @@ __device__ __forceinline__ void finish_rows(const Product<T>& a, int i, int step
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[u][q] = activate(z[u][q], act);
+      for (int q = 0; q < 4; ++q) v[u][q] = activate<T>(z[u][q], act);
   };
   if (a.act == kRelu) each(std::integral_constant<int, kRelu>{});
   else if (a.act == kGelu) each(std::integral_constant<int, kGelu>{});
@@ -194,7 +221,6 @@ __device__ __forceinline__ void finish_rows(const Product<T>& a, int i, int step
 #pragma unroll
     for (int u = 0; u < U; ++u) v[u] += r[u];
   }
-  const int64_t o = (int64_t)i * a.J + j;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (i + u * step >= a.I) continue;
@@ -214,19 +240,23 @@ __device__ __forceinline__ v4f bias_of(const Product<T>& a, int j) {
 }
 
 // Four columns j .. j + 3 of row i, the last of them past J perhaps.
-template <class T>
+template <class T, bool BARE>
 __device__ __forceinline__ void finish(const Product<T>& a, int i, int j, const v4f& s) {
   if (j + 4 <= a.J) {
     const v4f one[1] = {s};
-    finish_rows<T, 1>(a, i, 0, j, bias_of(a, j), one);
+    finish_rows<T, BARE>(a, i, 0, j, BARE ? v4f{} : bias_of(a, j), one);
     return;
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     if (j + q >= a.J) continue;
     const int64_t o = (int64_t)i * a.J + j + q;
+    if (BARE) {
+      put(a.out + o, s[q]);
+      continue;
+    }
     const float z = a.bias ? s[q] + get(a.bias + j + q) : s[q];
-    float v = activate(z, a.act);
+    float v = activate<T>(z, a.act);
     if (a.res) v += get(a.res + i * a.ldr + j + q);
     put(a.out + o, v);
     if (a.z) put(a.z + o, z);
@@ -234,10 +264,10 @@ __device__ __forceinline__ void finish(const Product<T>& a, int i, int j, const 
 }
 
 // Four columns of row i of a slice: finished, or left for the join.
-template <class T>
+template <class T, bool BARE>
 __device__ __forceinline__ void deliver(const Product<T>& a, int64_t slice, int i, int j,
                                         const v4f& s) {
-  if (a.slices == 1) finish(a, i, j, s);
+  if (a.slices == 1) finish<T, BARE>(a, i, j, s);
   else *reinterpret_cast<v4f*>(a.part + (slice * a.I + i) * part_line(a.J) + j) = s;
 }
 

@@ -324,7 +324,7 @@ __device__ __forceinline__ void product_tile(const Product<T>& a, uint32_t block
     for (int j = 0; j < M2; ++j) {
       const int col = j0 + (wj * M2 + j) * 16 + 4 * g;
       if (col >= a.J) continue;
-      deliver(a, slice, row, col, sum[i][j]);
+      deliver<T, XB>(a, slice, row, col, sum[i][j]);
     }
   }
 }
@@ -454,7 +454,7 @@ __global__ __launch_bounds__(64 * kDirectWaves, 2) void k_direct(Product<T> a) {
 #pragma unroll
     for (int k = 1; k < NW; ++k) s += part[k][b][lane];
     const int row = i0 + 16 * (b / NB) + r, col = j0 + 16 * (b % NB) + 4 * g;
-    if (row < a.I && col < a.J) deliver(a, blockIdx.y, row, col, s);
+    if (row < a.I && col < a.J) deliver<T, false>(a, blockIdx.y, row, col, s);
   }
 }
 
@@ -480,7 +480,7 @@ __device__ __forceinline__ void join_quad(const Product<T>& a, uint32_t t, vcg::
   else if (a.slices <= 4) some(0, std::integral_constant<int, 4>{});
   else
     for (int s = 0; s < a.slices; s += 8) some(s, std::integral_constant<int, 8>{});
-  finish(a, i, j, v);
+  finish<T, false>(a, i, j, v);
 }
 
 // Workgroups of the columns' sums first, where dz has any left to join.
@@ -629,26 +629,33 @@ __device__ __forceinline__ void slope_block(const Slope<T>& a, int bx, int by) {
       load8(a.dy + r * a.ldy, j, a.N, whole, d[q]);
       if (a.act != kNone) load8(a.z + r * a.ldz, j, a.N, whole, z[q]);
     }
+    const auto each = [&](auto act) {  // one branch chooses the slope of all
 #pragma unroll
-    for (int q = 0; q < R; ++q) {
-      const int64_t r = m + per * q;
-      if (r >= m1) break;
+      for (int q = 0; q < R; ++q) {
+        const int64_t r = m + per * q;
+        if (r >= m1) break;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (a.act != kNone) d[q][i] = dz_of(d[q][i], z[q][i], a.act);
-        sum[i] += d[q][i];
-      }
-      if (a.parts) {
-        uint16_t* const to = a.parts + r * a.line + j;
-        if (sizeof(T) == 2 && a.two) store_two(d[q], to, a.plane);
-        else store_parts<T>(d[q], to, a.plane);
-      }
-      if (a.dz) {
+        for (int i = 0; i < 8; ++i) {
+          if (act != kNone) d[q][i] = dz_of<T>(d[q][i], z[q][i], act);
+          sum[i] += d[q][i];
+        }
+        if (a.parts) {
+          uint16_t* const to = a.parts + r * a.line + j;
+          if (sizeof(T) == 2 && a.two) store_two(d[q], to, a.plane);
+          else store_parts<T>(d[q], to, a.plane);
+        }
+        if (a.dz) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (j + i < a.N) put(a.dz + r * a.N + j + i, d[q][i]);
+          for (int i = 0; i < 8; ++i)
+            if (j + i < a.N) put(a.dz + r * a.N + j + i, d[q][i]);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // one row's temporaries at a time
       }
-    }
+    };
+    if (a.act == kNone) each(std::integral_constant<int, kNone>{});
+    else if (a.act == kRelu) each(std::integral_constant<int, kRelu>{});
+    else if (a.act == kGelu) each(std::integral_constant<int, kGelu>{});
+    else each(std::integral_constant<int, kSilu>{});
   };
   if (j < a.N) {
     if (a.rows <= per) {

@@ -338,7 +338,7 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
   v4f* const sums = reinterpret_cast<v4f*>(lds);
   const int g = lane >> 4, r = lane & 15;
   const int q = tid % Q, row0 = tid / Q, j = j0 + 4 * q;
-  const v4f bias = bias_of(a, j);
+  const v4f bias = XB ? v4f{} : bias_of(a, j);
 #pragma unroll 1
   for (int p = 0; p < BI / ROWS; ++p) {
     __syncthreads();
@@ -367,7 +367,7 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
           for (int k = 0; k < 4; ++k) apart |= !finite(w[u][k]);
       }
       if (!apart && a.slices == 1) {
-        finish_rows<T, U>(a, i, STEP, j, bias, w);
+        finish_rows<T, XB>(a, i, STEP, j, bias, w);
       } else if (!apart) {
         const int line = part_line(a.J);
         float* const o = a.part + (slice * (int64_t)a.I + i) * line + j;
@@ -387,7 +387,7 @@ __device__ __forceinline__ void tile(const Product<T>& a, uint32_t block, char* 
                 x[k] = plain_sum<XA, XB>(a, iu, j + k, k0, k0 + left);
             }
           }
-          deliver(a, slice, iu, j, x);
+          deliver<T, XB>(a, slice, iu, j, x);
         }
       }
     }
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(512, 2) void k_raw(Product<float> a) {
   }
   const int row = tid / Q, q = tid % Q, j = j0 + 4 * q;
   if (i0 + row >= a.I || j >= a.J) return;
-  deliver(a, slice, i0 + row, j, sums[row * Q + (q ^ (row & 7))]);
+  deliver<float, false>(a, slice, i0 + row, j, sums[row * Q + (q ^ (row & 7))]);
 }
 
 // A kernel's LDS limit, set once per device.
