@@ -427,3 +427,28 @@ def test_backward_of_many_columns(gpu):
     _, dW, db = train.linear_backward(dy, x, W, need=('W', 'bias'))
     assert torch.equal(db, dy.sum(0)) and torch.equal(dW[:, 0], db)
     assert torch.equal(train.linear_backward(dy, x, W, need=('bias',))[2], db)
+
+
+# ------------------------------------------------------------------ optimiser
+
+def test_adamw_8_parameter_to_the_bit(gpu):
+    """The parameter of a step with 8-bit states: every operation rounded to 32 bits by itself
+    (in 64 bits and rounded again, which for these is the same)."""
+    n, (b1, b2), lr, eps, wd = 1 << 20, (0.9, 0.999), 1e-3, 1e-8, 0.1
+    f = tt._randn(gpu, 51)
+    one = tt._single
+    p, state = f(n, std=1e-3), train.adamw_state([f(n)], bits=8)
+    p[::3] = 0  # the step itself
+    w = [float(torch.tensor(v, dtype=F32)) for v in (b1, 1 - b1, b2, 1 - b2)]
+    for k in range(1, 4):
+        g = f(n) * torch.exp(3 * f(n))
+        m, u = (one(state[s].view(torch.float8_e4m3fn).double()
+                    * state[s + '_scale'].double().repeat_interleave(256)) for s in ('m', 'v'))
+        gd = g.double()
+        m = one(one(w[0] * m) + one(w[1] * gd))
+        u = one(one(one(w[2] * one(u * u)) + one(one(w[3] * gd) * gd)).sqrt())
+        c = [float(torch.tensor(v, dtype=F32)) for v in
+             (1 - lr * wd, -lr / (1 - b1 ** k), math.sqrt(1 - b2 ** k), eps)]
+        want = one(one(p.double() * c[0]) + one(one(c[1] * m) / one(one(u / c[2]) + c[3])))
+        train.adamw_step([p], [g], state, k, lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd)
+        assert torch.equal(p.double(), want)

@@ -9,7 +9,7 @@
 // 256 values: a wavefront takes one block, four values a lane.  Memory bounds it: 16
 // blocks a workgroup keep enough loads on their way (403 million values in 32 bits,
 // 28 bytes each, 1.87 to 2.15 ms, 5.2 to 6.0 TB/s; 200 million in 8 bits, 16 bytes each,
-// 651 us, 4.9), and small tensors cost a share of one launch.  In 32 bits it
+// 669 us, 4.8), and small tensors cost a share of one launch.  In 32 bits it
 // holds m and v.  In 8 bits it holds m and u = sqrt(v) as e4m3 values with one
 // fp32 scale a block, the block's largest / 448, and each is rounded up or down
 // with the probability of what is cut, by a hash of its place and the step.
@@ -39,7 +39,7 @@ struct Step {
   int w0[kTensors];  // its first workgroup
   int n;
   uint32_t seed;
-  float decay, b1, inv_bc2;
+  float decay, b1;
   AdamConst c;
   void *m, *v;
   float *ms, *vs;
@@ -154,16 +154,15 @@ __device__ __forceinline__ uint32_t dither_of(uint32_t i, uint32_t seed) {
   return (h ^ h >> 15) >> 12;
 }
 
-// One value's update; v becomes its root.  What is stored follows from m and the root by
-// a cut, so their last bits decide: they are those of the plain sequence of operations,
-// each rounded by itself (__fsqrt_rn can be off by one).  The parameter's own division is
-// a product with a reciprocal, off by some 2^-22 of the step (50 million values with two
-// rounded divisions 168 us, so 163).
+// One value's update, every operation rounded by itself; v becomes its root.  What is
+// stored follows from m and the root by a cut, so their last bits decide: they are those
+// of the plain sequence of operations (__fsqrt_rn can be off by one).  The parameter's are
+// too: with a product by a reciprocal it is off by some 2^-22 of the step (200 million
+// values 652 us, so 669).
 __device__ __forceinline__ float update8(float p, float g, float& m, float& v, const Step& a) {
   m = a.b1 * m + a.c.w1 * g;
   v = __builtin_sqrtf(a.c.b2 * v + a.c.w2 * g * g);
-  return __builtin_fmaf(a.c.neg_step * m,
-                        __builtin_amdgcn_rcpf(__builtin_fmaf(v, a.inv_bc2, a.c.eps)), p);
+  return p + __fdiv_rn(a.c.neg_step * m, __fdiv_rn(v, a.c.bc2) + a.c.eps);
 }
 
 template <class P, class G, int BITS, bool WHOLE>
@@ -266,7 +265,6 @@ extern "C" int vc_adamw_step(const void* const* p, const void* const* g, const v
   a.b1 = (float)b1;
   a.c = adam_const(b1, b2, eps, lr / (1.0 - pow(b1, (double)step)),
                    sqrt(1.0 - pow(b2, (double)step)));
-  a.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(b2, (double)step)));
   a.m = m;
   a.v = v;
   a.ms = m_scale;
