@@ -4,12 +4,13 @@ values and logits far from zero in the loss.
 Tolerances are those of test_gpu_train, whose helpers these tests use.
 """
 import math
+from array import array
 
 import pytest
 import torch
 
 import test_gpu_train as tt
-from vibecheck_amd import train
+from vibecheck_amd import _lib, train
 
 pytestmark = pytest.mark.gpu
 F32, F64, BF16 = torch.float32, torch.float64, torch.bfloat16
@@ -452,3 +453,17 @@ def test_adamw_8_parameter_to_the_bit(gpu):
         want = one(one(p.double() * c[0]) + one(one(c[1] * m) / one(one(u / c[2]) + c[3])))
         train.adamw_step([p], [g], state, k, lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd)
         assert torch.equal(p.double(), want)
+
+
+def test_adamw_refuses_before_it_changes_anything(gpu):
+    """A tensor larger than a launch takes, behind more small ones than one launch has."""
+    n = array('q', [256] * 99 + [1 << 36])
+    p, g = torch.ones(99, 256, device=gpu), torch.ones(99, 256, device=gpu)
+    state = train.adamw_state([p])
+    at = [t.data_ptr() for t in (*p, p[0])]
+    ptrs, grads = array('Q', at), array('Q', [t.data_ptr() for t in (*g, g[0])])
+    with pytest.raises(NotImplementedError):
+        _lib.call('vc_adamw_step', ptrs.buffer_info()[0], grads.buffer_info()[0], None,
+                  n.buffer_info()[0], len(n), 0, 0, 32, state['m'].data_ptr(),
+                  state['v'].data_ptr(), None, None, 0.1, 0.9, 0.999, 1e-8, 0.0, 1, None, _lib.stream())
+    assert bool((p == 1).all()) and not state['m'].any()

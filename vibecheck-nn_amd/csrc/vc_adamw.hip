@@ -25,6 +25,7 @@ constexpr int ANT = 256;
 constexpr int kBlock = 256;       // values that share a scale
 constexpr int kBlocksPerWg = 16;  // of one tensor
 constexpr int kTensors = 88;
+constexpr int64_t kMostWgs = 1 << 23;  // threads of a grid: below 2^32
 
 struct Tensor {
   void* p;
@@ -256,6 +257,8 @@ extern "C" int vc_adamw_step(const void* const* p, const void* const* g, const v
     total += n[i];
   }
   if (total == 0) return VC_OK;
+  for (int i = 0; i < count; ++i)  // all of them before the first is changed
+    if (n[i] > kMostWgs * kBlocksPerWg * kBlock) return VC_ERR_UNSUPPORTED;
   if (!m || !v || !aligned16(m) || !aligned16(v) || (bits == 8 && (!m_scale || !v_scale)))
     return VC_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
@@ -289,8 +292,7 @@ extern "C" int vc_adamw_step(const void* const* p, const void* const* g, const v
     const int64_t blocks = (n[i] + kBlock - 1) / kBlock;
     const int64_t w = (blocks + kBlocksPerWg - 1) / kBlocksPerWg;
     if (w == 0) continue;
-    if (w > (1 << 23)) return VC_ERR_UNSUPPORTED;  // threads of a grid: below 2^32
-    if (a.n == kTensors || wgs + w > (1 << 23)) flush();
+    if (a.n == kTensors || wgs + w > kMostWgs) flush();
     a.t[a.n] = Tensor{const_cast<void*>(p[i]), g[i], copy ? (uint16_t*)copy[i] : nullptr, n[i], block};
     a.w0[a.n++] = (int)wgs;
     wgs += w;
