@@ -143,6 +143,30 @@ def test_fp32_activations_to_a_few_units(gpu, act, M, K, N):
     tt._within(dx, dy.double() * (q + zd * other), tol + 1e-37, 'slope')
 
 
+@pytest.mark.parametrize('M,K,N', [(1, 64, 40), (17, 333, 65), (300, 203, 117), (520, 784, 1024), (1021, 1031, 1030)])
+def test_any_nan_stays_one(gpu, M, K, N):
+    """A NaN whose bits differ from an infinity's in the last sixteen alone, of either sign, in
+    each of the operands."""
+    def nan(t, i, j, bits):
+        t.view(torch.int32)[i, j] = bits
+
+    f = tt._randn(gpu, 61)
+    for bits in (0x7f800001, 0xff808000 - (1 << 32), 0x7f80ffff):
+        x, W, dy = f(M, K), f(N, K), f(M, N)
+        nan(x, M - 1, 5, bits)
+        nan(W, 7, K - 1, bits)
+        y = train.linear(x, W)
+        want = torch.zeros(M, N, dtype=torch.bool, device=gpu)
+        want[M - 1], want[:, 7] = True, True
+        assert torch.equal(y.isnan(), want) and not y.isinf().any()
+        nan(dy, 0, 3, bits)
+        dx, dW, db = train.linear_backward(dy, x, W)
+        wx, ww, wb = (torch.zeros(t.shape, dtype=torch.bool, device=gpu) for t in (dx, dW, db))
+        wx[0], wx[:, K - 1], ww[3], ww[:, 5], wb[3] = True, True, True, True, True
+        for got, nans in ((dx, wx), (dW, ww), (db, wb)):
+            assert torch.equal(got.isnan(), nans) and not got.isinf().any()
+
+
 # ----------------------------------------------------------------------- loss
 
 FILLS = [-1e9, -1e10, -1e20, -1e30, -1e35, 'lowest']

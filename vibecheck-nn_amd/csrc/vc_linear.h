@@ -35,8 +35,11 @@ __device__ __forceinline__ uint32_t bf_pack(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2bf));
 }
 
-// Two values' parts, the first cut: h + m + l is the value.
+// Two values' parts, the first cut: h + m + l is the value.  A NaN is made quiet first: one
+// whose upper sixteen bits are an infinity's would be cut to that.
 __device__ __forceinline__ void cut2(float x0, float x1, uint32_t& h, uint32_t& m, uint32_t& l) {
+  x0 = __builtin_canonicalizef(x0);
+  x1 = __builtin_canonicalizef(x1);
   const uint32_t b0 = __builtin_bit_cast(uint32_t, x0), b1 = __builtin_bit_cast(uint32_t, x1);
   h = __builtin_amdgcn_perm(b1, b0, 0x07060302);
   const float a0 = x0 - __builtin_bit_cast(float, b0 & 0xffff0000u);
