@@ -491,3 +491,24 @@ def test_adamw_refuses_before_it_changes_anything(gpu):
                   n.buffer_info()[0], len(n), 0, 0, 32, state['m'].data_ptr(),
                   state['v'].data_ptr(), None, None, 0.1, 0.9, 0.999, 1e-8, 0.0, 1, None, _lib.stream())
     assert bool((p == 1).all()) and not state['m'].any()
+
+
+def test_cross_entropy_out_over_the_logits(gpu):
+    """The logits' own place, or none of it: shifted or with rows closer together a row would be
+    read after another's gradient was written there."""
+    f, t = tt._randn(gpu, 71), torch.arange(6, device=gpu)
+    buf = f(4000)
+    z = buf[:3000].view(6, 500)
+    for out in (buf[4:3004], buf[500:3500]):
+        with pytest.raises(ValueError, match='overlaps'):
+            train.cross_entropy(z, t, out=out.view(6, 500))
+    with pytest.raises(ValueError, match='overlaps'):
+        train.cross_entropy(buf[:3600].view(6, 600)[:, :500], t, out=z)
+    want = train.cross_entropy(z, t)
+    for zz, out in ((z, buf[1000:1000].new_empty(6, 500)), (buf.clone()[:3000].view(6, 500),) * 2,
+                    (z[:2], buf[1000:2000].view(2, 500))):
+        loss, d = train.cross_entropy(zz, t[:len(zz)], out=out)
+        if len(zz) == 6:
+            assert torch.equal(loss, want[0]) and torch.equal(d, want[1])
+    loss, d = train.cross_entropy(buf[:600].view(1, 600)[:, :500], t[:1], out=buf[:500].view(1, 500))
+    assert bool(loss.isfinite())

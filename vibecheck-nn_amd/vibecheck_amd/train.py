@@ -293,6 +293,11 @@ def _cross_entropy(logits, target, reduction, ignore_index, smoothing, grad, out
     else:
         d = logits.new_empty(logits.shape) if grad else None
     z, ld = _rows(logits)
+    if out is not None and R > 0:
+        # row for row it may be the logits; shifted, a row would be read after it was written
+        at, to, e = z.data_ptr(), out.data_ptr(), out.element_size()
+        if (at != to or ld != V and R > 1) and to < at + ((R - 1) * ld + V) * e and at < to + R * V * e:
+            raise ValueError('vibecheck_amd: out overlaps the logits without being them')
     target = target.contiguous()
     work, at, nbytes = _work(logits, 'vc_cross_entropy_workspace', R, kind)
     call('vc_cross_entropy', k, z.data_ptr(), R, V, ld, target.data_ptr(), ignore_index, smoothing,
