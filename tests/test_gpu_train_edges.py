@@ -1,7 +1,10 @@
-"""Where the training operators can go wrong: dz's bits in the bf16 backward, masks by large finite
-values and logits far from zero in the loss.
+"""Where the training operators can go wrong: dz's bits in the bf16 backward, fp32 activations'
+last places, NaN and infinities behind them, masks by large finite values and logits far from
+zero, second derivatives and what is written in place, sizes near a launch's limit, the 8-bit
+step's parameter to the bit.
 
-Tolerances are those of test_gpu_train, whose helpers these tests use.
+Tolerances are those of test_gpu_train, whose helpers these tests use, where a test does not
+derive its own.
 """
 import math
 from array import array

@@ -223,7 +223,8 @@ __device__ void plain_row(const Rows& a, const T* z, T* dz, int64_t t, float zt,
 // (5.6 TB/s), x 50,021 343 (4.8); read twice, as the first kernel did, 2,726.  1000 x 50,021
 // fp32 rows that no 16 bytes divide, 91 us (4.4).  A team is as small as holds its row in at most 16
 // chunks a thread: what a smaller one saves is the joins across waves, what a larger
-// one saves is registers, of which 16 chunks leave a CU two teams.
+// one saves is registers: of sixteen waves with up to 4 chunks a thread (58 to 60
+// registers) a CU has two teams, with 6 (68 to 72) to 16 (110 to 124) one.
 template <class T, int W, int NV, int ENDS, bool SMOOTH>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_loss_rows(Rows a) {
   typedef Chunk<T> C;
