@@ -457,6 +457,20 @@ def test_backward_of_many_columns(gpu):
     assert torch.equal(train.linear_backward(dy, x, W, need=('bias',))[2], db)
 
 
+def test_bf16_backward_long_offsets(gpu):
+    """dz's parts past 2^32 values: a gradient in the last rows alone."""
+    M, K, N = (1 << 19) + 61, 64, 4096
+    f = tt._randn(gpu, 81)
+    x, W = f(M, K, to=BF16), f(N, K, to=BF16)
+    dy, z = torch.zeros(M, N, dtype=BF16, device=gpu), torch.zeros(M, N, dtype=BF16, device=gpu)
+    dy[-3:], z[-3:] = f(3, N, to=BF16), f(3, N, to=BF16)
+    dx, dW, db = train.linear_backward(dy, x, W, z=z, act='silu')
+    wx, ww, wb = train.linear_backward(dy[-3:], x[-3:], W, z=z[-3:], act='silu')
+    assert not dx[:-3].any()
+    for got, want in ((dx[-3:], wx), (dW, ww), (db, wb)):
+        tt._close(got, want)
+
+
 # ------------------------------------------------------------------ optimiser
 
 def test_adamw_8_parameter_to_the_bit(gpu):

@@ -117,6 +117,9 @@ def test_sizes_that_no_launch_holds():
         for M in (40_000_003, 140_000_003, 400_000_000):
             assert lib.vc_linear_workspace(k, M, 8, 8) >= 0
             assert lib.vc_linear_backward_workspace(k, M, 8, 8, 0, 7) >= 0
-    assert lib.vc_linear_backward_workspace(1, top, 8, 8, 2, 7) < 0  # sums over 2 M lines
+    for need in (1, 2, 7):
+        assert lib.vc_linear_backward_workspace(1, 1 << 29, 8, 8, 2, need) < 0
+        assert lib.vc_linear_backward_workspace(1, (1 << 29) - 512, 8, 8, 2, need) > 0
+    assert lib.vc_linear_backward_workspace(1, top, 8, 8, 2, 4) > 0  # db alone has no product
     with pytest.raises(NotImplementedError):
         _lib.call('vc_linear', 1, P, top, 64, 64, P, 1 << 30, None, 0, None, 0, P, None, None, 0, None)

@@ -1089,7 +1089,8 @@ BackwardPlan make_backward(int type, int64_t M, int K, int N, int act, int need)
   const int64_t np = up8(N), times = p.two ? 2 : 1;
   Job job[2];
   Cut c[2] = {};
-  // for both products, whichever are asked for: the same bits either way
+  // for both products, whichever are asked for: the same bits either way.  M and N are
+  // rows of a product: below 2^29 where a cut fits, so sums twice as long stay within 32 bits
   job[0] = {N, K, times * M};
   job[1] = {M, K, p.two ? 2 * np : N};
   if (need & 3) {
@@ -1253,9 +1254,7 @@ bool known(int type, int act) {
   return (type == VC_FP32 || type == VC_BF16) && act >= kNone && act <= kSilu;
 }
 bool backward_ok(int type, int64_t M, int K, int N, int act) {
-  if (!known(type, act & ~kRounded) || !sizes_ok(M, K, N)) return false;
-  // sums twice as long are counted in 32 bits
-  return !two_parts(type, act, 3) || (M <= (1 << 30) - 8 && N <= (1 << 29));
+  return known(type, act & ~kRounded) && sizes_ok(M, K, N);
 }
 
 }  // namespace
