@@ -16,7 +16,8 @@
 // Rounded to nearest instead, v would stand still after a few steps: with b2 =
 // 0.999 one changes u by at most 1/2000 of it in the long run, the grid's step
 // is 1/8 to 1/16.  u has half of v's octaves, and one that is positive is never
-// stored as zero, so that m / (u + eps) stays bounded.
+// stored as zero, so that m / (u + eps) stays bounded (a block that is all below 2^-100
+// is: the square of such a gradient is below fp32's smallest value).
 #include "vc_common.h"
 
 namespace {
